@@ -361,6 +361,120 @@ int mg_adam_step(float* master, const float* grad, float* momentum, float* varia
 /* Column means of the [rows][5] loss statistics (model/ppo.h:925-943). */
 int mg_stats_mean(const float* stats, int rows, float* out5, mg_stream_t stream);
 
+/* ---------------------------------------------------------------- controlled logits */
+
+/* Element types of the calls that take more than one. */
+enum mg_dtype { MG_DTYPE_F32 = 0, MG_DTYPE_BF16 = 1, MG_DTYPE_F16 = 2 };
+
+/* Controls on the logits of `actions` actions (no counterpart in the
+ * reference, whose policies take every action of their head). Row r, action
+ * a, raw logit x, n = how often a occurs in the row's history:
+ *   n > 0:  x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *           x = (x - frequency[r] * n) - presence[r]
+ *   x = x + bias[a]
+ *   a not allowed by the mask: x = -inf, whatever x was (NaN and infinities
+ *   in masked places have no effect)
+ * in fp32, each operation rounded once. Every pointer is device memory and
+ * may be NULL: that control is then left out. repetition must be positive.
+ * The struct itself is host memory, read during the call. */
+typedef struct mg_logit_controls {
+    const uint32_t* mask;       /* [rows][mask_stride]: bit a % 32 of word a / 32 set = action a allowed */
+    int64_t mask_stride;        /* words from one row to the next; 0: one mask for every row */
+    const float* bias;          /* [rows][bias_stride] */
+    int64_t bias_stride;        /* elements from one row to the next; 0: one bias for every row */
+    const int32_t* history;     /* [rows][history_stride]: earlier actions; entries outside [0, actions) do not count */
+    int64_t history_stride;
+    const int32_t* history_len; /* [rows]: entries of each row (taken into [0, history_max]); NULL: history_max each */
+    int history_max;            /* the most entries a row has, at most MG_LOGITS_MAX_HISTORY */
+    const float* repetition;    /* [rows]; NULL: 1 */
+    const float* frequency;     /* [rows]; NULL: 0 */
+    const float* presence;      /* [rows]; NULL: 0 */
+} mg_logit_controls;
+#define MG_LOGITS_MAX_ACTIONS (1 << 18)
+#define MG_LOGITS_MAX_HISTORY (1 << 14)
+
+/* out[r][a] = controlled logit, in the logits' type. logits [rows][ld] and out
+ * [rows][ldo] of `dtype` (mg_dtype); columns from `actions` on are neither
+ * read nor written. controls may be NULL (a copy). out may be logits itself
+ * (then ldo = ld); any other overlap is not allowed. */
+int mg_logits_control(const void* logits, int dtype, int64_t ld, const mg_logit_controls* controls, void* out,
+                      int64_t ldo, int rows, int actions, mg_stream_t stream);
+/* Its gradient with respect to the raw logits: d_logits = d_out times the
+ * repetition factor (1 / repetition for a raw logit > 0, else repetition,
+ * where the action occurred) and 0 where the mask leaves the action out. The
+ * raw logits give the sign (read only where a repetition penalty applies: not
+ * the controlled ones of an in-place call). d_logits may be d_out itself. */
+int mg_logits_control_backward(const void* logits, int dtype, int64_t ld, const mg_logit_controls* controls,
+                               const void* d_out, int64_t ldg, void* d_logits, int64_t ldd, int rows, int actions,
+                               mg_stream_t stream);
+/* An action per row drawn from the softmax of the controlled logits, its
+ * log-probability, the entropy of the row (nullable) and the value in column
+ * `actions` of the row (nullable; needs ld > actions), as
+ * mg_sample_categorical gives them from a 64-column head. rng[r] advances by
+ * one xorshift step to w; action a then has the time
+ *   E_a = -log(1 - (mix32(w + a * 0x9E3779B9) + 1/2) / 2^32)   (mg_mix32)
+ * and the action with the largest l_a - log E_a is drawn: exponential clocks
+ * of rates e^l, the first of which rings in a with the softmax's
+ * probability, and the draw of a row does not depend on how it is split over
+ * threads. rng NULL: the largest controlled logit. Equal ones: the lowest
+ * index. A row without an allowed action gets action -1, log-probability 0
+ * and entropy 0. A NaN at an allowed action is never drawn and makes the
+ * row's log-probability and entropy NaN. */
+int mg_logits_sample(const void* logits, int dtype, int64_t ld, const mg_logit_controls* controls, uint32_t* rng,
+                     int32_t* action, float* log_prob, float* entropy, float* value, int rows, int actions,
+                     mg_stream_t stream);
+/* mg_policy_loss over controlled logits: the clipped PPO loss of every row
+ * with its gradient with respect to the raw logits, d_logits [rows][ldd] in
+ * the logits' type, times grad_scale (1 / rows gives mg_policy_loss's mean);
+ * stats [rows][5] = policy, value, entropy, approx-KL, clipped. With ret (nullable)
+ * column `actions` of a row is its value: the value loss joins the statistics
+ * and its gradient goes to column `actions` of d_logits (ld, ldd > actions).
+ * Other columns of d_logits are left as they were. adv_stats as in
+ * mg_policy_loss. A row whose action is -1 (padding, or drawn from a row that
+ * allowed nothing) or not allowed by the mask gets zeros in its gradient and
+ * its statistics; any other action outside [0, actions) does too, and is
+ * recorded in the device status word. d_logits may be logits itself (then
+ * ldd = ld). */
+int mg_logits_policy_loss(const void* logits, int dtype, int64_t ld, const mg_logit_controls* controls,
+                          const int32_t* action, const float* adv, const float* adv_stats, const float* ret,
+                          const float* old_log_prob, void* d_logits, int64_t ldd, float* stats, int rows, int actions,
+                          float clip, float value_coef, float entropy_coef, float grad_scale, mg_stream_t stream);
+
+/* ---------------------------------------------------------------- orthogonalised updates */
+
+/* Bytes of the workspace that mg_orthogonalize and mg_muon_step need for
+ * `batch` matrices of rows x cols. One workspace serves one call at a time:
+ * calls that may overlap on the GPU (two streams, two captured graphs) need
+ * one each. */
+int mg_muon_workspace(int batch, int rows, int cols, size_t* bytes);
+/* out = the matrix of x brought near the closest matrix with orthonormal rows
+ * (rows <= cols) or columns, by `steps` (1..16) Newton-Schulz steps: X = x /
+ * |x|_F, then G = X X^T (or X^T X, the smaller), X = 3.4445 X + (-4.7750 G +
+ * 2.0315 G^2) X, which takes singular values into about [0.7, 1.2]; 5 steps
+ * do for the Muon update. x [batch][rows][ld] of `dtype`, batch_stride
+ * elements apart; out likewise with ldo, out_stride, of out_dtype
+ * MG_DTYPE_BF16 or MG_DTYPE_F16: the products take fp16 operands, X stays
+ * fp32 (measured 0.03 to 0.3 % of the result's norm off the exact iteration). A zero
+ * matrix gives zeros. x and out must not overlap. workspace: device memory of
+ * mg_muon_workspace bytes, 16-byte aligned. */
+int mg_orthogonalize(const void* x, int dtype, int64_t ld, int64_t batch_stride, void* out, int out_dtype, int64_t ldo,
+                     int64_t out_stride, int batch, int rows, int cols, int steps, void* workspace,
+                     size_t workspace_bytes, mg_stream_t stream);
+/* The Muon optimiser step of `batch` matrices of rows x cols (dense rows,
+ * batch_stride elements apart), beside mg_adam_step: g = grad times the
+ * global-norm clip factor of mg_adam_step (norm_partial as there; NULL with 0
+ * partials, or max_grad_norm 0: no clip), momentum = momentum_decay *
+ * momentum + g, u = nesterov ? g + momentum_decay * momentum : momentum, O =
+ * mg_orthogonalize's result of u in fp32, master = master (1 - lr
+ * weight_decay) - lr scale O, and the bf16 weights. scale is the factor by
+ * the matrix's shape that a program uses (0.2 sqrt(max(rows, cols)) gives
+ * updates of Adam's size). The squared norm is stored to norm_sq_out
+ * (nullable; needs norm_partial). Workspace as above. */
+int mg_muon_step(float* master, const float* grad, float* momentum, void* weights, int64_t batch_stride, int batch,
+                 int rows, int cols, const float* norm_partial, int n_norm_partials, float max_grad_norm, float lr,
+                 float scale, float momentum_decay, int nesterov, float weight_decay, int steps, float* norm_sq_out,
+                 void* workspace, size_t workspace_bytes, mg_stream_t stream);
+
 /* ---------------------------------------------------------------- sessions */
 
 /* A gym session: the env buffers of gym.h:15-121 on one device, with its

@@ -77,6 +77,15 @@ class CollectFusedArgs(ctypes.Structure):
                 ("lambda_", ctypes.c_float)]
 
 
+class LogitControls(ctypes.Structure):
+    """Layout of mg_logit_controls (include/metalgym_b200.h): device pointers, None leaves a control out."""
+
+    _fields_ = [("mask", ctypes.c_void_p), ("mask_stride", ctypes.c_int64), ("bias", ctypes.c_void_p),
+                ("bias_stride", ctypes.c_int64), ("history", ctypes.c_void_p), ("history_stride", ctypes.c_int64),
+                ("history_len", ctypes.c_void_p), ("history_max", ctypes.c_int), ("repetition", ctypes.c_void_p),
+                ("frequency", ctypes.c_void_p), ("presence", ctypes.c_void_p)]
+
+
 def _env_ops_info(name: str) -> dict:
     """Sizes and dims of a registered environment."""
     p = lib().mg_env_find(name.encode())

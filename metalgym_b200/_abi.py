@@ -10,6 +10,7 @@ I = C.c_int
 U = C.c_uint32
 F = C.c_float
 U64 = C.c_uint64
+I64 = C.c_int64
 S = C.c_char_p
 PI = C.POINTER(C.c_int)
 PF = C.POINTER(C.c_float)
@@ -60,6 +61,15 @@ SIGNATURES = {
     "mg_reduce_partials_num_norm_partials": (I, [C.c_int64]),
     "mg_adam_step": (I, [P, P, P, P, P, P, I, C.c_int64, F, F, F, F, P, P]),
     "mg_stats_mean": (I, [P, I, P, P]),
+    # controlled logits
+    "mg_logits_control": (I, [P, I, I64, P, P, I64, I, I, P]),
+    "mg_logits_control_backward": (I, [P, I, I64, P, P, I64, P, I64, I, I, P]),
+    "mg_logits_sample": (I, [P, I, I64, P, P, P, P, P, P, I, I, P]),
+    "mg_logits_policy_loss": (I, [P, I, I64, P, P, P, P, P, P, P, I64, P, I, I, F, F, F, F, P]),
+    # orthogonalised updates
+    "mg_muon_workspace": (I, [I, I, I, C.POINTER(C.c_size_t)]),
+    "mg_orthogonalize": (I, [P, I, I64, I64, P, I, I64, I64, I, I, I, I, P, C.c_size_t, P]),
+    "mg_muon_step": (I, [P, P, P, P, I64, I, I, I, P, I, F, F, F, F, I, F, I, P, P, C.c_size_t, P]),
     # sessions
     "mg_gym_create": (I, [S, I, U, U, I, C.POINTER(P)]),
     "mg_gym_destroy": (I, [P]),

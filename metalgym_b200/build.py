@@ -42,6 +42,8 @@ SOURCES: dict[str, list[str]] = {
     "engine.cu": [],
     "capi_session.cu": [],
     "noalloc.cu": [],
+    "logits.cu": [],
+    "muon.cu": [],
 }
 
 

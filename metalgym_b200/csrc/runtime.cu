@@ -181,6 +181,23 @@ int make_tmap_bf16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t 
     return MG_OK;
 }
 
+int make_tmap_f16_3d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t batch,
+                     uint64_t row_stride, uint32_t box_outer) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(MG_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    if ((reinterpret_cast<uintptr_t>(base) & 15) != 0) return fail(MG_ERR_ARGUMENT, "TMA base not 16-byte aligned");
+    if ((row_stride * 2) % 16 != 0) return fail(MG_ERR_ARGUMENT, "TMA row stride not a multiple of 16 bytes");
+    cuuint64_t dims[3] = {inner, outer, batch};
+    cuuint64_t strides[2] = {row_stride * 2, outer * row_stride * 2};
+    cuuint32_t box[3] = {64, box_outer, 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(MG_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+    return MG_OK;
+}
+
 int check_launch(const char* what) {
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, what);

@@ -77,6 +77,12 @@ int num_sms();
 int make_tmap_bf16(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride,
                    uint32_t box_outer);
 
+// 3D fp16 tensor map of `batch` dense matrices of `outer` rows (row_stride
+// elements apart), 128-byte swizzle, box of 64 x box_outer of one matrix;
+// reads past a matrix's rows or columns give zeros.
+int make_tmap_f16_3d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t batch,
+                     uint64_t row_stride, uint32_t box_outer);
+
 // Last launch error check (cudaGetLastError) with a message.
 int check_launch(const char* what);
 
