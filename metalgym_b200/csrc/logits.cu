@@ -2,8 +2,10 @@
 // out, differentiated, drawn from, and under the clipped PPO loss.
 #include <math.h>
 
+#include <algorithm>
 #include <atomic>
 #include <string>
+#include <utility>
 
 #include "logits.cuh"
 #include "runtime.h"
@@ -15,8 +17,51 @@
 namespace mg {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+// A team reads one row, or one part of it: a warp (eight rows a CTA) up to
+// kWarpActions actions, else a CTA of NT threads, with the row's parts in the
+// CTAs of a cluster where rows are few or so long that the rows being read
+// would not stay in L2 for the loss's second pass.
+constexpr int kWarpActions = 1024;
+constexpr int kWarpRows = 8;  // rows of a CTA of warp teams
+
+template <int NT>
+constexpr int kCtaThreads = NT == 32 ? 32 * kWarpRows : NT;
+template <int NT>
+constexpr int kTeamWarps = NT / 32;
+
+struct TeamPart {
+    int rows, actions;
+    int span;        // actions of a CTA (a multiple of 256, or all of them)
+    int parts;       // CTAs of a row
+    int tableBytes;  // shared memory of a team's history table
+};
+
+// The team's row and its part [lo, hi); false: no row.
+template <int NT>
+__device__ __forceinline__ bool team_part(const TeamPart& p, int& row, int& lo, int& hi) {
+    if (NT == 32) {
+        row = blockIdx.x * kWarpRows + (threadIdx.x >> 5);
+        lo = 0;
+        hi = p.actions;
+        return row < p.rows;
+    }
+    row = blockIdx.x / p.parts;
+    lo = min(p.actions, (int)(blockIdx.x % p.parts) * p.span);
+    hi = min(p.actions, lo + p.span);
+    return true;
+}
+
+template <int NT>
+__device__ __forceinline__ int team_rank() {
+    return NT == 32 ? threadIdx.x & 31 : threadIdx.x;
+}
+
+template <int NT>
+__device__ __forceinline__ HistoryTable team_table(const TeamPart& p, const mg_logit_controls& c, uint32_t* smem) {
+    HistoryTable t;
+    t.place(smem + (NT == 32 ? (threadIdx.x >> 5) * (p.tableBytes / 4) : 0), p.span, c.history_max);
+    return t;
+}
 
 // The controlled logit of action a (raw x); the table covers actions from lo.
 __device__ __forceinline__ float controlled(const RowControls& r, const HistoryTable& t, float x, int a, int lo) {
@@ -30,56 +75,118 @@ __device__ __forceinline__ float controlled(const RowControls& r, const HistoryT
 
 // ------------------------------------------------------------------ control and its gradient
 
-// One CTA per chunk of `span` actions of a row: in dimension x, row-major.
-template <class T, bool BACKWARD>
-__global__ void __launch_bounds__(kThreads)
+// Groups of a thread in flight together.
+constexpr int kControlGroups = 4;
+
+template <class T, int NT, bool BACKWARD>
+__global__ void __launch_bounds__(kCtaThreads<NT>)
     k_logits_control(const T* logits, int64_t ld, const mg_logit_controls c, const T* dOut, int64_t ldg, T* out,
-                     int64_t ldo, int actions, int span, int chunks) {
+                     int64_t ldo, const TeamPart part) {
+    constexpr int VE = kGroup<T>, U = kControlGroups;
     mg_pdl_trigger();
     mg_pdl_wait();
     extern __shared__ uint32_t smem[];
-    __shared__ uint32_t sums[kWarps];
-    const int row = blockIdx.x / chunks, lo = (blockIdx.x % chunks) * span, hi = min(actions, lo + span);
+    __shared__ uint32_t sums[kTeamWarps<NT>];
+    int row, lo, hi;
+    if (!team_part<NT>(part, row, lo, hi)) return;
     const RowControls r = row_controls(c, row);
-    HistoryTable t;
-    t.place(smem, span, c.history_max);
-    if (r.history)
-        history_fill(t, c.history + (int64_t)row * c.history_stride, row_history_len(c, row), lo, hi, c.history_max, sums);
+    const HistoryTable t = team_table<NT>(part, c, smem);
     const T* x = logits + (int64_t)row * ld;
+    const T* src = BACKWARD ? dOut + (int64_t)row * ldg : x;
     T* y = out + (int64_t)row * ldo;
-    for (int a = lo + threadIdx.x; a < hi; a += kThreads) {
-        if (!BACKWARD) {
-            from_f32(&y[a], controlled(r, t, to_f32(x[a]), a, lo));
-        } else {
-            float g = to_f32(dOut[(int64_t)row * ldg + a]);
-            if (r.history && t.count(a - lo) > 0)
-                g = to_f32(x[a]) > 0.0f ? __fdiv_rn(g, r.repetition) : __fmul_rn(g, r.repetition);
-            from_f32(&y[a], allowed(r, a) ? g : 0.0f);
+    const bool vec = same_alignment(src, y);
+    const int start = group_start(src, lo), groups = group_count<T>(start, hi), tid = team_rank<NT>();
+    bool filled = !r.history;
+    for (int g0 = 0; g0 < groups || !filled; g0 += NT * U) {
+        RawGroup<T> raw[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int a = start + (g0 + u * NT + tid) * VE;
+            raw[u] = group_load(src, a, group_valid<T>(a, lo, hi));
+        }
+        if (!filled) {  // while the first loads are in flight
+            history_fill<NT>(t, c.history + (int64_t)row * c.history_stride, row_history_len(c, row), lo, hi, c.history_max, sums);
+            filled = true;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int a = start + (g0 + u * NT + tid) * VE;
+            const uint32_t valid = group_valid<T>(a, lo, hi);
+            if (!valid) continue;
+            float v[VE];
+            if (!BACKWARD) {
+                group_control(r, t, raw[u], a, lo, valid, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VE; i++) v[i] = raw_value(raw[u], i);
+                if (r.history) {
+                    // the raw logits' signs, read only for groups that hold an action that occurred
+                    uint32_t seen = 0;
+#pragma unroll
+                    for (int i = 0; i < VE; i++)
+                        if ((valid >> i) & 1u) {
+                            const int k = a - lo + i;
+                            seen |= ((t.seen[k >> 5] >> (k & 31)) & 1u) << i;
+                        }
+                    if (seen) {
+#pragma unroll
+                        for (int i = 0; i < VE; i++)
+                            if ((seen >> i) & 1u)
+                                v[i] = to_f32(x[a + i]) > 0.0f ? __fdiv_rn(v[i], r.repetition) : __fmul_rn(v[i], r.repetition);
+                    }
+                }
+                if (r.mask) {
+#pragma unroll
+                    for (int i = 0; i < VE; i++)
+                        if (((valid >> i) & 1u) && !allowed(r, a + i)) v[i] = 0.0f;
+                }
+            }
+            group_store(y, a, valid, vec, v);
         }
     }
 }
 
 // ------------------------------------------------------------------ softmax statistics and the race
 
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_fast(float x) {  // within 2 ulp; results below 2^-126 are 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+// The largest of a warp's values (NaN ignored).
+__device__ __forceinline__ float warp_max(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Running softmax statistics: the maximum m, s = sum e^(l - m), t = sum
-// e^(l - m) (l - m); entropy = log s - t / s.
+// e^(l - m) (l - m); entropy = log s - t / s. In the passes m is the same in
+// the threads of a warp, s and t are a thread's.
 struct Softmax {
     float m = -INFINITY, s = 0.0f, t = 0.0f;
-    __device__ __forceinline__ void add(float l) {
-        if (l == -INFINITY) return;
-        if (l > m) {
-            if (m > -INFINITY) {
-                const float d = m - l, e = expf(d);
-                t = e * (t + s * d);
-                s = s * e;
-            }
-            m = l;
-            s += 1.0f;
-        } else {
-            const float d = l - m, e = expf(d);  // NaN when l is
-            s += e;
-            if (!(e == 0.0f)) t += e * d;
-        }
+    // Raises m (a whole warp) and returns the factor that carried s over.
+    __device__ __forceinline__ float raise(float top) {
+        const float d = m - top, e = m > -INFINITY ? exp2_fast(d * kLog2e) : 0.0f;
+        t = e > 0.0f ? e * (t + s * d) : 0.0f;
+        if (!(s != s)) s = s * e;
+        m = top;
+        return e;
+    }
+    // e^(l - m) of one logit, added to the sums; m > -inf. The difference is
+    // kept finite so that e^(..) = 0 times it is 0 (a NaN stays one).
+    __device__ __forceinline__ float add(float l) {
+        const float d = max_nan(l - m, -1e30f), e = exp2_fast(d * kLog2e);
+        s += e;
+        t = fmaf(e, d, t);
+        return e;
     }
     __device__ __forceinline__ void merge(const Softmax& o) {
         if (o.m == -INFINITY && o.s == 0.0f) return;
@@ -96,97 +203,212 @@ struct Softmax {
     }
 };
 
-// The best key of a race and its action; equal keys: the lower action.
-struct Best {
-    double key = -INFINITY;
-    int action = -1;
-    float logit = -INFINITY;
-    __device__ __forceinline__ void offer(double k, int a, float l) {
-        if (k > key || (k == key && a < action)) {
-            key = k;
-            action = a;
-            logit = l;
-        }
+// Adds a group's logits (-inf: not allowed) to a warp's statistics. `raised` is
+// told when m rises; each(i, e) gets every element's e^(l - m).
+template <int VE, class Raised, class Each>
+__device__ __forceinline__ void softmax_group(Softmax& v, const float* x, Raised raised, Each each) {
+    float top = x[0];
+#pragma unroll
+    for (int i = 1; i < VE; i++) top = fmaxf(top, x[i]);
+    top = warp_max(top);
+    if (top > v.m) raised(v.raise(top));
+    if (v.m == -INFINITY) {  // nothing allowed so far: a NaN still shows
+#pragma unroll
+        for (int i = 0; i < VE; i++)
+            if (x[i] != x[i]) v.s = x[i];
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < VE; i++) each(i, v.add(x[i]));
+}
+
+__device__ __forceinline__ uint32_t race_bits(uint32_t word, int a) { return mg_mix32(word + (uint32_t)a * 0x9E3779B9u); }
+__device__ __forceinline__ double race_key(uint32_t h, float l) {
+    return (double)l - log(-log1p(-((double)h + 0.5) * (1.0 / 4294967296.0)));
+}
+
+// A runner of the race: its key in 32 bits, and what gives the key in 64.
+struct Runner {
+    float key = -INFINITY, logit = -INFINITY;
+    uint32_t bits = 0;
+    int action = -1;
 };
 
-__device__ __forceinline__ double race_time(uint32_t word, int a) {
-    const uint32_t h = mg_mix32(word + (uint32_t)a * 0x9E3779B9u);
-    return -log1p(-((double)h + 0.5) * (1.0 / 4294967296.0));
+// Whether a's key is above b's (equal keys: the lower action). 32 bits decide
+// where they can: both keys are good to about 2^-21 of their size.
+template <bool GREEDY>
+__device__ __forceinline__ bool beats(const Runner& a, const Runner& b) {
+    if (a.action < 0 || b.action < 0) return a.action >= 0;
+    if (GREEDY) return a.logit > b.logit || (a.logit == b.logit && a.action < b.action);
+    const float d = a.key - b.key, margin = 1e-4f * (1.0f + fabsf(b.key));
+    if (d > margin) return true;
+    if (d < -margin) return false;
+    const double ka = race_key(a.bits, a.logit), kb = race_key(b.bits, b.logit);
+    return ka > kb || (ka == kb && a.action < b.action);
 }
 
-template <class V>
-__device__ __forceinline__ V warp_xor(V v, int d) {
-    return __shfl_xor_sync(0xffffffffu, v, d);
-}
-__device__ __forceinline__ Softmax shuffle(const Softmax& a, int d) {
-    Softmax o;
-    o.m = warp_xor(a.m, d);
-    o.s = warp_xor(a.s, d);
-    o.t = warp_xor(a.t, d);
-    return o;
-}
+// What the CTAs of a row tell each other.
+struct RowPart {
+    Softmax v;
+    Runner best;
+    float chosen;
+};
 
-// The CTA's statistics in every thread, merged in one fixed order.
-__device__ inline Softmax block_softmax(Softmax v, Softmax* slot) {
+__device__ __forceinline__ float warp_add(float x) {
 #pragma unroll
-    for (int d = 16; d; d >>= 1) v.merge(shuffle(v, d));
-    if ((threadIdx.x & 31) == 0) slot[threadIdx.x >> 5] = v;
+    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+}
+
+// The `rank`-th CTA's copy of a shared variable (distributed shared memory).
+template <class V>
+__device__ __forceinline__ const V* cluster_peer(const V* local, int rank) {
+    uint64_t remote;
+    asm("mapa.u64 %0, %1, %2;" : "=l"(remote) : "l"(reinterpret_cast<uint64_t>(local)), "r"(rank));
+    return reinterpret_cast<const V*>(remote);
+}
+
+// The row's statistics (and best runner) in every thread of its CTAs, merged in
+// one fixed order: lanes, warps, CTAs. With several parts the caller ends with
+// cluster_sync, so that no CTA leaves while another reads its part.
+template <int NT, bool RACE, bool GREEDY>
+__device__ inline void row_merge(RowPart& mine, RowPart* warps, RowPart* whole, int parts, int chosenRank) {
+    mine.v.s = warp_add(mine.v.s);
+    mine.v.t = warp_add(mine.v.t);
+    if (RACE) {
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            Runner o;
+            o.key = __shfl_xor_sync(0xffffffffu, mine.best.key, d);
+            o.logit = __shfl_xor_sync(0xffffffffu, mine.best.logit, d);
+            o.bits = __shfl_xor_sync(0xffffffffu, mine.best.bits, d);
+            o.action = __shfl_xor_sync(0xffffffffu, mine.best.action, d);
+            if (beats<GREEDY>(o, mine.best)) mine.best = o;
+        }
+    }
+    if (NT == 32) return;
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = mine;
     __syncthreads();
-    Softmax all = slot[0];
-    for (int w = 1; w < kWarps; w++) all.merge(slot[w]);
-    return all;
+    auto join = [&](RowPart& all, const RowPart& o) {
+        all.v.merge(o.v);
+        if (RACE && beats<GREEDY>(o.best, all.best)) all.best = o.best;
+    };
+    if (threadIdx.x == 0) {
+        RowPart all = warps[0];
+        for (int w = 1; w < kTeamWarps<NT>; w++) join(all, warps[w]);
+        *whole = all;
+    }
+    if (parts == 1) {
+        __syncthreads();
+        mine = *whole;
+        return;
+    }
+    cluster_sync();
+    RowPart all = *cluster_peer(whole, 0);
+    for (int k = 1; k < parts; k++) join(all, *cluster_peer(whole, k));
+    if (!RACE) all.chosen = cluster_peer(whole, chosenRank)->chosen;
+    mine = all;
 }
 
 // ------------------------------------------------------------------ draw
 
-// One CTA per row.
-template <class T>
-__global__ void __launch_bounds__(kThreads)
+// One pass. An action a can win only where its time E_a >= v_a = (h + 1/2) /
+// 2^32 is below the best ratio E / e^(l - m) so far times its own e^(l - m):
+// the test takes the upper bits of h as a number of [1, 2) against 1 + that
+// bound (a millionth more than it, so that rounding never hides a winner), and
+// only the few that pass take logarithms.
+template <class T, int NT, bool GREEDY>
+__global__ void __launch_bounds__(kCtaThreads<NT>)
     k_logits_sample(const T* logits, int64_t ld, const mg_logit_controls c, uint32_t* rng, int32_t* action,
-                    float* logProb, float* entropy, float* value, int actions) {
+                    float* logProb, float* entropy, float* value, const TeamPart part) {
+    constexpr int VE = kGroup<T>;
     mg_pdl_trigger();
     mg_pdl_wait();
     extern __shared__ uint32_t smem[];
-    __shared__ uint32_t sums[kWarps];
-    __shared__ Softmax stats[kWarps];
-    __shared__ Best best[kWarps];
-    const int row = blockIdx.x;
+    __shared__ uint32_t sums[kTeamWarps<NT>];
+    __shared__ __align__(8) unsigned char slots[(kTeamWarps<NT> + 1) * sizeof(RowPart)];
+    RowPart* warps = reinterpret_cast<RowPart*>(slots);
+    RowPart* whole = warps + kTeamWarps<NT>;
+    int row, lo, hi;
+    if (!team_part<NT>(part, row, lo, hi)) return;
     const RowControls r = row_controls(c, row);
-    HistoryTable t;
-    t.place(smem, actions, c.history_max);
+    const HistoryTable t = team_table<NT>(part, c, smem);
     if (r.history)
-        history_fill(t, c.history + (int64_t)row * c.history_stride, row_history_len(c, row), 0, actions, c.history_max, sums);
+        history_fill<NT>(t, c.history + (int64_t)row * c.history_stride, row_history_len(c, row), lo, hi, c.history_max, sums);
     const T* x = logits + (int64_t)row * ld;
-    uint32_t word = rng ? rng[row] : 0u;
-    if (rng) rngNext(word);
-    Softmax v;
-    Best b;
-    for (int a = threadIdx.x; a < actions; a += kThreads) {
-        const float l = controlled(r, t, to_f32(x[a]), a, 0);
-        v.add(l);
-        if (l > -INFINITY) b.offer(rng ? (double)l - log(race_time(word, a)) : (double)l, a, l);
-    }
+    uint32_t word = GREEDY ? 0u : rng[row];
+    if (!GREEDY) rngNext(word);
+    RowPart mine;
+    float bound = 3e38f;  // the warp's best ratio E / e^(l - m)
+    const int start = group_start(x, lo), groups = group_count<T>(start, hi), tid = team_rank<NT>();
+    const int rounds = (groups + NT - 1) / NT;
+    for (int k = 0; k < rounds; k++) {
+        const int a = start + (k * NT + tid) * VE;
+        const uint32_t valid = group_valid<T>(a, lo, hi);
+        float l[VE], e[VE];
+        const RawGroup<T> raw = group_load(x, a, valid);
+        if (valid) {
+            group_control(r, t, raw, a, lo, valid, l);
+        } else {
 #pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        const double k = warp_xor(b.key, d);
-        const int a = warp_xor(b.action, d);
-        const float l = warp_xor(b.logit, d);
-        if (a >= 0) b.offer(k, a, l);
+            for (int i = 0; i < VE; i++) l[i] = -INFINITY;
+        }
+        bool live = false;
+        softmax_group<VE>(
+            mine.v, l, [&](float f) { bound = f > 0.0f ? fminf(bound / f, 3e38f) : 3e38f; },
+            [&](int i, float v) {
+                e[i] = v;
+                live = true;
+            });
+        if (!live) continue;  // the whole warp: m is the warp's
+        if (GREEDY) {
+#pragma unroll
+            for (int i = 0; i < VE; i++)
+                if (l[i] > mine.best.logit) {
+                    mine.best.logit = l[i];
+                    mine.best.action = a + i;
+                }
+            continue;
+        }
+        uint32_t pass = 0;
+        const float limit = bound * 1.0001f;
+#pragma unroll
+        for (int i = 0; i < VE; i++) {
+            const uint32_t h = race_bits(word, a + i);
+            const float f = __uint_as_float((h >> 9) | 0x3f800000u);
+            if (f <= fmaf(limit, e[i], 1.0f)) pass |= 1u << i;
+        }
+        if (__any_sync(0xffffffffu, pass != 0)) {
+            float least = 3e38f;
+#pragma unroll
+            for (int i = 0; i < VE; i++)
+                if (((pass >> i) & 1u) && l[i] > -INFINITY) {
+                    const uint32_t h = race_bits(word, a + i);
+                    // -log(1 - v) from whichever of v and 1 - v is small
+                    const float time = h < 0x80000000u ? -log1pf(-((float)h + 0.5f) * 2.3283064e-10f)
+                                                       : -logf(((float)(~h) + 0.5f) * 2.3283064e-10f);
+                    Runner o;
+                    o.key = l[i] - logf(time);
+                    o.logit = l[i];
+                    o.bits = h;
+                    o.action = a + i;
+                    if (beats<false>(o, mine.best)) mine.best = o;
+                    least = fminf(least, time / e[i]);
+                }
+            bound = fminf(bound, __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least))));
+        }
     }
-    if ((threadIdx.x & 31) == 0) best[threadIdx.x >> 5] = b;
-    const Softmax all = block_softmax(v, stats);
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kWarps; w++)
-            if (best[w].action >= 0) b.offer(best[w].key, best[w].action, best[w].logit);
-        const float ls = logf(all.s);
-        const bool some = b.action >= 0 || all.s != all.s;
-        action[row] = b.action;
-        logProb[row] = some ? (b.logit - all.m) - ls : 0.0f;
-        if (entropy) entropy[row] = some ? ls - all.t / all.s : 0.0f;
-        if (value) value[row] = to_f32(x[actions]);
-        if (rng) rng[row] = word;
+    row_merge<NT, true, GREEDY>(mine, warps, whole, part.parts, 0);
+    if (tid == 0 && lo == 0) {
+        const float ls = logf(mine.v.s);
+        const bool some = mine.best.action >= 0 || mine.v.s != mine.v.s;
+        action[row] = mine.best.action;
+        logProb[row] = some ? (mine.best.logit - mine.v.m) - ls : 0.0f;
+        if (entropy) entropy[row] = some ? ls - mine.v.t / mine.v.s : 0.0f;
+        if (value) value[row] = to_f32(x[part.actions]);
+        if (!GREEDY) rng[row] = word;
     }
+    if (NT > 32 && part.parts > 1) cluster_sync();
 }
 
 // ------------------------------------------------------------------ loss
@@ -199,60 +421,99 @@ struct LossArgs {
     int* status;
 };
 
-// One CTA per row: the row's statistics, then its gradient.
-template <class T>
-__global__ void __launch_bounds__(kThreads)
-    k_logits_loss(const T* logits, int64_t ld, const mg_logit_controls c, T* dLogits, int64_t ldd, int actions,
+// The row's statistics in one pass, its gradient in a second one that reads the
+// row again, from L2.
+template <class T, int NT>
+__global__ void __launch_bounds__(kCtaThreads<NT>)
+    k_logits_loss(const T* logits, int64_t ld, const mg_logit_controls c, T* dLogits, int64_t ldd, const TeamPart part,
                   const LossArgs L) {
+    constexpr int VE = kGroup<T>;
     mg_pdl_trigger();
     mg_pdl_wait();
     extern __shared__ uint32_t smem[];
-    __shared__ uint32_t sums[kWarps];
-    __shared__ Softmax slot[kWarps];
-    const int row = blockIdx.x;
+    __shared__ uint32_t sums[kTeamWarps<NT>];
+    __shared__ __align__(8) unsigned char slots[(kTeamWarps<NT> + 1) * sizeof(RowPart)];
+    RowPart* warps = reinterpret_cast<RowPart*>(slots);
+    RowPart* whole = warps + kTeamWarps<NT>;
+    int row, lo, hi;
+    if (!team_part<NT>(part, row, lo, hi)) return;
+    const int actions = part.actions, tid = team_rank<NT>();
     const RowControls r = row_controls(c, row);
-    HistoryTable t;
-    t.place(smem, actions, c.history_max);
+    const HistoryTable t = team_table<NT>(part, c, smem);
     const T* x = logits + (int64_t)row * ld;
     T* d = dLogits + (int64_t)row * ldd;
     const int act = L.action[row];
     const bool inside = act >= 0 && act < actions;
-    if (!inside || !allowed(r, act)) {
-        if (threadIdx.x == 0 && !inside && act != -1) record_error(L.status, kDevBadAction);
-        for (int a = threadIdx.x; a < actions + (L.ret ? 1 : 0); a += kThreads) from_f32(&d[a], 0.0f);
-        if (threadIdx.x < 5) L.stats[(int64_t)row * 5 + threadIdx.x] = 0.0f;
+    if (!inside || !allowed(r, act)) {  // the same for every CTA of the row
+        if (tid == 0 && lo == 0 && !inside && act != -1) record_error(L.status, kDevBadAction);
+        for (int a = lo + tid; a < hi; a += NT) from_f32(&d[a], 0.0f);
+        if (lo == 0 && L.ret && tid == 0) from_f32(&d[actions], 0.0f);
+        if (lo == 0 && tid < 5) L.stats[(int64_t)row * 5 + tid] = 0.0f;
         return;
     }
     if (r.history)
-        history_fill(t, c.history + (int64_t)row * c.history_stride, row_history_len(c, row), 0, actions, c.history_max, sums);
-    const float valueX = L.ret ? to_f32(x[actions]) : 0.0f;
-    const float lAct = controlled(r, t, to_f32(x[act]), act, 0);
-    Softmax v;
-    for (int a = threadIdx.x; a < actions; a += kThreads) v.add(controlled(r, t, to_f32(x[a]), a, 0));
-    const Softmax all = block_softmax(v, slot);
-    const float ls = logf(all.s), entropy = ls - all.t / all.s;
-    const float logp = (lAct - all.m) - ls, old = L.oldLogProb[row];
+        history_fill<NT>(t, c.history + (int64_t)row * c.history_stride, row_history_len(c, row), lo, hi, c.history_max, sums);
+    RowPart mine;
+    mine.chosen = act >= lo && act < hi ? controlled(r, t, to_f32(x[act]), act, lo) : 0.0f;
+    const int start = group_start(x, lo), groups = group_count<T>(start, hi);
+    const int rounds = (groups + NT - 1) / NT;
+    for (int k = 0; k < rounds; k++) {
+        const int a = start + (k * NT + tid) * VE;
+        const uint32_t valid = group_valid<T>(a, lo, hi);
+        float l[VE];
+        const RawGroup<T> raw = group_load(x, a, valid);
+        if (valid) {
+            group_control(r, t, raw, a, lo, valid, l);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VE; i++) l[i] = -INFINITY;
+        }
+        softmax_group<VE>(mine.v, l, [](float) {}, [](int, float) {});
+    }
+    row_merge<NT, false, false>(mine, warps, whole, part.parts, act / part.span);
+    const float ls = logf(mine.v.s), entropy = ls - mine.v.t / mine.v.s;
+    const float logp = (mine.chosen - mine.v.m) - ls, old = L.oldLogProb[row];
     const float ratio = expf(logp - old);
     const float adv = L.advStats ? (L.adv[row] - L.advStats[0]) * L.advStats[1] : L.adv[row];
     const float one = ratio * adv, two = fminf(fmaxf(ratio, 1.0f - L.clip), 1.0f + L.clip) * adv;
     const float slope = one <= two ? -adv * ratio : 0.0f;
-    // every thread has read the action's logit (the gradient may replace it)
-    __syncthreads();
-    for (int a = threadIdx.x; a < actions; a += kThreads) {
-        const float raw = to_f32(x[a]);
-        const float l = controlled(r, t, raw, a, 0);
-        const float lp = (l - all.m) - ls, p = expf(lp);
-        float g = slope * ((a == act ? 1.0f : 0.0f) - p);
-        if (p > 0.0f) g += L.entropyCoef * p * (lp + entropy);
-        g *= L.scale;
-        if (r.history && t.count(a) > 0) g = raw > 0.0f ? __fdiv_rn(g, r.repetition) : g * r.repetition;
-        from_f32(&d[a], allowed(r, a) ? g : 0.0f);
+    // every thread has read the action's logit: the gradient may take its place
+    if (NT == 32)
+        __syncwarp();
+    else if (part.parts > 1)
+        cluster_sync();
+    else
+        __syncthreads();
+    // dl = scale (slope (1[a = act] - p) + ent p (log p + H)) = p (s1 (log p + H) - s0), + s0 at act
+    const float s0 = slope * L.scale, s1 = L.entropyCoef * L.scale;
+    const bool vec = same_alignment(x, d);
+    for (int k = 0; k < rounds; k++) {
+        const int a = start + (k * NT + tid) * VE;
+        const uint32_t valid = group_valid<T>(a, lo, hi);
+        if (!valid) continue;
+        float l[VE], g[VE];
+        const RawGroup<T> raw = group_load(x, a, valid);
+        const GroupControls gc = group_control(r, t, raw, a, lo, valid, l);
+#pragma unroll
+        for (int i = 0; i < VE; i++) {
+            const float lp = max_nan(l[i] - mine.v.m, -1e30f) - ls;
+            const float p = exp2_fast(lp * kLog2e);
+            g[i] = p * fmaf(s1, lp + entropy, -s0);
+            if (a + i == act) g[i] += s0;
+        }
+        group_factor<T>(r, gc, g);
+        if (gc.ok != (1u << VE) - 1u) {  // not allowed: 0, whatever became of a row with a NaN
+#pragma unroll
+            for (int i = 0; i < VE; i++)
+                if (!((gc.ok >> i) & 1u)) g[i] = 0.0f;
+        }
+        group_store(d, a, valid, vec, g);
     }
-    if (threadIdx.x == 0) {
+    if (tid == 0 && lo == 0) {
         float* st = L.stats + (int64_t)row * 5;
         float vLoss = 0.0f;
         if (L.ret) {
-            const float err = valueX - L.ret[row];
+            const float err = to_f32(x[actions]) - L.ret[row];
             vLoss = 0.5f * L.valueCoef * err * err;
             from_f32(&d[actions], L.valueCoef * err * L.scale);
         }
@@ -304,44 +565,123 @@ int check_common(const char* name, const void* logits, int dtype, int64_t ld, co
     return MG_OK;
 }
 
-constexpr int kChunk = 8192;  // actions of a CTA of the control kernels
+// How a call's rows are split over teams.
+TeamPart plan(int nt, int rows, int actions, int parts, int historyMax) {
+    TeamPart p;
+    p.rows = rows;
+    p.actions = actions;
+    p.parts = parts;
+    p.span = nt == 32 || parts == 1 ? actions : ((actions + parts - 1) / parts + 255) / 256 * 256;
+    p.tableBytes = historyMax ? (int)HistoryTable::bytes(p.span, historyMax) : 0;
+    return p;
+}
 
-template <class T, bool BACKWARD>
+template <int NT>
+size_t table_smem(const TeamPart& p) {
+    return (size_t)p.tableBytes * (NT == 32 ? kWarpRows : 1);
+}
+
+constexpr int kTableSmemMax = 100 * 1024;  // >= the largest table, and >= eight of kWarpActions actions
+
+// A launch of rows x parts CTAs (or warp teams), the parts of a row in one cluster.
+template <int NT, class... KArgs, class... Args>
+int launch_rows(void (*kern)(KArgs...), const TeamPart& p, cudaStream_t st, const char* what, Args&&... args) {
+    const int64_t ctas = NT == 32 ? ((int64_t)p.rows + kWarpRows - 1) / kWarpRows : (int64_t)p.rows * p.parts;
+    if (ctas > INT32_MAX) return fail(MG_ERR_ARGUMENT, std::string(what) + ": too many rows");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(kCtaThreads<NT>);
+    cfg.dynamicSmemBytes = table_smem<NT>(p);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = p.parts;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = NT > 32 && p.parts > 1 ? 2 : 1;
+    MG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...));
+    return check_launch(what);
+}
+
+// Parts of a row for the calls that need the whole row's statistics: more
+// while the CTAs do not fill the GPU (and a part keeps 4096 actions), and, for
+// the loss, so many that the rows in flight stay in half of L2.
+int row_parts(int rows, int actions, int size, int nt, bool twice) {
+    int parts = 1;
+    const int fill = 4 * num_sms();
+    while (parts < 8 && (int64_t)rows * parts < fill && actions / (2 * parts) >= 4096) parts *= 2;
+    if (twice)
+        while (parts < 8 && (int64_t)num_sms() * (1024 / nt) / parts * actions * size > (48 << 20)) parts *= 2;
+    return parts;
+}
+
+template <class T, int NT, bool BACKWARD>
 int launch_control(const void* logits, int64_t ld, const mg_logit_controls& c, const void* dOut, int64_t ldg, void* out,
                    int64_t ldo, int rows, int actions, cudaStream_t st) {
-    const int span = actions < kChunk ? actions : kChunk, chunks = (actions + span - 1) / span;
-    MG_CHECK_ARG((int64_t)rows * chunks <= INT32_MAX, "logits_control: too many rows");
-    auto kern = k_logits_control<T, BACKWARD>;
+    auto kern = k_logits_control<T, NT, BACKWARD>;
     static std::atomic<uint64_t> done{0};
-    const size_t smem = c.history ? HistoryTable::bytes(span, c.history_max) : 0;
-    MG_TRY(smem_limit_once(kern, 100 * 1024, done));
-    MG_CUDA_TRY(MG_LAUNCH(kern, (unsigned)(rows * chunks), kThreads, smem, st, static_cast<const T*>(logits), ld, c,
-                          static_cast<const T*>(dOut), ldg, static_cast<T*>(out), ldo, actions, span, chunks));
+    MG_TRY(smem_limit_once(kern, kTableSmemMax, done));
+    TeamPart p = plan(NT, rows, actions, 1, c.history_max);
+    if (NT > 32) {  // independent chunks, no cluster
+        p.span = std::min(actions, NT * kControlGroups * kGroup<T>);
+        p.parts = (actions + p.span - 1) / p.span;
+        p.tableBytes = c.history ? (int)HistoryTable::bytes(p.span, c.history_max) : 0;
+    }
+    const int64_t ctas = NT == 32 ? ((int64_t)rows + kWarpRows - 1) / kWarpRows : (int64_t)rows * p.parts;
+    MG_CHECK_ARG(ctas <= INT32_MAX, "logits_control: too many rows");
+    MG_CUDA_TRY(MG_LAUNCH(kern, (unsigned)ctas, kCtaThreads<NT>, table_smem<NT>(p), st, static_cast<const T*>(logits), ld, c,
+                          static_cast<const T*>(dOut), ldg, static_cast<T*>(out), ldo, p));
     return check_launch("k_logits_control");
 }
 
-template <class T>
+template <class T, bool BACKWARD>
+int control(const void* logits, int64_t ld, const mg_logit_controls& c, const void* dOut, int64_t ldg, void* out, int64_t ldo,
+            int rows, int actions, cudaStream_t st) {
+    return actions <= kWarpActions
+               ? launch_control<T, 32, BACKWARD>(logits, ld, c, dOut, ldg, out, ldo, rows, actions, st)
+               : launch_control<T, 256, BACKWARD>(logits, ld, c, dOut, ldg, out, ldo, rows, actions, st);
+}
+
+template <class T, int NT, bool GREEDY>
 int launch_sample(const void* logits, int64_t ld, const mg_logit_controls& c, uint32_t* rng, int32_t* action, float* logProb,
                   float* entropy, float* value, int rows, int actions, cudaStream_t st) {
-    auto kern = k_logits_sample<T>;
+    auto kern = k_logits_sample<T, NT, GREEDY>;
     static std::atomic<uint64_t> done{0};
-    const size_t smem = c.history ? HistoryTable::bytes(actions, c.history_max) : 0;
-    MG_TRY(smem_limit_once(kern, 100 * 1024, done));
-    MG_CUDA_TRY(MG_LAUNCH(kern, rows, kThreads, smem, st, static_cast<const T*>(logits), ld, c, rng, action, logProb, entropy,
-                          value, actions));
-    return check_launch("k_logits_sample");
+    MG_TRY(smem_limit_once(kern, kTableSmemMax, done));
+    const TeamPart p = plan(NT, rows, actions, NT == 32 ? 1 : row_parts(rows, actions, sizeof(T), NT, false), c.history_max);
+    return launch_rows<NT>(kern, p, st, "k_logits_sample", static_cast<const T*>(logits), ld, c, rng, action, logProb, entropy,
+                           value, p);
 }
 
 template <class T>
+int sample(const void* logits, int64_t ld, const mg_logit_controls& c, uint32_t* rng, int32_t* action, float* logProb,
+           float* entropy, float* value, int rows, int actions, cudaStream_t st) {
+    const bool warp = actions <= kWarpActions;
+    if (rng)
+        return warp ? launch_sample<T, 32, false>(logits, ld, c, rng, action, logProb, entropy, value, rows, actions, st)
+                    : launch_sample<T, 256, false>(logits, ld, c, rng, action, logProb, entropy, value, rows, actions, st);
+    return warp ? launch_sample<T, 32, true>(logits, ld, c, rng, action, logProb, entropy, value, rows, actions, st)
+                : launch_sample<T, 256, true>(logits, ld, c, rng, action, logProb, entropy, value, rows, actions, st);
+}
+
+template <class T, int NT>
 int launch_loss(const void* logits, int64_t ld, const mg_logit_controls& c, void* d, int64_t ldd, int rows, int actions,
                 const LossArgs& L, cudaStream_t st) {
-    auto kern = k_logits_loss<T>;
+    auto kern = k_logits_loss<T, NT>;
     static std::atomic<uint64_t> done{0};
-    const size_t smem = c.history ? HistoryTable::bytes(actions, c.history_max) : 0;
-    MG_TRY(smem_limit_once(kern, 100 * 1024, done));
-    MG_CUDA_TRY(MG_LAUNCH(kern, rows, kThreads, smem, st, static_cast<const T*>(logits), ld, c, static_cast<T*>(d), ldd,
-                          actions, L));
-    return check_launch("k_logits_loss");
+    MG_TRY(smem_limit_once(kern, kTableSmemMax, done));
+    const TeamPart p = plan(NT, rows, actions, NT == 32 ? 1 : row_parts(rows, actions, sizeof(T), NT, true), c.history_max);
+    return launch_rows<NT>(kern, p, st, "k_logits_loss", static_cast<const T*>(logits), ld, c, static_cast<T*>(d), ldd, p, L);
+}
+
+template <class T>
+int loss(const void* logits, int64_t ld, const mg_logit_controls& c, void* d, int64_t ldd, int rows, int actions,
+         const LossArgs& L, cudaStream_t st) {
+    return actions <= kWarpActions ? launch_loss<T, 32>(logits, ld, c, d, ldd, rows, actions, L, st)
+                                   : launch_loss<T, 256>(logits, ld, c, d, ldd, rows, actions, L, st);
 }
 
 }  // namespace
@@ -363,10 +703,10 @@ int mg_logits_control(const void* logits, int dtype, int64_t ld, const mg_logit_
     MG_CHECK_ARG(out != logits || ldo == ld, "logits_control: in place needs ldo = ld");
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (dtype == MG_DTYPE_F32)
-        return launch_control<float, false>(logits, ld, c, nullptr, 0, out, ldo, rows, actions, st);
+        return control<float, false>(logits, ld, c, nullptr, 0, out, ldo, rows, actions, st);
     if (dtype == MG_DTYPE_BF16)
-        return launch_control<__nv_bfloat16, false>(logits, ld, c, nullptr, 0, out, ldo, rows, actions, st);
-    return launch_control<__half, false>(logits, ld, c, nullptr, 0, out, ldo, rows, actions, st);
+        return control<__nv_bfloat16, false>(logits, ld, c, nullptr, 0, out, ldo, rows, actions, st);
+    return control<__half, false>(logits, ld, c, nullptr, 0, out, ldo, rows, actions, st);
 }
 
 int mg_logits_control_backward(const void* logits, int dtype, int64_t ld, const mg_logit_controls* controls,
@@ -385,10 +725,10 @@ int mg_logits_control_backward(const void* logits, int dtype, int64_t ld, const 
     if (!c.repetition) c.history = nullptr;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (dtype == MG_DTYPE_F32)
-        return launch_control<float, true>(logits, ld, c, d_out, ldg, d_logits, ldd, rows, actions, st);
+        return control<float, true>(logits, ld, c, d_out, ldg, d_logits, ldd, rows, actions, st);
     if (dtype == MG_DTYPE_BF16)
-        return launch_control<__nv_bfloat16, true>(logits, ld, c, d_out, ldg, d_logits, ldd, rows, actions, st);
-    return launch_control<__half, true>(logits, ld, c, d_out, ldg, d_logits, ldd, rows, actions, st);
+        return control<__nv_bfloat16, true>(logits, ld, c, d_out, ldg, d_logits, ldd, rows, actions, st);
+    return control<__half, true>(logits, ld, c, d_out, ldg, d_logits, ldd, rows, actions, st);
 }
 
 int mg_logits_sample(const void* logits, int dtype, int64_t ld, const mg_logit_controls* controls, uint32_t* rng,
@@ -397,7 +737,7 @@ int mg_logits_sample(const void* logits, int dtype, int64_t ld, const mg_logit_c
     mg_logit_controls c;
     MG_TRY(check_common("logits_sample", logits, dtype, ld, controls, rows, actions, actions + (value ? 1 : 0), &c));
     MG_CHECK_ARG(action && log_prob, "logits_sample: null action or log_prob");
-    return MG_BY_TYPE(dtype, launch_sample)(logits, ld, c, rng, action, log_prob, entropy, value, rows, actions,
+    return MG_BY_TYPE(dtype, sample)(logits, ld, c, rng, action, log_prob, entropy, value, rows, actions,
                                             reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -414,7 +754,7 @@ int mg_logits_policy_loss(const void* logits, int dtype, int64_t ld, const mg_lo
     MG_CHECK_ARG(d_logits != logits || ldd == ld, "logits_policy_loss: in place needs ldd = ld");
     MG_CHECK_ARG(clip >= 0.0f, "logits_policy_loss: negative clip");
     LossArgs L{action, adv, adv_stats, ret, old_log_prob, stats, clip, value_coef, entropy_coef, grad_scale, status_ptr()};
-    return MG_BY_TYPE(dtype, launch_loss)(logits, ld, c, d_logits, ldd, rows, actions, L,
+    return MG_BY_TYPE(dtype, loss)(logits, ld, c, d_logits, ldd, rows, actions, L,
                                           reinterpret_cast<cudaStream_t>(stream));
 }
 
