@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <atomic>
 #include <string>
+#include <type_traits>
 #include <utility>
 
 #include "logits.cuh"
@@ -51,6 +52,11 @@ __device__ __forceinline__ bool team_part(const TeamPart& p, int& row, int& lo, 
     return true;
 }
 
+// Whether 16-byte boundaries of `a` are ones of `b` too.
+__device__ __forceinline__ bool same_alignment(const void* a, const void* b) {
+    return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15) == 0;
+}
+
 template <int NT>
 __device__ __forceinline__ int team_rank() {
     return NT == 32 ? threadIdx.x & 31 : threadIdx.x;
@@ -63,23 +69,13 @@ __device__ __forceinline__ HistoryTable team_table(const TeamPart& p, const mg_l
     return t;
 }
 
-// The controlled logit of action a (raw x); the table covers actions from lo.
-__device__ __forceinline__ float controlled(const RowControls& r, const HistoryTable& t, float x, int a, int lo) {
-    if (r.history) {
-        const int n = t.count(a - lo);
-        if (n > 0) x = penalise(r, x, n);
-    }
-    if (r.bias) x = __fadd_rn(x, r.bias[a]);
-    return allowed(r, a) ? x : -INFINITY;
-}
-
 // ------------------------------------------------------------------ control and its gradient
 
-// Groups of a thread in flight together.
-constexpr int kControlGroups = 4;
+// Groups of a thread in flight together, and groups a thread has in all (one CTA).
+constexpr int kControlGroups = 2, kControlRounds = 2;
 
 template <class T, int NT, bool BACKWARD>
-__global__ void __launch_bounds__(kCtaThreads<NT>)
+__global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 6)
     k_logits_control(const T* logits, int64_t ld, const mg_logit_controls c, const T* dOut, int64_t ldg, T* out,
                      int64_t ldo, const TeamPart part) {
     constexpr int VE = kGroup<T>, U = kControlGroups;
@@ -95,60 +91,53 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
     const T* src = BACKWARD ? dOut + (int64_t)row * ldg : x;
     T* y = out + (int64_t)row * ldo;
     const bool vec = same_alignment(src, y);
-    const int start = group_start(src, lo), groups = group_count<T>(start, hi), tid = team_rank<NT>();
+    const RowSpan s = row_span(src, lo, hi);
+    const int tid = team_rank<NT>();
     bool filled = !r.history;
-    for (int g0 = 0; g0 < groups || !filled; g0 += NT * U) {
-        RawGroup<T> raw[U];
+    for (int g0 = tid; g0 - tid < s.groups || !filled; g0 += NT * U) {
+        uint4 raw[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int a = start + (g0 + u * NT + tid) * VE;
-            raw[u] = group_load(src, a, group_valid<T>(a, lo, hi));
-        }
+        for (int u = 0; u < U; u++)
+            if (g0 + u * NT < s.groups) raw[u] = group_load(src + s.body + (g0 + u * NT) * VE);
         if (!filled) {  // while the first loads are in flight
             history_fill<NT>(t, c.history + (int64_t)row * c.history_stride, row_history_len(c, row), lo, hi, c.history_max, sums);
             filled = true;
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const int a = start + (g0 + u * NT + tid) * VE;
-            const uint32_t valid = group_valid<T>(a, lo, hi);
-            if (!valid) continue;
+            if (g0 + u * NT >= s.groups) break;
+            const int a = s.body + (g0 + u * NT) * VE;
             float v[VE];
+            group_floats(raw[u], src, v);
+            uint32_t seen = 0, positive = 0;
             if (!BACKWARD) {
-                group_control(r, t, raw[u], a, lo, valid, v);
+                group_control<VE>(r, t, a, lo, v, seen, positive);
             } else {
-#pragma unroll
-                for (int i = 0; i < VE; i++) v[i] = raw_value(raw[u], i);
-                if (r.history) {
-                    // the raw logits' signs, read only for groups that hold an action that occurred
-                    uint32_t seen = 0;
-#pragma unroll
-                    for (int i = 0; i < VE; i++)
-                        if ((valid >> i) & 1u) {
-                            const int k = a - lo + i;
-                            seen |= ((t.seen[k >> 5] >> (k & 31)) & 1u) << i;
-                        }
-                    if (seen) {
-#pragma unroll
-                        for (int i = 0; i < VE; i++)
-                            if ((seen >> i) & 1u)
-                                v[i] = to_f32(x[a + i]) > 0.0f ? __fdiv_rn(v[i], r.repetition) : __fmul_rn(v[i], r.repetition);
+                if (r.history) {  // the raw logits' signs, read only where they count
+                    seen = bit_window<VE>(t.seen, a - lo) & ((1u << VE) - 1u);
+                    for (uint32_t left = seen; left; left &= left - 1) {
+                        const int i = __ffs(left) - 1;
+                        if (to_f32(x[a + i]) > 0.0f) positive |= 1u << i;
                     }
                 }
-                if (r.mask) {
-#pragma unroll
-                    for (int i = 0; i < VE; i++)
-                        if (((valid >> i) & 1u) && !allowed(r, a + i)) v[i] = 0.0f;
-                }
+                group_gradient<VE>(r, a, seen, positive, v);
             }
-            group_store(y, a, valid, vec, v);
+            group_store(y + a, vec, group_pack(v, src));
+        }
+    }
+    if (s.edges() && tid < 32) {
+        const int a = s.edge<VE>(tid);
+        if (a >= 0) {
+            const float raw = to_f32(src[a]);
+            from_f32(&y[a], BACKWARD ? control_gradient(r, t, raw, r.history ? to_f32(x[a]) : 0.0f, a, lo)
+                                     : controlled(r, t, raw, a, lo));
         }
     }
 }
 
 // ------------------------------------------------------------------ softmax statistics and the race
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float exp2_fast(float x) {  // within 2 ulp; results below 2^-126 are 0
     float y;
@@ -167,25 +156,23 @@ __device__ __forceinline__ float warp_max(float x) {
     return y;
 }
 
-// Running softmax statistics: the maximum m, s = sum e^(l - m), t = sum
-// e^(l - m) (l - m); entropy = log s - t / s. In the passes m is the same in
-// the threads of a warp, s and t are a thread's.
+// log2(e^l) - m. Every use takes the same m, so that the rounding of m (the
+// largest logit in these units) is the same for all and falls out of
+// probabilities and their logarithms; the product is not rounded (FMA). Kept
+// finite, so that e^-inf = 0 times it is 0 (a NaN stays one).
+__device__ __forceinline__ float log2_weight(float l, float m) { return max_nan(fmaf(l, kLog2e, -m), -1e30f); }
+
+// Running softmax statistics in units of log2: the maximum m, s = sum 2^d, t =
+// sum 2^d d with d = log2_weight(l, m); entropy = ln 2 (log2 s - t / s). In the
+// passes m is the same in the threads of a warp, s and t are a thread's.
 struct Softmax {
     float m = -INFINITY, s = 0.0f, t = 0.0f;
     // Raises m (a whole warp) and returns the factor that carried s over.
     __device__ __forceinline__ float raise(float top) {
-        const float d = m - top, e = m > -INFINITY ? exp2_fast(d * kLog2e) : 0.0f;
+        const float d = m - top, e = m > -INFINITY ? exp2_fast(d) : 0.0f;
         t = e > 0.0f ? e * (t + s * d) : 0.0f;
         if (!(s != s)) s = s * e;
         m = top;
-        return e;
-    }
-    // e^(l - m) of one logit, added to the sums; m > -inf. The difference is
-    // kept finite so that e^(..) = 0 times it is 0 (a NaN stays one).
-    __device__ __forceinline__ float add(float l) {
-        const float d = max_nan(l - m, -1e30f), e = exp2_fast(d * kLog2e);
-        s += e;
-        t = fmaf(e, d, t);
         return e;
     }
     __device__ __forceinline__ void merge(const Softmax& o) {
@@ -195,7 +182,7 @@ struct Softmax {
             return;
         }
         const float top = fmaxf(m, o.m);
-        const float da = m - top, db = o.m - top, ea = expf(da), eb = expf(db);
+        const float da = m - top, db = o.m - top, ea = exp2f(da), eb = exp2f(db);
         const float ta = ea == 0.0f ? 0.0f : ea * (t + s * da), tb = eb == 0.0f ? 0.0f : eb * (o.t + o.s * db);
         s = s * ea + o.s * eb;
         t = ta + tb;
@@ -203,23 +190,44 @@ struct Softmax {
     }
 };
 
-// Adds a group's logits (-inf: not allowed) to a warp's statistics. `raised` is
-// told when m rises; each(i, e) gets every element's e^(l - m).
-template <int VE, class Raised, class Each>
-__device__ __forceinline__ void softmax_group(Softmax& v, const float* x, Raised raised, Each each) {
+// Adds N logits (-inf: not allowed) to a warp's statistics and gives their e^(l
+// - max) in e; `raised` is told when m rises. False: nothing allowed so far, e
+// is not set.
+template <int N, class Raised>
+__device__ __forceinline__ bool softmax_group(Softmax& v, const float* x, float* e, Raised raised) {
     float top = x[0];
 #pragma unroll
-    for (int i = 1; i < VE; i++) top = fmaxf(top, x[i]);
-    top = warp_max(top);
+    for (int i = 1; i < N; i++) top = fmaxf(top, x[i]);
+    top = warp_max(top) * kLog2e;
     if (top > v.m) raised(v.raise(top));
-    if (v.m == -INFINITY) {  // nothing allowed so far: a NaN still shows
+    if (v.m == -INFINITY) {  // a NaN still shows
 #pragma unroll
-        for (int i = 0; i < VE; i++)
+        for (int i = 0; i < N; i++)
             if (x[i] != x[i]) v.s = x[i];
-        return;
+        return false;
     }
+    float2 s2 = make_float2(0.0f, 0.0f), t2 = s2;
+    const float2 k2 = make_float2(kLog2e, kLog2e), m2 = make_float2(-v.m, -v.m);
 #pragma unroll
-    for (int i = 0; i < VE; i++) each(i, v.add(x[i]));
+    for (int i = 0; i + 1 < N; i += 2) {  // two at a time (f32x2)
+        float2 d = f2fma_rn(make_float2(x[i], x[i + 1]), k2, m2);
+        d.x = max_nan(d.x, -1e30f);
+        d.y = max_nan(d.y, -1e30f);
+        const float2 w = make_float2(exp2_fast(d.x), exp2_fast(d.y));
+        s2 = f2add_rn(s2, w);
+        t2 = f2fma_rn(w, d, t2);
+        e[i] = w.x;
+        e[i + 1] = w.y;
+    }
+    if (N & 1) {
+        const float d = log2_weight(x[N - 1], v.m);
+        e[N - 1] = exp2_fast(d);
+        s2.x += e[N - 1];
+        t2.x = fmaf(e[N - 1], d, t2.x);
+    }
+    v.s += s2.x + s2.y;
+    v.t += t2.x + t2.y;
+    return true;
 }
 
 __device__ __forceinline__ uint32_t race_bits(uint32_t word, int a) { return mg_mix32(word + (uint32_t)a * 0x9E3779B9u); }
@@ -276,7 +284,7 @@ __device__ inline void row_merge(RowPart& mine, RowPart* warps, RowPart* whole, 
     mine.v.s = warp_add(mine.v.s);
     mine.v.t = warp_add(mine.v.t);
     if (RACE) {
-#pragma unroll
+#pragma unroll 1
         for (int d = 16; d; d >>= 1) {
             Runner o;
             o.key = __shfl_xor_sync(0xffffffffu, mine.best.key, d);
@@ -295,6 +303,7 @@ __device__ inline void row_merge(RowPart& mine, RowPart* warps, RowPart* whole, 
     };
     if (threadIdx.x == 0) {
         RowPart all = warps[0];
+#pragma unroll 1
         for (int w = 1; w < kTeamWarps<NT>; w++) join(all, warps[w]);
         *whole = all;
     }
@@ -305,6 +314,7 @@ __device__ inline void row_merge(RowPart& mine, RowPart* warps, RowPart* whole, 
     }
     cluster_sync();
     RowPart all = *cluster_peer(whole, 0);
+#pragma unroll 1
     for (int k = 1; k < parts; k++) join(all, *cluster_peer(whole, k));
     if (!RACE) all.chosen = cluster_peer(whole, chosenRank)->chosen;
     mine = all;
@@ -312,11 +322,11 @@ __device__ inline void row_merge(RowPart& mine, RowPart* warps, RowPart* whole, 
 
 // ------------------------------------------------------------------ draw
 
-// One pass. An action a can win only where its time E_a >= v_a = (h + 1/2) /
-// 2^32 is below the best ratio E / e^(l - m) so far times its own e^(l - m):
-// the test takes the upper bits of h as a number of [1, 2) against 1 + that
-// bound (a millionth more than it, so that rounding never hides a winner), and
-// only the few that pass take logarithms.
+// One pass. An action can win only where its time E >= v = (h + 1/2) / 2^32 is
+// below the best ratio E / e^(l - m) so far times its own e^(l - m). The test
+// takes the upper 16 bits of h, which the last step of mg_mix32 leaves alone,
+// as 2^23 + k against 2^23 + 2^16 times that bound (1e-4 more than it, so that
+// rounding never hides a winner); only the few that pass take logarithms.
 template <class T, int NT, bool GREEDY>
 __global__ void __launch_bounds__(kCtaThreads<NT>)
     k_logits_sample(const T* logits, int64_t ld, const mg_logit_controls c, uint32_t* rng, int32_t* action,
@@ -340,71 +350,84 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
     if (!GREEDY) rngNext(word);
     RowPart mine;
     float bound = 3e38f;  // the warp's best ratio E / e^(l - m)
-    const int start = group_start(x, lo), groups = group_count<T>(start, hi), tid = team_rank<NT>();
-    const int rounds = (groups + NT - 1) / NT;
-    for (int k = 0; k < rounds; k++) {
-        const int a = start + (k * NT + tid) * VE;
-        const uint32_t valid = group_valid<T>(a, lo, hi);
-        float l[VE], e[VE];
-        const RawGroup<T> raw = group_load(x, a, valid);
-        if (valid) {
-            group_control(r, t, raw, a, lo, valid, l);
+    const RowSpan s = row_span(x, lo, hi);
+    const int tid = team_rank<NT>();
+
+    // N actions from a on (every lane of the warp calls it; -inf where a lane has none)
+    auto take = [&](const float* l, int a, auto count) {
+        constexpr int N = decltype(count)::value;
+        float e[N];
+        if (!softmax_group<N>(mine.v, l, e, [&](float f) { bound = f > 0.0f ? fminf(bound / f, 3e38f) : 3e38f; })) return;
+        if (GREEDY) {
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (l[i] > mine.best.logit || (N == 1 && l[i] == mine.best.logit && a + i < mine.best.action)) {
+                    mine.best.logit = l[i];
+                    mine.best.action = a + i;
+                }
+            return;
+        }
+        bool pass = false;
+        const float limit = fminf(bound * 65542.6f, 3e38f);  // 2^16 (1 + 1e-4)
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            uint32_t h = word + (uint32_t)a * 0x9E3779B9u + (uint32_t)i * 0x9E3779B9u;
+            h ^= h >> 16;
+            h *= 0x7feb352du;
+            h ^= h >> 15;
+            h *= 0x846ca68bu;
+            const float f = __uint_as_float(__byte_perm(h, 0x4B000000u, 0x7632));
+            pass = pass || f <= fmaf(limit, e[i], 8388608.0f);
+        }
+        if (__any_sync(0xffffffffu, pass)) {
+            float least = 3e38f;
+            if (pass) {
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const uint32_t h = race_bits(word, a + i);
+                    const float f = (float)(h >> 16);
+                    if (l[i] > -INFINITY && f <= limit * e[i]) {
+                        // -log(1 - v) from whichever of v and 1 - v is small
+                        const float time = h < 0x80000000u ? -log1pf(-((float)h + 0.5f) * 2.3283064e-10f)
+                                                           : -logf(((float)(~h) + 0.5f) * 2.3283064e-10f);
+                        Runner o;
+                        o.key = l[i] - logf(time);
+                        o.logit = l[i];
+                        o.bits = h;
+                        o.action = a + i;
+                        if (beats<false>(o, mine.best)) mine.best = o;
+                        least = fminf(least, time / e[i]);
+                    }
+                }
+            }
+            bound = fminf(bound, __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least))));
+        }
+    };
+    for (int g0 = 0; g0 < s.groups; g0 += NT) {
+        const int g = g0 + tid, a = s.body + g * VE;
+        float l[VE];
+        if (g < s.groups) {
+            group_floats(group_load(x + a), x, l);
+            uint32_t seen, positive;
+            group_control<VE>(r, t, a, lo, l, seen, positive);
         } else {
 #pragma unroll
             for (int i = 0; i < VE; i++) l[i] = -INFINITY;
         }
-        bool live = false;
-        softmax_group<VE>(
-            mine.v, l, [&](float f) { bound = f > 0.0f ? fminf(bound / f, 3e38f) : 3e38f; },
-            [&](int i, float v) {
-                e[i] = v;
-                live = true;
-            });
-        if (!live) continue;  // the whole warp: m is the warp's
-        if (GREEDY) {
-#pragma unroll
-            for (int i = 0; i < VE; i++)
-                if (l[i] > mine.best.logit) {
-                    mine.best.logit = l[i];
-                    mine.best.action = a + i;
-                }
-            continue;
-        }
-        uint32_t pass = 0;
-        const float limit = bound * 1.0001f;
-#pragma unroll
-        for (int i = 0; i < VE; i++) {
-            const uint32_t h = race_bits(word, a + i);
-            const float f = __uint_as_float((h >> 9) | 0x3f800000u);
-            if (f <= fmaf(limit, e[i], 1.0f)) pass |= 1u << i;
-        }
-        if (__any_sync(0xffffffffu, pass != 0)) {
-            float least = 3e38f;
-#pragma unroll
-            for (int i = 0; i < VE; i++)
-                if (((pass >> i) & 1u) && l[i] > -INFINITY) {
-                    const uint32_t h = race_bits(word, a + i);
-                    // -log(1 - v) from whichever of v and 1 - v is small
-                    const float time = h < 0x80000000u ? -log1pf(-((float)h + 0.5f) * 2.3283064e-10f)
-                                                       : -logf(((float)(~h) + 0.5f) * 2.3283064e-10f);
-                    Runner o;
-                    o.key = l[i] - logf(time);
-                    o.logit = l[i];
-                    o.bits = h;
-                    o.action = a + i;
-                    if (beats<false>(o, mine.best)) mine.best = o;
-                    least = fminf(least, time / e[i]);
-                }
-            bound = fminf(bound, __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least))));
-        }
+        take(l, a, std::integral_constant<int, VE>());
+    }
+    if (s.edges() && tid < 32) {
+        const int a = s.edge<VE>(tid);
+        const float l = a >= 0 ? controlled(r, t, to_f32(x[a]), a, lo) : -INFINITY;
+        take(&l, a, std::integral_constant<int, 1>());
     }
     row_merge<NT, true, GREEDY>(mine, warps, whole, part.parts, 0);
     if (tid == 0 && lo == 0) {
-        const float ls = logf(mine.v.s);
+        const float ls = log2f(mine.v.s);
         const bool some = mine.best.action >= 0 || mine.v.s != mine.v.s;
         action[row] = mine.best.action;
-        logProb[row] = some ? (mine.best.logit - mine.v.m) - ls : 0.0f;
-        if (entropy) entropy[row] = some ? ls - mine.v.t / mine.v.s : 0.0f;
+        logProb[row] = some ? (log2_weight(mine.best.logit, mine.v.m) - ls) * kLn2 : 0.0f;
+        if (entropy) entropy[row] = some ? (ls - mine.v.t / mine.v.s) * kLn2 : 0.0f;
         if (value) value[row] = to_f32(x[part.actions]);
         if (!GREEDY) rng[row] = word;
     }
@@ -455,24 +478,28 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
         history_fill<NT>(t, c.history + (int64_t)row * c.history_stride, row_history_len(c, row), lo, hi, c.history_max, sums);
     RowPart mine;
     mine.chosen = act >= lo && act < hi ? controlled(r, t, to_f32(x[act]), act, lo) : 0.0f;
-    const int start = group_start(x, lo), groups = group_count<T>(start, hi);
-    const int rounds = (groups + NT - 1) / NT;
-    for (int k = 0; k < rounds; k++) {
-        const int a = start + (k * NT + tid) * VE;
-        const uint32_t valid = group_valid<T>(a, lo, hi);
-        float l[VE];
-        const RawGroup<T> raw = group_load(x, a, valid);
-        if (valid) {
-            group_control(r, t, raw, a, lo, valid, l);
+    const RowSpan s = row_span(x, lo, hi);
+    for (int g0 = 0; g0 < s.groups; g0 += NT) {
+        const int g = g0 + tid, a = s.body + g * VE;
+        float l[VE], e[VE];
+        if (g < s.groups) {
+            group_floats(group_load(x + a), x, l);
+            uint32_t seen, positive;
+            group_control<VE>(r, t, a, lo, l, seen, positive);
         } else {
 #pragma unroll
             for (int i = 0; i < VE; i++) l[i] = -INFINITY;
         }
-        softmax_group<VE>(mine.v, l, [](float) {}, [](int, float) {});
+        softmax_group<VE>(mine.v, l, e, [](float) {});
+    }
+    if (s.edges() && tid < 32) {
+        const int a = s.edge<VE>(tid);
+        float l = a >= 0 ? controlled(r, t, to_f32(x[a]), a, lo) : -INFINITY, e;
+        softmax_group<1>(mine.v, &l, &e, [](float) {});
     }
     row_merge<NT, false, false>(mine, warps, whole, part.parts, act / part.span);
-    const float ls = logf(mine.v.s), entropy = ls - mine.v.t / mine.v.s;
-    const float logp = (mine.chosen - mine.v.m) - ls, old = L.oldLogProb[row];
+    const float m = mine.v.m, ls = log2f(mine.v.s), entropy = (ls - mine.v.t / mine.v.s) * kLn2;
+    const float logp = (log2_weight(mine.chosen, m) - ls) * kLn2, old = L.oldLogProb[row];
     const float ratio = expf(logp - old);
     const float adv = L.advStats ? (L.adv[row] - L.advStats[0]) * L.advStats[1] : L.adv[row];
     const float one = ratio * adv, two = fminf(fmaxf(ratio, 1.0f - L.clip), 1.0f + L.clip) * adv;
@@ -484,30 +511,44 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
         cluster_sync();
     else
         __syncthreads();
-    // dl = scale (slope (1[a = act] - p) + ent p (log p + H)) = p (s1 (log p + H) - s0), + s0 at act
-    const float s0 = slope * L.scale, s1 = L.entropyCoef * L.scale;
+    // dl = scale (slope (1[a = act] - p) + ent p (ln p + H)) = p (s1 log2 p + (ent H - slope) scale), + s0 at act
+    const float s0 = slope * L.scale, s1 = L.entropyCoef * L.scale * kLn2, sh = fmaf(L.entropyCoef * L.scale, entropy, -s0);
     const bool vec = same_alignment(x, d);
-    for (int k = 0; k < rounds; k++) {
-        const int a = start + (k * NT + tid) * VE;
-        const uint32_t valid = group_valid<T>(a, lo, hi);
-        if (!valid) continue;
-        float l[VE], g[VE];
-        const RawGroup<T> raw = group_load(x, a, valid);
-        const GroupControls gc = group_control(r, t, raw, a, lo, valid, l);
+    for (int g = tid; g < s.groups; g += NT) {
+        const int a = s.body + g * VE;
+        float l[VE];
+        group_floats(group_load(x + a), x, l);
+        uint32_t seen, positive;
+        group_control<VE>(r, t, a, lo, l, seen, positive);
+        const float2 k2 = make_float2(kLog2e, kLog2e), m2 = make_float2(-m, -m), ls2 = make_float2(-ls, -ls);
+        const float2 s12 = make_float2(s1, s1), sh2 = make_float2(sh, sh);
 #pragma unroll
-        for (int i = 0; i < VE; i++) {
-            const float lp = max_nan(l[i] - mine.v.m, -1e30f) - ls;
-            const float p = exp2_fast(lp * kLog2e);
-            g[i] = p * fmaf(s1, lp + entropy, -s0);
-            if (a + i == act) g[i] += s0;
+        for (int i = 0; i < VE; i += 2) {
+            float2 q = f2fma_rn(make_float2(l[i], l[i + 1]), k2, m2);
+            q.x = max_nan(q.x, -1e30f);
+            q.y = max_nan(q.y, -1e30f);
+            q = f2add_rn(q, ls2);
+            const float2 p = make_float2(exp2_fast(q.x), exp2_fast(q.y));
+            const float2 o = f2mul_rn(p, f2fma_rn(s12, q, sh2));
+            l[i] = o.x;
+            l[i + 1] = o.y;
         }
-        group_factor<T>(r, gc, g);
-        if (gc.ok != (1u << VE) - 1u) {  // not allowed: 0, whatever became of a row with a NaN
+        if ((unsigned)(act - a) < (unsigned)VE) {
 #pragma unroll
-            for (int i = 0; i < VE; i++)
-                if (!((gc.ok >> i) & 1u)) g[i] = 0.0f;
+            for (int i = 0; i < VE; i++) l[i] = a + i == act ? l[i] + s0 : l[i];
         }
-        group_store(d, a, valid, vec, g);
+        group_gradient<VE>(r, a, seen, positive, l);
+        group_store(d + a, vec, group_pack(l, x));
+    }
+    if (s.edges() && tid < 32) {
+        const int a = s.edge<VE>(tid);
+        if (a >= 0) {
+            const float raw = to_f32(x[a]);
+            const float q = log2_weight(controlled(r, t, raw, a, lo), m) - ls;
+            float g = exp2_fast(q) * fmaf(s1, q, sh);
+            if (a == act) g += s0;
+            from_f32(&d[a], control_gradient(r, t, g, raw, a, lo));
+        }
     }
     if (tid == 0 && lo == 0) {
         float* st = L.stats + (int64_t)row * 5;
@@ -626,7 +667,7 @@ int launch_control(const void* logits, int64_t ld, const mg_logit_controls& c, c
     MG_TRY(smem_limit_once(kern, kTableSmemMax, done));
     TeamPart p = plan(NT, rows, actions, 1, c.history_max);
     if (NT > 32) {  // independent chunks, no cluster
-        p.span = std::min(actions, NT * kControlGroups * kGroup<T>);
+        p.span = std::min(actions, NT * kControlGroups * kControlRounds * kGroup<T>);
         p.parts = (actions + p.span - 1) / p.span;
         p.tableBytes = c.history ? (int)HistoryTable::bytes(p.span, c.history_max) : 0;
     }

@@ -13,7 +13,6 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
-#include <string.h>
 
 #include "../../include/metalgym_b200.h"
 
@@ -157,141 +156,154 @@ __device__ __forceinline__ float penalise(const RowControls& r, float x, int n) 
     return __fsub_rn(__fsub_rn(x, __fmul_rn(r.frequency, (float)n)), r.presence);
 }
 
+// The controlled logit of action a (raw x); the table covers actions from lo.
+__device__ __forceinline__ float controlled(const RowControls& r, const HistoryTable& t, float x, int a, int lo) {
+    if (r.history) {
+        const int n = t.count(a - lo);
+        if (n > 0) x = penalise(r, x, n);
+    }
+    if (r.bias) x = __fadd_rn(x, r.bias[a]);
+    return allowed(r, a) ? x : -INFINITY;
+}
+// The gradient of an action's raw logit x from that of its controlled one.
+__device__ __forceinline__ float control_gradient(const RowControls& r, const HistoryTable& t, float g, float x, int a, int lo) {
+    if (r.history && t.count(a - lo) > 0) g = x > 0.0f ? __fdiv_rn(g, r.repetition) : __fmul_rn(g, r.repetition);
+    return allowed(r, a) ? g : 0.0f;
+}
+
 // ------------------------------------------------------------------ groups
-// A row is read in groups of 16 bytes, cut at 16-byte boundaries of memory
-// whatever the row's start: a group that the row (or the part [lo, hi) of it)
-// fills takes one vector load, the first and last ones element loads.
+// A row (or a part [lo, hi) of it) is read in groups of 16 bytes, one vector
+// load each, cut at 16-byte boundaries of memory; the up to kGroup - 1
+// actions before the first boundary and behind the last one, the edges, are
+// done one by one by the first warp of the team.
 
 template <class T>
 constexpr int kGroup = 16 / (int)sizeof(T);
 
-// The first action of group 0 of [lo, hi) (at or up to kGroup - 1 before lo),
-// and the number of groups.
-template <class T>
-__device__ __forceinline__ int group_start(const T* row, int lo) {
-    return lo - (int)((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
-}
-template <class T>
-__device__ __forceinline__ int group_count(int start, int hi) {
-    return (hi - start + kGroup<T> - 1) / kGroup<T>;
-}
-
-// The group's values as they lie in memory.
-template <class T>
-struct RawGroup {
-    uint4 w;
+struct RowSpan {
+    int body, groups;    // first action of group 0, number of groups
+    int lo, head, tail;  // actions before the groups, and behind them
+    // The action of lane `lane` of the edges, or -1.
+    template <int VE>
+    __device__ __forceinline__ int edge(int lane) const {
+        if (lane < head) return lo + lane;
+        return lane >= 16 && lane - 16 < tail ? body + groups * VE + lane - 16 : -1;
+    }
+    __device__ __forceinline__ bool edges() const { return (head | tail) != 0; }
 };
 
-__device__ __forceinline__ float raw_value(const RawGroup<float>& g, int i) {
-    return __uint_as_float(i == 0 ? g.w.x : i == 1 ? g.w.y : i == 2 ? g.w.z : g.w.w);
-}
-__device__ __forceinline__ float raw_value(const RawGroup<__nv_bfloat16>& g, int i) {
-    const uint32_t u = (i >> 1) == 0 ? g.w.x : (i >> 1) == 1 ? g.w.y : (i >> 1) == 2 ? g.w.z : g.w.w;
-    return __uint_as_float((i & 1) ? (u & 0xffff0000u) : (u << 16));
-}
-__device__ __forceinline__ float raw_value(const RawGroup<__half>& g, int i) {
-    const uint32_t u = (i >> 1) == 0 ? g.w.x : (i >> 1) == 1 ? g.w.y : (i >> 1) == 2 ? g.w.z : g.w.w;
-    return __half2float(__ushort_as_half((unsigned short)((i & 1) ? (u >> 16) : (u & 0xffffu))));
-}
-
-// Bits of the group's elements that lie in [lo, hi).
 template <class T>
-__device__ __forceinline__ uint32_t group_valid(int a, int lo, int hi) {
+__device__ __forceinline__ RowSpan row_span(const T* row, int lo, int hi) {
     constexpr int VE = kGroup<T>;
-    uint32_t v = (1u << VE) - 1u;
-    if (a < lo) v &= ~0u << (lo - a);
-    if (a + VE > hi) v = hi <= a ? 0u : v & ((1u << (hi - a)) - 1u);
-    return v;
+    const int past = (int)((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
+    RowSpan s;
+    s.lo = lo;
+    s.head = min(hi - lo, past ? VE - past : 0);
+    s.body = lo + s.head;
+    s.groups = (hi - s.body) / VE;
+    s.tail = hi - s.body - s.groups * VE;
+    return s;
 }
 
 template <class T>
-__device__ __forceinline__ RawGroup<T> group_load(const T* row, int a, uint32_t valid) {
-    constexpr int VE = kGroup<T>;
-    RawGroup<T> g;
-    if (valid == (1u << VE) - 1u) {
-        g.w = *reinterpret_cast<const uint4*>(row + a);
-        return g;
+__device__ __forceinline__ uint4 group_load(const T* p) {
+    return *reinterpret_cast<const uint4*>(p);
+}
+__device__ __forceinline__ void group_floats(const uint4& w, const float*, float* x) {
+    x[0] = __uint_as_float(w.x);
+    x[1] = __uint_as_float(w.y);
+    x[2] = __uint_as_float(w.z);
+    x[3] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ void group_floats(const uint4& w, const __nv_bfloat16*, float* x) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        x[2 * i] = __uint_as_float(u[i] << 16);
+        x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
-    uint32_t w[4] = {0, 0, 0, 0};
+}
+__device__ __forceinline__ void group_floats(const uint4& w, const __half*, float* x) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < VE; i++)
-        if ((valid >> i) & 1u) {
-            if (sizeof(T) == 4)
-                w[i] = reinterpret_cast<const uint32_t*>(row)[a + i];
-            else
-                w[i >> 1] |= (uint32_t)reinterpret_cast<const unsigned short*>(row)[a + i] << ((i & 1) * 16);
-        }
-    g.w = make_uint4(w[0], w[1], w[2], w[3]);
-    return g;
+    for (int i = 0; i < 4; i++) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ uint4 group_pack(const float* v, const float*) {
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+__device__ __forceinline__ uint4 group_pack(const float* v, const __nv_bfloat16*) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        u[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
+}
+__device__ __forceinline__ uint4 group_pack(const float* v, const __half*) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        u[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
-// Writes a group's values; `vec`: out + a is 16-byte aligned where the group is full.
+// Writes a full group; `vec`: p is 16-byte aligned.
 template <class T>
-__device__ __forceinline__ void group_store(T* out, int a, uint32_t valid, bool vec, const float* v) {
-    constexpr int VE = kGroup<T>;
-    T o[VE];
-#pragma unroll
-    for (int i = 0; i < VE; i++) from_f32(&o[i], v[i]);
-    if (vec && valid == (1u << VE) - 1u) {
-        uint32_t w[4];
-        memcpy(w, o, 16);
-        *reinterpret_cast<uint4*>(out + a) = make_uint4(w[0], w[1], w[2], w[3]);
+__device__ __forceinline__ void group_store(T* p, bool vec, const uint4& w) {
+    if (vec) {
+        *reinterpret_cast<uint4*>(p) = w;
         return;
     }
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < VE; i++)
-        if ((valid >> i) & 1u) out[a + i] = o[i];
+    for (int i = 0; i < kGroup<T>; i++) {
+        if (sizeof(T) == 4)
+            reinterpret_cast<uint32_t*>(p)[i] = u[i & 3];
+        else
+            reinterpret_cast<unsigned short*>(p)[i] = (unsigned short)(u[(i >> 1) & 3] >> ((i & 1) * 16));
+    }
 }
 
-// Whether full groups of `row` are 16-byte aligned in `out` too.
-template <class T>
-__device__ __forceinline__ bool same_alignment(const T* row, const T* out) {
-    return ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-}
-
-// VE bits of a bit row from bit `at` on (all of them inside it).
+// VE bits of a bit row from bit `at` on (all of them inside the row; those
+// above VE are not cleared).
 template <int VE>
 __device__ __forceinline__ uint32_t bit_window(const uint32_t* words, int at) {
-    const uint32_t lo = words[at >> 5], hi = words[(at + VE - 1) >> 5];
-    return __funnelshift_r(lo, hi, at & 31) & ((1u << VE) - 1u);
+    const int sh = at & 31;
+    const uint32_t* w = words + (at >> 5);
+    return __funnelshift_r(w[0], sh + VE > 32 ? w[1] : 0u, sh);
 }
 
-// What the controls did to a group: the elements that may be taken, those that
-// occurred before, and of these those whose raw logit is positive.
-struct GroupControls {
-    uint32_t ok, seen, positive;
-};
-
-// Raw values of group a -> controlled logits (-inf outside `valid` and where
-// the mask says so). The table covers actions from lo.
-template <class T>
-__device__ __forceinline__ GroupControls group_control(const RowControls& r, const HistoryTable& t, const RawGroup<T>& g, int a,
-                                                       int lo, uint32_t valid, float* x) {
-    constexpr int VE = kGroup<T>;
-    constexpr uint32_t ALL = (1u << VE) - 1u;
-    GroupControls c{valid, 0u, 0u};
-#pragma unroll
-    for (int i = 0; i < VE; i++) x[i] = raw_value(g, i);
+// Controls a full group of actions from a on: raw values in x, controlled ones
+// out (-inf where the mask says so). seen: the elements that occurred before
+// (bits above the group are 0); positive: those of them whose raw logit is > 0.
+template <int VE>
+__device__ __forceinline__ void group_control(const RowControls& r, const HistoryTable& t, int a, int lo, float* x,
+                                              uint32_t& seen, uint32_t& positive) {
+    seen = positive = 0;
     if (r.history) {
-        if (valid == ALL) {
-            c.seen = bit_window<VE>(t.seen, a - lo);
-        } else {
+        seen = bit_window<VE>(t.seen, a - lo) & ((1u << VE) - 1u);
+#pragma unroll 1
+        for (uint32_t left = seen; left; left &= left - 1) {  // few: one at a time, in little code
+            const int i = __ffs(left) - 1;
+            float y = 0.0f;
 #pragma unroll
-            for (int i = 0; i < VE; i++)
-                if (((valid >> i) & 1u) && ((t.seen[(a - lo + i) >> 5] >> ((a - lo + i) & 31)) & 1u)) c.seen |= 1u << i;
-        }
-        if (c.seen) {
+            for (int k = 0; k < VE; k++) y = k == i ? x[k] : y;
+            if (y > 0.0f) positive |= 1u << i;
+            y = penalise(r, y, t.count(a - lo + i));
 #pragma unroll
-            for (int i = 0; i < VE; i++)
-                if ((c.seen >> i) & 1u) {
-                    if (x[i] > 0.0f) c.positive |= 1u << i;
-                    x[i] = penalise(r, x[i], t.count(a - lo + i));
-                }
+            for (int k = 0; k < VE; k++) x[k] = k == i ? y : x[k];
         }
     }
     if (r.bias) {
         const float* b = r.bias + a;
-        if (valid == ALL && (reinterpret_cast<uintptr_t>(b) & 15) == 0) {
+        if ((reinterpret_cast<uintptr_t>(b) & 15) == 0) {
 #pragma unroll
             for (int i = 0; i < VE; i += 4) {
                 const float4 q = *reinterpret_cast<const float4*>(b + i);
@@ -302,35 +314,33 @@ __device__ __forceinline__ GroupControls group_control(const RowControls& r, con
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < VE; i++)
-                if ((valid >> i) & 1u) x[i] = __fadd_rn(x[i], b[i]);
+            for (int i = 0; i < VE; i++) x[i] = __fadd_rn(x[i], b[i]);
         }
     }
     if (r.mask) {
-        if (valid == ALL) {
-            c.ok = bit_window<VE>(r.mask, a);
-        } else {
+        const uint32_t ok = bit_window<VE>(r.mask, a);
 #pragma unroll
-            for (int i = 0; i < VE; i++)
-                if (((valid >> i) & 1u) && !((r.mask[(a + i) >> 5] >> ((a + i) & 31)) & 1u)) c.ok &= ~(1u << i);
-        }
+        for (int i = 0; i < VE; i++) x[i] = ((ok >> i) & 1u) ? x[i] : -INFINITY;
     }
-    if (c.ok != ALL) {
-#pragma unroll
-        for (int i = 0; i < VE; i++)
-            if (!((c.ok >> i) & 1u)) x[i] = -INFINITY;
-    }
-    return c;
 }
 
-// Its gradient factor on seen elements.
-template <class T>
-__device__ __forceinline__ void group_factor(const RowControls& r, const GroupControls& c, float* g) {
-    if (c.seen) {
+// The gradient of the raw logits of a group from that of its controlled ones.
+template <int VE>
+__device__ __forceinline__ void group_gradient(const RowControls& r, int a, uint32_t seen, uint32_t positive, float* g) {
+#pragma unroll 1
+    for (uint32_t left = seen; left; left &= left - 1) {
+        const int i = __ffs(left) - 1;
+        float y = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kGroup<T>; i++)
-            if ((c.seen >> i) & 1u)
-                g[i] = ((c.positive >> i) & 1u) ? __fdiv_rn(g[i], r.repetition) : __fmul_rn(g[i], r.repetition);
+        for (int k = 0; k < VE; k++) y = k == i ? g[k] : y;
+        y = ((positive >> i) & 1u) ? __fdiv_rn(y, r.repetition) : __fmul_rn(y, r.repetition);
+#pragma unroll
+        for (int k = 0; k < VE; k++) g[k] = k == i ? y : g[k];
+    }
+    if (r.mask) {
+        const uint32_t ok = bit_window<VE>(r.mask, a);
+#pragma unroll
+        for (int i = 0; i < VE; i++) g[i] = ((ok >> i) & 1u) ? g[i] : 0.0f;
     }
 }
 
