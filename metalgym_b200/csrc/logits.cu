@@ -71,56 +71,51 @@ __device__ __forceinline__ HistoryTable team_table(const TeamPart& p, const mg_l
 
 // ------------------------------------------------------------------ control and its gradient
 
-// Groups of a thread in flight together, and groups a thread has in all (one CTA).
-constexpr int kControlGroups = 2, kControlRounds = 2;
+// The work is cut into units of kUnit actions of a row, and the units are dealt
+// out evenly and in order to as many CTAs as the GPU holds (or warp teams: a
+// row each), so that a CTA fills a row's history table once for all the units
+// it has of the row.
+constexpr int kUnit = 2048;
+constexpr int kControlGroups = 4;  // 16-byte loads of a thread in flight
+constexpr int kControlCtas = 5;    // CTAs an SM holds
 
 template <class T, int NT, bool BACKWARD>
-__global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 6)
-    k_logits_control(const T* logits, int64_t ld, const mg_logit_controls c, const T* dOut, int64_t ldg, T* out,
-                     int64_t ldo, const TeamPart part) {
+__device__ __forceinline__ void control_part(const T* x, const T* src, T* y, const RowControls& r, HistoryTable& t,
+                                             const mg_logit_controls& c, int row, int lo, int hi, uint32_t* sums) {
     constexpr int VE = kGroup<T>, U = kControlGroups;
-    mg_pdl_trigger();
-    mg_pdl_wait();
-    extern __shared__ uint32_t smem[];
-    __shared__ uint32_t sums[kTeamWarps<NT>];
-    int row, lo, hi;
-    if (!team_part<NT>(part, row, lo, hi)) return;
-    const RowControls r = row_controls(c, row);
-    const HistoryTable t = team_table<NT>(part, c, smem);
-    const T* x = logits + (int64_t)row * ld;
-    const T* src = BACKWARD ? dOut + (int64_t)row * ldg : x;
-    T* y = out + (int64_t)row * ldo;
+    const int tid = team_rank<NT>();
     const bool vec = same_alignment(src, y);
     const RowSpan s = row_span(src, lo, hi);
-    const int tid = team_rank<NT>();
-    bool filled = !r.history;
-    for (int g0 = tid; g0 - tid < s.groups || !filled; g0 += NT * U) {
+    if (r.history) {
+        history_fill<NT>(t, c.history + (int64_t)row * c.history_stride, row_history_len(c, row), lo, hi, c.history_max, sums);
+        // the values of the actions that occurred, before anything is written (the call may be in place)
+        for (int j = tid, n = t.total(); j < n; j += NT) {
+            const int a = t.list[j];
+            const float raw = to_f32(x[a]);
+            if (BACKWARD)
+                t.value[j] = allowed(r, a) ? seen_gradient(r, to_f32(src[a]), raw) : 0.0f;
+            else
+                t.value[j] = bias_mask(r, penalise(r, raw, t.count_at(j)), a);
+        }
+        team_sync<NT>();
+    }
+    for (int g0 = tid; g0 < s.groups; g0 += NT * U) {
         uint4 raw[U];
 #pragma unroll
         for (int u = 0; u < U; u++)
             if (g0 + u * NT < s.groups) raw[u] = group_load(src + s.body + (g0 + u * NT) * VE);
-        if (!filled) {  // while the first loads are in flight
-            history_fill<NT>(t, c.history + (int64_t)row * c.history_stride, row_history_len(c, row), lo, hi, c.history_max, sums);
-            filled = true;
-        }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (g0 + u * NT >= s.groups) break;
             const int a = s.body + (g0 + u * NT) * VE;
             float v[VE];
             group_floats(raw[u], src, v);
-            uint32_t seen = 0, positive = 0;
             if (!BACKWARD) {
-                group_control<VE>(r, t, a, lo, v, seen, positive);
-            } else {
-                if (r.history) {  // the raw logits' signs, read only where they count
-                    seen = bit_window<VE>(t.seen, a - lo) & ((1u << VE) - 1u);
-                    for (uint32_t left = seen; left; left &= left - 1) {
-                        const int i = __ffs(left) - 1;
-                        if (to_f32(x[a + i]) > 0.0f) positive |= 1u << i;
-                    }
-                }
-                group_gradient<VE>(r, a, seen, positive, v);
+                group_bias_mask<VE>(r, a, 0u, v);
+            } else if (r.mask) {
+                const uint32_t ok = bit_window<VE>(r.mask, a);
+#pragma unroll
+                for (int i = 0; i < VE; i++) v[i] = (ok & (1u << i)) ? v[i] : 0.0f;
             }
             group_store(y + a, vec, group_pack(v, src));
         }
@@ -129,9 +124,44 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 6)
         const int a = s.edge<VE>(tid);
         if (a >= 0) {
             const float raw = to_f32(src[a]);
-            from_f32(&y[a], BACKWARD ? control_gradient(r, t, raw, r.history ? to_f32(x[a]) : 0.0f, a, lo)
-                                     : controlled(r, t, raw, a, lo));
+            from_f32(&y[a], !BACKWARD ? bias_mask(r, raw, a) : allowed(r, a) ? raw : 0.0f);
         }
+    }
+    if (r.history) {
+        team_sync<NT>();  // the values replace what the pass wrote for these actions
+        for (int j = tid, n = t.total(); j < n; j += NT) from_f32(&y[t.list[j]], t.value[j]);
+        team_sync<NT>();
+    }
+}
+
+template <class T, int NT, bool BACKWARD>
+__global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : kControlCtas)
+    k_logits_control(const T* logits, int64_t ld, const mg_logit_controls c, const T* dOut, int64_t ldg, T* out,
+                     int64_t ldo, const TeamPart part) {
+    mg_pdl_trigger();
+    mg_pdl_wait();
+    extern __shared__ uint32_t smem[];
+    __shared__ uint32_t sums[kTeamWarps<NT>];
+    HistoryTable t = team_table<NT>(part, c, smem);
+    auto run = [&](int row, int lo, int hi) {
+        const T* x = logits + (int64_t)row * ld;
+        control_part<T, NT, BACKWARD>(x, BACKWARD ? dOut + (int64_t)row * ldg : x, out + (int64_t)row * ldo, row_controls(c, row),
+                                      t, c, row, lo, hi, sums);
+    };
+    if (NT == 32) {
+        int row, lo, hi;
+        if (team_part<NT>(part, row, lo, hi)) run(row, lo, hi);
+        return;
+    }
+    const int perRow = part.parts;  // units of a row
+    const int64_t total = (int64_t)part.rows * perRow;
+    int64_t u = total * blockIdx.x / gridDim.x;
+    const int64_t end = total * (blockIdx.x + 1) / gridDim.x;
+    while (u < end) {
+        const int row = (int)(u / perRow), first = (int)(u - (int64_t)row * perRow);
+        const int last = (int)min((int64_t)perRow, first + (end - u));
+        run(row, first * kUnit, min(part.actions, last * kUnit));
+        u += last - first;
     }
 }
 
@@ -190,11 +220,11 @@ struct Softmax {
     }
 };
 
-// Adds N logits (-inf: not allowed) to a warp's statistics and gives their e^(l
-// - max) in e; `raised` is told when m rises. False: nothing allowed so far, e
-// is not set.
-template <int N, class Raised>
-__device__ __forceinline__ bool softmax_group(Softmax& v, const float* x, float* e, Raised raised) {
+// Adds N logits (-inf: not allowed) to a warp's statistics; `raised` is told
+// when m rises, before each(i, e^(l - max)) gets every logit's weight. False:
+// nothing allowed so far, no weights.
+template <int N, class Raised, class Each>
+__device__ __forceinline__ bool softmax_group(Softmax& v, const float* x, Raised raised, Each each) {
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < N; i++) top = fmaxf(top, x[i]);
@@ -216,14 +246,14 @@ __device__ __forceinline__ bool softmax_group(Softmax& v, const float* x, float*
         const float2 w = make_float2(exp2_fast(d.x), exp2_fast(d.y));
         s2 = f2add_rn(s2, w);
         t2 = f2fma_rn(w, d, t2);
-        e[i] = w.x;
-        e[i + 1] = w.y;
+        each(i, w.x);
+        each(i + 1, w.y);
     }
     if (N & 1) {
-        const float d = log2_weight(x[N - 1], v.m);
-        e[N - 1] = exp2_fast(d);
-        s2.x += e[N - 1];
-        t2.x = fmaf(e[N - 1], d, t2.x);
+        const float d = log2_weight(x[N - 1], v.m), w = exp2_fast(d);
+        s2.x += w;
+        t2.x = fmaf(w, d, t2.x);
+        each(N - 1, w);
     }
     v.s += s2.x + s2.y;
     v.t += t2.x + t2.y;
@@ -320,6 +350,53 @@ __device__ inline void row_merge(RowPart& mine, RowPart* warps, RowPart* whole, 
     mine = all;
 }
 
+// Passes the team's part of a row, controlled but without the actions that
+// occurred, to take(l, at, count): whole warps, 16 logits a lane while there
+// are as many, then a group a lane, then the edges.
+template <class T, int NT, class Take>
+__device__ __forceinline__ void row_walk(const T* x, const RowControls& r, const HistoryTable& t, const RowSpan& s, int lo,
+                                         Take take) {
+    constexpr int VE = kGroup<T>, U = 16 / VE;
+    const int tid = team_rank<NT>();
+    auto control = [&](const uint4& raw, int a, float* l) {
+        group_floats(raw, x, l);
+        group_bias_mask<VE>(r, a, r.history ? bit_window<VE>(t.seen, a - lo) : 0u, l);
+    };
+    int g0 = 0;
+    if (s.groups >= NT * U) {
+        uint4 raw[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) raw[u] = group_load(x + s.body + (u * NT + tid) * VE);
+        for (; g0 + NT * U <= s.groups; g0 += NT * U) {
+            const int a = s.body + (g0 + tid) * VE;
+            float l[16];
+#pragma unroll
+            for (int u = 0; u < U; u++) control(raw[u], a + u * NT * VE, l + u * VE);
+            if (g0 + 2 * NT * U <= s.groups) {  // the next loads while these logits are worked on
+#pragma unroll
+                for (int u = 0; u < U; u++) raw[u] = group_load(x + a + (NT * U + u * NT) * VE);
+            }
+            take(l, [&](int i) { return a + (i / VE) * (NT * VE) + i % VE; }, std::integral_constant<int, 16>());
+        }
+    }
+    for (; g0 < s.groups; g0 += NT) {
+        const int g = g0 + tid, a = s.body + g * VE;
+        float l[VE];
+        if (g < s.groups) {
+            control(group_load(x + a), a, l);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VE; i++) l[i] = -INFINITY;
+        }
+        take(l, [&](int i) { return a + i; }, std::integral_constant<int, VE>());
+    }
+    if (s.edges() && tid < 32) {
+        const int a = s.edge<VE>(tid);
+        const float l = a < 0 || (r.history && t.has(a - lo)) ? -INFINITY : bias_mask(r, to_f32(x[a]), a);
+        take(&l, [&](int) { return a; }, std::integral_constant<int, 1>());
+    }
+}
+
 // ------------------------------------------------------------------ draw
 
 // One pass. An action can win only where its time E >= v = (h + 1/2) / 2^32 is
@@ -331,7 +408,6 @@ template <class T, int NT, bool GREEDY>
 __global__ void __launch_bounds__(kCtaThreads<NT>)
     k_logits_sample(const T* logits, int64_t ld, const mg_logit_controls c, uint32_t* rng, int32_t* action,
                     float* logProb, float* entropy, float* value, const TeamPart part) {
-    constexpr int VE = kGroup<T>;
     mg_pdl_trigger();
     mg_pdl_wait();
     extern __shared__ uint32_t smem[];
@@ -342,7 +418,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
     int row, lo, hi;
     if (!team_part<NT>(part, row, lo, hi)) return;
     const RowControls r = row_controls(c, row);
-    const HistoryTable t = team_table<NT>(part, c, smem);
+    HistoryTable t = team_table<NT>(part, c, smem);
     if (r.history)
         history_fill<NT>(t, c.history + (int64_t)row * c.history_stride, row_history_len(c, row), lo, hi, c.history_max, sums);
     const T* x = logits + (int64_t)row * ld;
@@ -353,73 +429,69 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
     const RowSpan s = row_span(x, lo, hi);
     const int tid = team_rank<NT>();
 
-    // N actions from a on (every lane of the warp calls it; -inf where a lane has none)
-    auto take = [&](const float* l, int a, auto count) {
+    // N logits (every lane of the warp calls it; -inf where a lane has none):
+    // the i-th is of action at(i)
+    auto take = [&](const float* l, auto at, auto count) {
         constexpr int N = decltype(count)::value;
-        float e[N];
-        if (!softmax_group<N>(mine.v, l, e, [&](float f) { bound = f > 0.0f ? fminf(bound / f, 3e38f) : 3e38f; })) return;
         if (GREEDY) {
+            softmax_group<N>(mine.v, l, [](float) {}, [](int, float) {});
 #pragma unroll
             for (int i = 0; i < N; i++)
-                if (l[i] > mine.best.logit || (N == 1 && l[i] == mine.best.logit && a + i < mine.best.action)) {
+                if (l[i] > mine.best.logit || (l[i] == mine.best.logit && at(i) < mine.best.action)) {
                     mine.best.logit = l[i];
-                    mine.best.action = a + i;
+                    mine.best.action = at(i);
                 }
             return;
         }
         bool pass = false;
-        const float limit = fminf(bound * 65542.6f, 3e38f);  // 2^16 (1 + 1e-4)
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            uint32_t h = word + (uint32_t)a * 0x9E3779B9u + (uint32_t)i * 0x9E3779B9u;
-            h ^= h >> 16;
-            h *= 0x7feb352du;
-            h ^= h >> 15;
-            h *= 0x846ca68bu;
-            const float f = __uint_as_float(__byte_perm(h, 0x4B000000u, 0x7632));
-            pass = pass || f <= fmaf(limit, e[i], 8388608.0f);
-        }
-        if (__any_sync(0xffffffffu, pass)) {
+        float limit = 0.0f;
+        const bool some = softmax_group<N>(
+            mine.v, l,
+            [&](float f) { bound = f > 0.0f ? fminf(bound / f, 3e38f) : 3e38f; },
+            [&](int i, float e) {
+                if (i == 0) limit = fminf(bound * 65542.6f, 3e38f);  // 2^16 (1 + 1e-4)
+                uint32_t h = word + (uint32_t)at(i) * 0x9E3779B9u;
+                h ^= h >> 16;
+                h *= 0x7feb352du;
+                h ^= h >> 15;
+                h *= 0x846ca68bu;
+                const float f = __uint_as_float(__byte_perm(h, 0x4B000000u, 0x7632));
+                pass = pass || f <= fmaf(limit, e, 8388608.0f);
+            });
+        if (some && __any_sync(0xffffffffu, pass)) {
             float least = 3e38f;
             if (pass) {
-#pragma unroll
+#pragma unroll 1
                 for (int i = 0; i < N; i++) {
-                    const uint32_t h = race_bits(word, a + i);
-                    const float f = (float)(h >> 16);
-                    if (l[i] > -INFINITY && f <= limit * e[i]) {
+                    float li = l[0];
+#pragma unroll
+                    for (int k = 1; k < N; k++) li = k == i ? l[k] : li;
+                    const uint32_t h = race_bits(word, at(i));
+                    const float e = exp2_fast(log2_weight(li, mine.v.m));
+                    if (li > -INFINITY && (float)(h >> 16) <= limit * e) {
                         // -log(1 - v) from whichever of v and 1 - v is small
                         const float time = h < 0x80000000u ? -log1pf(-((float)h + 0.5f) * 2.3283064e-10f)
                                                            : -logf(((float)(~h) + 0.5f) * 2.3283064e-10f);
                         Runner o;
-                        o.key = l[i] - logf(time);
-                        o.logit = l[i];
+                        o.key = li - logf(time);
+                        o.logit = li;
                         o.bits = h;
-                        o.action = a + i;
+                        o.action = at(i);
                         if (beats<false>(o, mine.best)) mine.best = o;
-                        least = fminf(least, time / e[i]);
+                        least = fminf(least, time / e);
                     }
                 }
             }
             bound = fminf(bound, __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least))));
         }
     };
-    for (int g0 = 0; g0 < s.groups; g0 += NT) {
-        const int g = g0 + tid, a = s.body + g * VE;
-        float l[VE];
-        if (g < s.groups) {
-            group_floats(group_load(x + a), x, l);
-            uint32_t seen, positive;
-            group_control<VE>(r, t, a, lo, l, seen, positive);
-        } else {
-#pragma unroll
-            for (int i = 0; i < VE; i++) l[i] = -INFINITY;
+    row_walk<T, NT>(x, r, t, s, lo, take);
+    if (r.history) {
+        for (int j0 = 0, n = t.total(); j0 < n; j0 += NT) {
+            const int j = j0 + tid, a = j < n ? (int)t.list[j] : 0;
+            const float l = j < n ? bias_mask(r, penalise(r, to_f32(x[a]), t.count_at(j)), a) : -INFINITY;
+            take(&l, [&](int) { return a; }, std::integral_constant<int, 1>());
         }
-        take(l, a, std::integral_constant<int, VE>());
-    }
-    if (s.edges() && tid < 32) {
-        const int a = s.edge<VE>(tid);
-        const float l = a >= 0 ? controlled(r, t, to_f32(x[a]), a, lo) : -INFINITY;
-        take(&l, a, std::integral_constant<int, 1>());
     }
     row_merge<NT, true, GREEDY>(mine, warps, whole, part.parts, 0);
     if (tid == 0 && lo == 0) {
@@ -462,7 +534,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
     if (!team_part<NT>(part, row, lo, hi)) return;
     const int actions = part.actions, tid = team_rank<NT>();
     const RowControls r = row_controls(c, row);
-    const HistoryTable t = team_table<NT>(part, c, smem);
+    HistoryTable t = team_table<NT>(part, c, smem);
     const T* x = logits + (int64_t)row * ld;
     T* d = dLogits + (int64_t)row * ldd;
     const int act = L.action[row];
@@ -479,23 +551,23 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
     RowPart mine;
     mine.chosen = act >= lo && act < hi ? controlled(r, t, to_f32(x[act]), act, lo) : 0.0f;
     const RowSpan s = row_span(x, lo, hi);
-    for (int g0 = 0; g0 < s.groups; g0 += NT) {
-        const int g = g0 + tid, a = s.body + g * VE;
-        float l[VE], e[VE];
-        if (g < s.groups) {
-            group_floats(group_load(x + a), x, l);
-            uint32_t seen, positive;
-            group_control<VE>(r, t, a, lo, l, seen, positive);
-        } else {
-#pragma unroll
-            for (int i = 0; i < VE; i++) l[i] = -INFINITY;
+    auto take = [&](const float* l, auto, auto count) {
+        softmax_group<decltype(count)::value>(mine.v, l, [](float) {}, [](int, float) {});
+    };
+    row_walk<T, NT>(x, r, t, s, lo, take);
+    if (r.history) {
+        for (int j0 = 0, n = t.total(); j0 < n; j0 += NT) {
+            const int j = j0 + tid;
+            float l = -INFINITY;
+            if (j < n) {
+                const int a = t.list[j];
+                const float raw = to_f32(x[a]);
+                l = bias_mask(r, penalise(r, raw, t.count_at(j)), a);
+                t.value[j] = l;
+                if (raw > 0.0f) t.list[j] = (uint32_t)a | 0x80000000u;  // the sign, for the gradient
+            }
+            take(&l, 0, std::integral_constant<int, 1>());
         }
-        softmax_group<VE>(mine.v, l, e, [](float) {});
-    }
-    if (s.edges() && tid < 32) {
-        const int a = s.edge<VE>(tid);
-        float l = a >= 0 ? controlled(r, t, to_f32(x[a]), a, lo) : -INFINITY, e;
-        softmax_group<1>(mine.v, &l, &e, [](float) {});
     }
     row_merge<NT, false, false>(mine, warps, whole, part.parts, act / part.span);
     const float m = mine.v.m, ls = log2f(mine.v.s), entropy = (ls - mine.v.t / mine.v.s) * kLn2;
@@ -513,41 +585,60 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
         __syncthreads();
     // dl = scale (slope (1[a = act] - p) + ent p (ln p + H)) = p (s1 log2 p + (ent H - slope) scale), + s0 at act
     const float s0 = slope * L.scale, s1 = L.entropyCoef * L.scale * kLn2, sh = fmaf(L.entropyCoef * L.scale, entropy, -s0);
-    const bool vec = same_alignment(x, d);
-    for (int g = tid; g < s.groups; g += NT) {
-        const int a = s.body + g * VE;
-        float l[VE];
-        group_floats(group_load(x + a), x, l);
-        uint32_t seen, positive;
-        group_control<VE>(r, t, a, lo, l, seen, positive);
-        const float2 k2 = make_float2(kLog2e, kLog2e), m2 = make_float2(-m, -m), ls2 = make_float2(-ls, -ls);
-        const float2 s12 = make_float2(s1, s1), sh2 = make_float2(sh, sh);
+    const bool vec = same_alignment(x, d), all_nan = !(fabsf(sh) < INFINITY && fabsf(s1) < INFINITY);
+    auto gradient = [&](float l, int a) {
+        const float q = log2_weight(l, m) - ls;
+        const float g = exp2_fast(q) * fmaf(s1, q, sh);
+        return a == act ? g + s0 : g;
+    };
+    constexpr int U = 2;
+    for (int g0 = tid; g0 < s.groups; g0 += NT * U) {
+        uint4 raw[U];
 #pragma unroll
-        for (int i = 0; i < VE; i += 2) {
-            float2 q = f2fma_rn(make_float2(l[i], l[i + 1]), k2, m2);
-            q.x = max_nan(q.x, -1e30f);
-            q.y = max_nan(q.y, -1e30f);
-            q = f2add_rn(q, ls2);
-            const float2 p = make_float2(exp2_fast(q.x), exp2_fast(q.y));
-            const float2 o = f2mul_rn(p, f2fma_rn(s12, q, sh2));
-            l[i] = o.x;
-            l[i + 1] = o.y;
-        }
-        if ((unsigned)(act - a) < (unsigned)VE) {
+        for (int u = 0; u < U; u++)
+            if (g0 + u * NT < s.groups) raw[u] = group_load(x + s.body + (g0 + u * NT) * VE);
 #pragma unroll
-            for (int i = 0; i < VE; i++) l[i] = a + i == act ? l[i] + s0 : l[i];
+        for (int u = 0; u < U; u++) {
+            if (g0 + u * NT >= s.groups) break;
+            const int a = s.body + (g0 + u * NT) * VE;
+            float l[VE];
+            group_floats(raw[u], x, l);
+            group_bias_mask<VE>(r, a, 0u, l);
+            const float2 k2 = make_float2(kLog2e, kLog2e), m2 = make_float2(-m, -m), ls2 = make_float2(-ls, -ls);
+            const float2 s12 = make_float2(s1, s1), sh2 = make_float2(sh, sh);
+#pragma unroll
+            for (int i = 0; i < VE; i += 2) {
+                float2 q = f2fma_rn(make_float2(l[i], l[i + 1]), k2, m2);
+                q.x = max_nan(q.x, -1e30f);
+                q.y = max_nan(q.y, -1e30f);
+                q = f2add_rn(q, ls2);
+                const float2 p = make_float2(exp2_fast(q.x), exp2_fast(q.y));
+                const float2 o = f2mul_rn(p, f2fma_rn(s12, q, sh2));
+                l[i] = o.x;
+                l[i + 1] = o.y;
+            }
+            if ((unsigned)(act - a) < (unsigned)VE) {
+#pragma unroll
+                for (int i = 0; i < VE; i++) l[i] = a + i == act ? l[i] + s0 : l[i];
+            }
+            if (r.mask && all_nan) {  // a NaN somewhere in the row: still 0 where the mask says so
+                const uint32_t ok = bit_window<VE>(r.mask, a);
+#pragma unroll
+                for (int i = 0; i < VE; i++) l[i] = (ok & (1u << i)) ? l[i] : 0.0f;
+            }
+            group_store(d + a, vec, group_pack(l, x));
         }
-        group_gradient<VE>(r, a, seen, positive, l);
-        group_store(d + a, vec, group_pack(l, x));
     }
     if (s.edges() && tid < 32) {
         const int a = s.edge<VE>(tid);
-        if (a >= 0) {
-            const float raw = to_f32(x[a]);
-            const float q = log2_weight(controlled(r, t, raw, a, lo), m) - ls;
-            float g = exp2_fast(q) * fmaf(s1, q, sh);
-            if (a == act) g += s0;
-            from_f32(&d[a], control_gradient(r, t, g, raw, a, lo));
+        if (a >= 0) from_f32(&d[a], allowed(r, a) ? gradient(bias_mask(r, to_f32(x[a]), a), a) : 0.0f);
+    }
+    if (r.history) {  // the actions that occurred, over what the pass wrote for them
+        team_sync<NT>();
+        for (int j = tid, n = t.total(); j < n; j += NT) {
+            const int a = t.list[j] & 0x7fffffff;
+            const float g = gradient(t.value[j], a);
+            from_f32(&d[a], allowed(r, a) ? ((t.list[j] >> 31) ? __fdiv_rn(g, r.repetition) : __fmul_rn(g, r.repetition)) : 0.0f);
         }
     }
     if (tid == 0 && lo == 0) {
@@ -622,7 +713,8 @@ size_t table_smem(const TeamPart& p) {
     return (size_t)p.tableBytes * (NT == 32 ? kWarpRows : 1);
 }
 
-constexpr int kTableSmemMax = 100 * 1024;  // >= the largest table, and >= eight of kWarpActions actions
+// the largest table (2^18 actions, 2^14 entries); eight of kWarpActions actions take less
+constexpr int kTableSmemMax = 216 * 1024;
 
 // A launch of rows x parts CTAs (or warp teams), the parts of a row in one cluster.
 template <int NT, class... KArgs, class... Args>
@@ -666,13 +758,14 @@ int launch_control(const void* logits, int64_t ld, const mg_logit_controls& c, c
     static std::atomic<uint64_t> done{0};
     MG_TRY(smem_limit_once(kern, kTableSmemMax, done));
     TeamPart p = plan(NT, rows, actions, 1, c.history_max);
-    if (NT > 32) {  // independent chunks, no cluster
-        p.span = std::min(actions, NT * kControlGroups * kControlRounds * kGroup<T>);
-        p.parts = (actions + p.span - 1) / p.span;
+    int64_t ctas = ((int64_t)rows + kWarpRows - 1) / kWarpRows;
+    if (NT > 32) {
+        p.parts = (actions + kUnit - 1) / kUnit;
+        const int64_t units = (int64_t)rows * p.parts;
+        ctas = std::min(units, (int64_t)num_sms() * kControlCtas);
+        p.span = (int)std::min((int64_t)actions, (units + ctas - 1) / ctas * kUnit);
         p.tableBytes = c.history ? (int)HistoryTable::bytes(p.span, c.history_max) : 0;
     }
-    const int64_t ctas = NT == 32 ? ((int64_t)rows + kWarpRows - 1) / kWarpRows : (int64_t)rows * p.parts;
-    MG_CHECK_ARG(ctas <= INT32_MAX, "logits_control: too many rows");
     MG_CUDA_TRY(MG_LAUNCH(kern, (unsigned)ctas, kCtaThreads<NT>, table_smem<NT>(p), st, static_cast<const T*>(logits), ld, c,
                           static_cast<const T*>(dOut), ldg, static_cast<T*>(out), ldo, p));
     return check_launch("k_logits_control");

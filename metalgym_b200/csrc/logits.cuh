@@ -29,31 +29,43 @@ __device__ __forceinline__ void from_f32(__nv_bfloat16* p, float x) { *p = __flo
 __device__ __forceinline__ void from_f32(__half* p, float x) { *p = __float2half_rn(x); }
 
 // The occurrences of actions [lo, hi) in one row's history, in shared memory:
-// a bit per action, the number of set bits before each word, and a 16-bit
-// count per set bit. Whole numbers only, so the order of the atomics that
-// fill it does not matter. A row's history names few of its actions: the bits
-// cost 1/32 word an action, and only actions that occurred look a count up.
+// a bit per action, the number of set bits before each word, and for each set
+// bit (in the order of the actions) its action, a 16-bit count and a place
+// for a value. A history names few of a row's actions: the passes over a row
+// leave them out by their bits, at 1/32 word an action, and the list is done
+// one by one, in an order that does not depend on the atomics that fill the
+// table (they add whole numbers).
 struct HistoryTable {
     uint32_t* seen;    // [words]
-    uint16_t* before;  // [words]
     uint32_t* counts;  // two 16-bit counts a word
+    uint32_t* list;    // actions
+    float* value;
+    uint16_t* before;  // [words]
+    int words;
 
-    __host__ __device__ static int words(int span) { return (span + 31) / 32; }
-    __host__ __device__ static int count_words(int span, int history) { return ((span < history ? span : history) + 1) / 2; }
+    __host__ __device__ static int words_of(int span) { return (span + 31) / 32; }
+    __host__ __device__ static int entries(int span, int history) { return span < history ? span : history; }
     __host__ __device__ static size_t bytes(int span, int history) {
-        return (size_t)words(span) * 4 + (size_t)count_words(span, history) * 4 + (size_t)(words(span) + 1) / 2 * 4;
+        const int w = words_of(span), n = entries(span, history);
+        return (size_t)w * 4 + (size_t)((n + 1) / 2) * 4 + (size_t)n * 8 + (size_t)((w + 1) / 2) * 4;
     }
     __device__ void place(void* smem, int span, int history) {
+        const int w = words_of(span), n = entries(span, history);
         seen = static_cast<uint32_t*>(smem);
-        counts = seen + words(span);
-        before = reinterpret_cast<uint16_t*>(counts + count_words(span, history));
+        counts = seen + w;
+        list = counts + (n + 1) / 2;
+        value = reinterpret_cast<float*>(list + n);
+        before = reinterpret_cast<uint16_t*>(value + n);
+        words = 0;
     }
+    // Actions that occurred (after history_fill).
+    __device__ __forceinline__ int total() const { return before[words - 1] + __popc(seen[words - 1]); }
+    __device__ __forceinline__ int count_at(int at) const { return (counts[at >> 1] >> ((at & 1) * 16)) & 0xffff; }
+    __device__ __forceinline__ bool has(int i) const { return (seen[i >> 5] >> (i & 31)) & 1u; }
     // Number of occurrences of action lo + i.
     __device__ __forceinline__ int count(int i) const {
         const uint32_t w = seen[i >> 5], bit = 1u << (i & 31);
-        if (!(w & bit)) return 0;
-        const int at = before[i >> 5] + __popc(w & (bit - 1u));
-        return (counts[at >> 1] >> ((at & 1) * 16)) & 0xffff;
+        return (w & bit) ? count_at(before[i >> 5] + __popc(w & (bit - 1u))) : 0;
     }
 };
 
@@ -70,9 +82,10 @@ __device__ __forceinline__ void team_sync() {
 // per warp. The first entries of a thread stay in registers between the two
 // passes over the history.
 template <int NT>
-__device__ inline void history_fill(const HistoryTable& t, const int32_t* history, int n, int lo, int hi, int capacity,
+__device__ inline void history_fill(HistoryTable& t, const int32_t* history, int n, int lo, int hi, int capacity,
                                     uint32_t* sums) {
-    const int span = hi - lo, words = HistoryTable::words(span), cw = HistoryTable::count_words(span, capacity);
+    const int span = hi - lo, words = HistoryTable::words_of(span), cw = (HistoryTable::entries(span, capacity) + 1) / 2;
+    t.words = words;
     const int tid = NT == 32 ? threadIdx.x & 31 : threadIdx.x;
     constexpr int nt = NT, KEEP = 4;
     int kept[KEEP];
@@ -114,6 +127,7 @@ __device__ inline void history_fill(const HistoryTable& t, const int32_t* histor
         if (a < lo || a >= hi) return;
         const int k = a - lo;
         const int at = t.before[k >> 5] + __popc(t.seen[k >> 5] & ((1u << (k & 31)) - 1u));
+        t.list[at] = (uint32_t)a;
         atomicAdd(&t.counts[at >> 1], 1u << ((at & 1) * 16));
     };
 #pragma unroll
@@ -156,19 +170,19 @@ __device__ __forceinline__ float penalise(const RowControls& r, float x, int n) 
     return __fsub_rn(__fsub_rn(x, __fmul_rn(r.frequency, (float)n)), r.presence);
 }
 
-// The controlled logit of action a (raw x); the table covers actions from lo.
-__device__ __forceinline__ float controlled(const RowControls& r, const HistoryTable& t, float x, int a, int lo) {
-    if (r.history) {
-        const int n = t.count(a - lo);
-        if (n > 0) x = penalise(r, x, n);
-    }
+// Bias and mask of action a.
+__device__ __forceinline__ float bias_mask(const RowControls& r, float x, int a) {
     if (r.bias) x = __fadd_rn(x, r.bias[a]);
     return allowed(r, a) ? x : -INFINITY;
 }
-// The gradient of an action's raw logit x from that of its controlled one.
-__device__ __forceinline__ float control_gradient(const RowControls& r, const HistoryTable& t, float g, float x, int a, int lo) {
-    if (r.history && t.count(a - lo) > 0) g = x > 0.0f ? __fdiv_rn(g, r.repetition) : __fmul_rn(g, r.repetition);
-    return allowed(r, a) ? g : 0.0f;
+// The controlled logit of action a (raw x); the table covers actions from lo.
+__device__ __forceinline__ float controlled(const RowControls& r, const HistoryTable& t, float x, int a, int lo) {
+    const int n = r.history ? t.count(a - lo) : 0;
+    return bias_mask(r, n > 0 ? penalise(r, x, n) : x, a);
+}
+// The gradient of the raw logit x of an action that occurred.
+__device__ __forceinline__ float seen_gradient(const RowControls& r, float g, float x) {
+    return x > 0.0f ? __fdiv_rn(g, r.repetition) : __fmul_rn(g, r.repetition);
 }
 
 // ------------------------------------------------------------------ groups
@@ -280,27 +294,10 @@ __device__ __forceinline__ uint32_t bit_window(const uint32_t* words, int at) {
     return __funnelshift_r(w[0], sh + VE > 32 ? w[1] : 0u, sh);
 }
 
-// Controls a full group of actions from a on: raw values in x, controlled ones
-// out (-inf where the mask says so). seen: the elements that occurred before
-// (bits above the group are 0); positive: those of them whose raw logit is > 0.
+// Bias and mask of a full group of actions from a on (-inf where the mask says
+// so, and where `skip` has a bit).
 template <int VE>
-__device__ __forceinline__ void group_control(const RowControls& r, const HistoryTable& t, int a, int lo, float* x,
-                                              uint32_t& seen, uint32_t& positive) {
-    seen = positive = 0;
-    if (r.history) {
-        seen = bit_window<VE>(t.seen, a - lo) & ((1u << VE) - 1u);
-#pragma unroll 1
-        for (uint32_t left = seen; left; left &= left - 1) {  // few: one at a time, in little code
-            const int i = __ffs(left) - 1;
-            float y = 0.0f;
-#pragma unroll
-            for (int k = 0; k < VE; k++) y = k == i ? x[k] : y;
-            if (y > 0.0f) positive |= 1u << i;
-            y = penalise(r, y, t.count(a - lo + i));
-#pragma unroll
-            for (int k = 0; k < VE; k++) x[k] = k == i ? y : x[k];
-        }
-    }
+__device__ __forceinline__ void group_bias_mask(const RowControls& r, int a, uint32_t skip, float* x) {
     if (r.bias) {
         const float* b = r.bias + a;
         if ((reinterpret_cast<uintptr_t>(b) & 15) == 0) {
@@ -317,30 +314,11 @@ __device__ __forceinline__ void group_control(const RowControls& r, const Histor
             for (int i = 0; i < VE; i++) x[i] = __fadd_rn(x[i], b[i]);
         }
     }
-    if (r.mask) {
-        const uint32_t ok = bit_window<VE>(r.mask, a);
+    uint32_t out = skip;
+    if (r.mask) out |= ~bit_window<VE>(r.mask, a);
+    if (r.mask || r.history) {
 #pragma unroll
-        for (int i = 0; i < VE; i++) x[i] = ((ok >> i) & 1u) ? x[i] : -INFINITY;
-    }
-}
-
-// The gradient of the raw logits of a group from that of its controlled ones.
-template <int VE>
-__device__ __forceinline__ void group_gradient(const RowControls& r, int a, uint32_t seen, uint32_t positive, float* g) {
-#pragma unroll 1
-    for (uint32_t left = seen; left; left &= left - 1) {
-        const int i = __ffs(left) - 1;
-        float y = 0.0f;
-#pragma unroll
-        for (int k = 0; k < VE; k++) y = k == i ? g[k] : y;
-        y = ((positive >> i) & 1u) ? __fdiv_rn(y, r.repetition) : __fmul_rn(y, r.repetition);
-#pragma unroll
-        for (int k = 0; k < VE; k++) g[k] = k == i ? y : g[k];
-    }
-    if (r.mask) {
-        const uint32_t ok = bit_window<VE>(r.mask, a);
-#pragma unroll
-        for (int i = 0; i < VE; i++) g[i] = ((ok >> i) & 1u) ? g[i] : 0.0f;
+        for (int i = 0; i < VE; i++) x[i] = (out & (1u << i)) ? -INFINITY : x[i];
     }
 }
 
