@@ -265,6 +265,13 @@ __device__ __forceinline__ double race_key(uint32_t h, float l) {
     return (double)l - log(-log1p(-((double)h + 0.5) * (1.0 / 4294967296.0)));
 }
 
+// Floats as integers of the same order, and back.
+__device__ __forceinline__ int float_order(float x) {
+    const int i = __float_as_int(x);
+    return i >= 0 ? i : i ^ 0x7fffffff;
+}
+__device__ __forceinline__ float ordered_float(int i) { return __int_as_float(i >= 0 ? i : i ^ 0x7fffffff); }
+
 // A runner of the race: its key in 32 bits, and what gives the key in 64.
 struct Runner {
     float key = -INFINITY, logit = -INFINITY;
@@ -426,6 +433,11 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
     if (!GREEDY) rngNext(word);
     RowPart mine;
     float bound = 3e38f;  // the warp's best ratio E / e^(l - m)
+    __shared__ int sharedBound;  // the CTA's, as an ordered log2 (E / e^l)
+    if (NT > 32 && !GREEDY) {
+        if (threadIdx.x == 0) sharedBound = 0x7f800000;
+        __syncthreads();
+    }
     const RowSpan s = row_span(x, lo, hi);
     const int tid = team_rank<NT>();
 
@@ -443,46 +455,51 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
                 }
             return;
         }
-        bool pass = false;
+        uint32_t pass = 0;
         float limit = 0.0f;
-        const bool some = softmax_group<N>(
-            mine.v, l,
-            [&](float f) { bound = f > 0.0f ? fminf(bound / f, 3e38f) : 3e38f; },
-            [&](int i, float e) {
-                if (i == 0) limit = fminf(bound * 65542.6f, 3e38f);  // 2^16 (1 + 1e-4)
-                uint32_t h = word + (uint32_t)at(i) * 0x9E3779B9u;
-                h ^= h >> 16;
-                h *= 0x7feb352du;
-                h ^= h >> 15;
-                h *= 0x846ca68bu;
-                const float f = __uint_as_float(__byte_perm(h, 0x4B000000u, 0x7632));
-                pass = pass || f <= fmaf(limit, e, 8388608.0f);
-            });
-        if (some && __any_sync(0xffffffffu, pass)) {
-            float least = 3e38f;
+        auto raised = [&](float f) { bound = f > 0.0f ? fminf(bound / f, 3e38f) : 3e38f; };
+        const bool some = softmax_group<N>(mine.v, l, raised, [&](int i, float e) {
+            if (i == 0) {
+                if (NT > 32) bound = fminf(bound, exp2_fast(ordered_float(*(volatile int*)&sharedBound) + mine.v.m));
+                limit = fminf(bound * 65542.6f, 3e38f);  // 2^16 (1 + 1e-4)
+            }
+            uint32_t h = word + (uint32_t)at(i) * 0x9E3779B9u;
+            h ^= h >> 16;
+            h *= 0x7feb352du;
+            h ^= h >> 15;
+            h *= 0x846ca68bu;
+            const float f = __uint_as_float(__byte_perm(h, 0x4B000000u, 0x7632));
+            if (f <= fmaf(limit, e, 8388608.0f)) pass |= 1u << i;
+        });
+        // the lanes' candidates, one a lane at a time, each against the bound that the ones before it left
+        while (some && __any_sync(0xffffffffu, pass != 0)) {
+            float ratio = 3e38f;
             if (pass) {
-#pragma unroll 1
-                for (int i = 0; i < N; i++) {
-                    float li = l[0];
+                const int i = __ffs(pass) - 1;
+                pass &= pass - 1;
+                float li = l[0];
 #pragma unroll
-                    for (int k = 1; k < N; k++) li = k == i ? l[k] : li;
-                    const uint32_t h = race_bits(word, at(i));
-                    const float e = exp2_fast(log2_weight(li, mine.v.m));
-                    if (li > -INFINITY && (float)(h >> 16) <= limit * e) {
-                        // -log(1 - v) from whichever of v and 1 - v is small
-                        const float time = h < 0x80000000u ? -log1pf(-((float)h + 0.5f) * 2.3283064e-10f)
-                                                           : -logf(((float)(~h) + 0.5f) * 2.3283064e-10f);
-                        Runner o;
-                        o.key = li - logf(time);
-                        o.logit = li;
-                        o.bits = h;
-                        o.action = at(i);
-                        if (beats<false>(o, mine.best)) mine.best = o;
-                        least = fminf(least, time / e);
-                    }
+                for (int k = 1; k < N; k++) li = k == i ? l[k] : li;
+                const uint32_t h = race_bits(word, at(i));
+                const float e = exp2_fast(log2_weight(li, mine.v.m));
+                if (li > -INFINITY && (float)(h >> 16) <= bound * 65542.6f * e) {
+                    // -log(1 - v) from whichever of v and 1 - v is small
+                    const float time = h < 0x80000000u ? -log1pf(-((float)h + 0.5f) * 2.3283064e-10f)
+                                                       : -logf(((float)(~h) + 0.5f) * 2.3283064e-10f);
+                    Runner o;
+                    o.key = li - logf(time);
+                    o.logit = li;
+                    o.bits = h;
+                    o.action = at(i);
+                    if (beats<false>(o, mine.best)) mine.best = o;
+                    ratio = time / e;
                 }
             }
-            bound = fminf(bound, __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(least))));
+            const float least = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(ratio)));
+            if (least < bound) {
+                bound = least;
+                if (NT > 32 && (threadIdx.x & 31) == 0) atomicMin(&sharedBound, float_order(log2f(least) - mine.v.m));
+            }
         }
     };
     row_walk<T, NT>(x, r, t, s, lo, take);
