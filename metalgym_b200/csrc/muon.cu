@@ -47,24 +47,26 @@ struct MuonShape {
 };
 
 constexpr int kPrepThreads = 256;
-constexpr int kPrepParts = 64;  // CTAs (and norm partials) per matrix
+constexpr int kPrepWarps = kPrepThreads / 32;
+constexpr int kPrepMaxParts = 1024;  // CTAs (and norm partials) per matrix at most
 
 // U into X32 (not yet divided by its norm) and one 64-bit sum of squares a CTA:
-// the squares of any finite fp32 U neither overflow nor vanish in 64 bits.
-template <class T, bool MUON>
+// the squares of any finite fp32 U neither overflow nor vanish in 64 bits. A
+// warp takes a row, a lane V columns at a time.
+template <class T, bool MUON, int V>
 __global__ void __launch_bounds__(kPrepThreads)
     k_muon_prepare(const MuonInput in, MuonShape s, float* x32, double* partial) {
     mg_pdl_trigger();
     mg_pdl_wait();
     __shared__ float sScale;
-    __shared__ double sSum[kPrepThreads / 32];
-    const int b = blockIdx.y;
+    __shared__ double sSum[kPrepWarps];
+    const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (MUON) {
-        if (threadIdx.x < 32) {  // the clip factor, as the Adam step forms it
+        if (warp == 0) {  // the clip factor, as the Adam step forms it
             float sum = 0.0f;
-            for (int i = threadIdx.x; i < in.nNorm; i += 32) sum = __fadd_rn(sum, in.normPartial[i]);
+            for (int i = lane; i < in.nNorm; i += 32) sum = __fadd_rn(sum, in.normPartial[i]);
             sum = warp_sum(sum);
-            if (threadIdx.x == 0) {
+            if (lane == 0) {
                 const float norm = __fsqrt_rn(sum);
                 sScale = (in.maxGradNorm > 0.0f && norm > in.maxGradNorm)
                              ? __fdiv_rn(in.maxGradNorm, __fadd_rn(norm, 1e-6f))
@@ -74,65 +76,119 @@ __global__ void __launch_bounds__(kPrepThreads)
         }
         __syncthreads();
     }
+    // the matrix in pieces of V columns, dealt out evenly and in order
+    const int perRow = (s.cols + V - 1) / V;
+    const int64_t total = (int64_t)s.rows * perRow;
+    const int64_t first = total * blockIdx.x / gridDim.x, end = total * (blockIdx.x + 1) / gridDim.x;
     double sum = 0.0;
-    for (int r = blockIdx.x; r < s.rows; r += gridDim.x) {
-        float* dst = x32 + ((int64_t)b * s.rows + r) * s.ldx;
-        for (int c = threadIdx.x; c < s.cols; c += kPrepThreads) {
-            float u;
-            if (MUON) {
-                const int64_t i = (int64_t)b * in.stride + (int64_t)r * s.cols + c;
-                const float g = __fmul_rn(in.grad[i], sScale);
-                const float m = __fadd_rn(__fmul_rn(in.decay, in.momentum[i]), g);
-                in.momentum[i] = m;
-                u = in.nesterov ? __fadd_rn(g, __fmul_rn(in.decay, m)) : m;
+    for (int64_t i = first + threadIdx.x; i < end; i += kPrepThreads) {
+        const int r = (int)(i / perRow), c = (int)(i - (int64_t)r * perRow) * V;
+        float* dst = x32 + ((int64_t)b * s.rows + r) * s.ldx + c;
+        float u[V];
+        if (MUON) {
+            const int64_t at = (int64_t)b * in.stride + (int64_t)r * s.cols + c;
+            float g[V], m[V];
+            if (V == 4) {
+                *reinterpret_cast<float4*>(g) = *reinterpret_cast<const float4*>(in.grad + at);
+                *reinterpret_cast<float4*>(m) = *reinterpret_cast<const float4*>(in.momentum + at);
             } else {
-                u = to_f32(static_cast<const T*>(in.x)[(int64_t)b * in.stride + (int64_t)r * in.ld + c]);
+                g[0] = in.grad[at];
+                m[0] = in.momentum[at];
             }
-            dst[c] = u;
-            sum += (double)u * (double)u;
+#pragma unroll
+            for (int k = 0; k < V; k++) {
+                g[k] = __fmul_rn(g[k], sScale);
+                m[k] = __fadd_rn(__fmul_rn(in.decay, m[k]), g[k]);
+                u[k] = in.nesterov ? __fadd_rn(g[k], __fmul_rn(in.decay, m[k])) : m[k];
+            }
+            if (V == 4)
+                *reinterpret_cast<float4*>(in.momentum + at) = *reinterpret_cast<const float4*>(m);
+            else
+                in.momentum[at] = m[0];
+        } else {
+            const T* src = static_cast<const T*>(in.x) + (int64_t)b * in.stride + (int64_t)r * in.ld + c;
+            if (V == 4) {
+                T raw[4];
+                if (sizeof(T) == 4)
+                    *reinterpret_cast<float4*>(raw) = *reinterpret_cast<const float4*>(src);
+                else
+                    *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(src);
+#pragma unroll
+                for (int k = 0; k < V; k++) u[k] = to_f32(raw[k]);
+            } else {
+                u[0] = to_f32(src[0]);
+            }
         }
+        if (V == 4)
+            *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(u);
+        else
+            dst[0] = u[0];
+#pragma unroll
+        for (int k = 0; k < V; k++) sum += (double)u[k] * (double)u[k];
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if ((threadIdx.x & 31) == 0) sSum[threadIdx.x >> 5] = sum;
+    if (lane == 0) sSum[warp] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < kPrepThreads / 32; w++) sum += sSum[w];
-        partial[(int64_t)b * kPrepParts + blockIdx.x] = sum;
+        for (int w = 1; w < kPrepWarps; w++) sum += sSum[w];
+        partial[(int64_t)b * kPrepMaxParts + blockIdx.x] = sum;
     }
 }
 
-// X = U / |U| (0 for a zero U), and its fp16 copy.
+// X = U / |U| (0 for a zero U), and its fp16 copy; four columns a thread (the
+// workspace's rows are padded to eight).
 __global__ void __launch_bounds__(kPrepThreads)
     k_muon_normalise(MuonShape s, float* x32, __half* x16, const double* partial, int parts) {
     mg_pdl_trigger();
     mg_pdl_wait();
-    __shared__ double sInv;
-    const int b = blockIdx.y;
-    if (threadIdx.x == 0) {
-        double sum = 0.0;
-        for (int i = 0; i < parts; i++) sum += partial[(int64_t)b * kPrepParts + i];
-        sInv = sum == 0.0 ? 0.0 : 1.0 / sqrt(sum);
-    }
+    __shared__ double sSum[kPrepWarps];
+    const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < parts; i += kPrepThreads) sum += partial[(int64_t)b * kPrepMaxParts + i];
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) sSum[warp] = sum;
     __syncthreads();
-    for (int r = blockIdx.x; r < s.rows; r += gridDim.x) {
-        const int64_t at = ((int64_t)b * s.rows + r) * s.ldx;
-        for (int c = threadIdx.x; c < s.cols; c += kPrepThreads) {
-            const float v = (float)((double)x32[at + c] * sInv);
-            x32[at + c] = v;
-            x16[at + c] = __float2half_rn(v * kNsScale);
-        }
+    sum = sSum[0];
+    for (int w = 1; w < kPrepWarps; w++) sum += sSum[w];
+    const double inv = sum == 0.0 ? 0.0 : 1.0 / sqrt(sum);
+    const int64_t total = (int64_t)s.rows * s.ldx / 4;
+    float4* x = reinterpret_cast<float4*>(x32 + (int64_t)b * s.rows * s.ldx);
+    uint2* h = reinterpret_cast<uint2*>(x16 + (int64_t)b * s.rows * s.ldx);
+    for (int64_t i = (int64_t)blockIdx.x * kPrepThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kPrepThreads) {
+        float4 v = x[i];  // (the padding's values are never read as operands)
+        v.x = (float)((double)v.x * inv);
+        v.y = (float)((double)v.y * inv);
+        v.z = (float)((double)v.z * inv);
+        v.w = (float)((double)v.w * inv);
+        x[i] = v;
+        h[i] = pack_half4(v.x * kNsScale, v.y * kNsScale, v.z * kNsScale, v.w * kNsScale);
     }
 }
 
-template <int KIND, bool A_MN, bool B_MN>
-int launch_product(const CUtensorMap& ta, const CUtensorMap& tb, const NsProduct& p, int batch, cudaStream_t st) {
-    auto kern = k_ns_product<KIND, A_MN, B_MN>;
+template <int KIND, int BN, bool A_MN, bool B_MN>
+int launch_tiled(const CUtensorMap& ta, const CUtensorMap& tb, NsProduct p, cudaStream_t st) {
+    using S = NsTile<BN>;
+    auto kern = k_ns_product<KIND, BN, A_MN, B_MN>;
     static std::atomic<uint64_t> done{0};
-    MG_TRY(smem_limit_once(kern, NsTile::SMEM_BYTES, done));
-    const int tm = (p.M + NsTile::BM - 1) / NsTile::BM, tn = (p.N + NsTile::BN - 1) / NsTile::BN;
-    MG_CUDA_TRY(MG_LAUNCH(kern, dim3(tn, tm, batch), 128, NsTile::SMEM_BYTES, st, ta, tb, p));
+    MG_TRY(smem_limit_once(kern, S::SMEM_BYTES, done));
+    p.tilesM = (p.M + S::BM - 1) / S::BM;
+    p.tilesN = (p.N + BN - 1) / BN;
+    const int64_t units = (int64_t)ns_tiles<KIND, BN>(p.tilesM, p.tilesN) * p.batch;
+    if (units > INT32_MAX) return fail(MG_ERR_ARGUMENT, "newton_schulz: too many tiles");
+    const int grid = (int)std::min<int64_t>(units, num_sms());
+    MG_CUDA_TRY(MG_LAUNCH(kern, grid, S::THREADS, S::SMEM_BYTES, st, ta, tb, p));
     return check_launch("k_ns_product");
+}
+
+// 256-wide tiles where they fill the GPU: half the operand bytes per product
+// of 128-wide ones, which below a wave leave too many SMs idle.
+template <int KIND, bool A_MN, bool B_MN>
+int launch_product(const CUtensorMap& ta, const CUtensorMap& tb, const NsProduct& p, cudaStream_t st) {
+    const int64_t tiles = (int64_t)ns_tiles<KIND, 256>((p.M + 127) / 128, (p.N + 255) / 256) * p.batch;
+    return tiles >= num_sms() ? launch_tiled<KIND, 256, A_MN, B_MN>(ta, tb, p, st)
+                              : launch_tiled<KIND, 128, A_MN, B_MN>(ta, tb, p, st);
 }
 
 struct Workspace {
@@ -155,7 +211,7 @@ Workspace layout(int batch, int rows, int cols, void* base) {
         return q;
     };
     const size_t s = std::min(rows, cols), x = (size_t)batch * rows * round8(cols), g = (size_t)batch * s * round8((int)s);
-    w.partial = static_cast<double*>(take((size_t)batch * kPrepParts * 8));
+    w.partial = static_cast<double*>(take((size_t)batch * kPrepMaxParts * 8));
     w.x32 = static_cast<float*>(take(x * 4));
     w.x16[0] = static_cast<__half*>(take(x * 2));
     w.x16[1] = static_cast<__half*>(take(x * 2));
@@ -189,18 +245,20 @@ int check_workspace(const char* name, int batch, int rows, int cols, int steps, 
 // epilogue writes `fin`.
 int newton_schulz(const Workspace& w, int batch, int rows, int cols, int steps, int parts, const NsFinal& fin, cudaStream_t st) {
     const MuonShape shape{rows, cols, round8(cols)};
-    MG_CUDA_TRY(MG_LAUNCH(k_muon_normalise, dim3(std::min(rows, 512), batch), kPrepThreads, 0, st, shape, w.x32, w.x16[0],
-                          w.partial, parts));
+    const int64_t quads = (int64_t)rows * shape.ldx / 4;
+    const int ctas = (int)std::min<int64_t>((quads + 4 * kPrepThreads - 1) / (4 * kPrepThreads), std::max(1, num_sms() * 8 / batch));
+    MG_CUDA_TRY(MG_LAUNCH(k_muon_normalise, dim3(ctas, batch), kPrepThreads, 0, st, shape, w.x32, w.x16[0], w.partial, parts));
     MG_TRY(check_launch("k_muon_normalise"));
     const bool wide = rows <= cols;  // G = X X^T, else X^T X
     const int s = std::min(rows, cols), l = std::max(rows, cols), lds = round8(s);
     CUtensorMap mx[2], mg16, mb16;
-    for (int i = 0; i < 2; i++) MG_TRY(make_tmap_f16_3d(&mx[i], w.x16[i], cols, rows, batch, shape.ldx, NsTile::BM));
+    for (int i = 0; i < 2; i++) MG_TRY(make_tmap_f16_3d(&mx[i], w.x16[i], cols, rows, batch, shape.ldx, 128));
     CUtensorMap mxk[2];  // boxes of 64 rows, for X as an operand whose K index is the row
     for (int i = 0; i < 2; i++) MG_TRY(make_tmap_f16_3d(&mxk[i], w.x16[i], cols, rows, batch, shape.ldx, 64));
-    MG_TRY(make_tmap_f16_3d(&mg16, w.g16, s, s, batch, lds, NsTile::BM));
-    MG_TRY(make_tmap_f16_3d(&mb16, w.b16, s, s, batch, lds, NsTile::BM));
+    MG_TRY(make_tmap_f16_3d(&mg16, w.g16, s, s, batch, lds, 128));
+    MG_TRY(make_tmap_f16_3d(&mb16, w.b16, s, s, batch, lds, 128));
     NsProduct p{};
+    p.batch = batch;
     p.status = status_ptr();
     for (int i = 0; i < steps; i++) {
         const int cur = i & 1;
@@ -209,14 +267,14 @@ int newton_schulz(const Workspace& w, int batch, int rows, int cols, int steps, 
         p.ldo = lds;
         p.out16 = w.g16;
         p.a = 0.0f;
-        MG_TRY(wide ? (launch_product<kNsGram, false, false>(mx[cur], mx[cur], p, batch, st))
-                    : (launch_product<kNsGram, true, true>(mxk[cur], mxk[cur], p, batch, st)));
+        MG_TRY(wide ? (launch_product<kNsGram, false, false>(mx[cur], mx[cur], p, st))
+                    : (launch_product<kNsGram, true, true>(mxk[cur], mxk[cur], p, st)));
         p.K = s;
         p.out16 = w.b16;
         p.g16 = w.g16;
         p.b = kNsB;
         p.c = kNsC;
-        MG_TRY((launch_product<kNsPoly, false, false>(mg16, mg16, p, batch, st)));
+        MG_TRY((launch_product<kNsPoly, false, false>(mg16, mg16, p, st)));
         p.M = rows;
         p.N = cols;
         p.K = s;
@@ -226,17 +284,22 @@ int newton_schulz(const Workspace& w, int batch, int rows, int cols, int steps, 
         p.a = kNsA;
         p.last = i + 1 == steps;
         if (p.last) p.fin = fin;
-        MG_TRY(wide ? (launch_product<kNsApply, false, true>(mb16, mxk[cur], p, batch, st))
-                    : (launch_product<kNsApply, false, false>(mx[cur], mb16, p, batch, st)));
+        MG_TRY(wide ? (launch_product<kNsApply, false, true>(mb16, mxk[cur], p, st))
+                    : (launch_product<kNsApply, false, false>(mx[cur], mb16, p, st)));
     }
     return MG_OK;
 }
 
 template <class T, bool MUON>
-int prepare(const MuonInput& in, const Workspace& w, int batch, int rows, int cols, int* parts, cudaStream_t st) {
+int prepare(const MuonInput& in, const Workspace& w, int batch, int rows, int cols, bool vec, int* parts, cudaStream_t st) {
     const MuonShape shape{rows, cols, round8(cols)};
-    *parts = std::min(rows, kPrepParts);
-    MG_CUDA_TRY(MG_LAUNCH((k_muon_prepare<T, MUON>), dim3(*parts, batch), kPrepThreads, 0, st, in, shape, w.x32, w.partial));
+    const int64_t pieces = (int64_t)rows * ((cols + (vec ? 3 : 0)) / (vec ? 4 : 1));
+    const int64_t most = std::min<int64_t>(kPrepMaxParts, std::max(1, num_sms() * 8 / batch));
+    *parts = (int)std::min<int64_t>((pieces + 4 * kPrepThreads - 1) / (4 * kPrepThreads), most);
+    if (vec)
+        MG_CUDA_TRY(MG_LAUNCH((k_muon_prepare<T, MUON, 4>), dim3(*parts, batch), kPrepThreads, 0, st, in, shape, w.x32, w.partial));
+    else
+        MG_CUDA_TRY(MG_LAUNCH((k_muon_prepare<T, MUON, 1>), dim3(*parts, batch), kPrepThreads, 0, st, in, shape, w.x32, w.partial));
     return check_launch("k_muon_prepare");
 }
 
@@ -276,17 +339,19 @@ int mg_orthogonalize(const void* x, int dtype, int64_t ld, int64_t batch_stride,
     in.ld = ld;
     in.stride = batch_stride;
     int parts = 0;
+    const bool vec = cols % 4 == 0 && ld % 4 == 0 && batch_stride % 4 == 0 && aligned_to(x, dtype == MG_DTYPE_F32 ? 16 : 8);
     if (dtype == MG_DTYPE_F32)
-        MG_TRY((prepare<float, false>(in, w, batch, rows, cols, &parts, st)));
+        MG_TRY((prepare<float, false>(in, w, batch, rows, cols, vec, &parts, st)));
     else if (dtype == MG_DTYPE_BF16)
-        MG_TRY((prepare<__nv_bfloat16, false>(in, w, batch, rows, cols, &parts, st)));
+        MG_TRY((prepare<__nv_bfloat16, false>(in, w, batch, rows, cols, vec, &parts, st)));
     else
-        MG_TRY((prepare<__half, false>(in, w, batch, rows, cols, &parts, st)));
+        MG_TRY((prepare<__half, false>(in, w, batch, rows, cols, vec, &parts, st)));
     NsFinal fin{};
     fin.out = out;
     fin.outBf16 = out_dtype == MG_DTYPE_BF16;
     fin.ld = ldo;
     fin.stride = out_stride;
+    fin.vec = ldo % 4 == 0 && out_stride % 4 == 0 && aligned_to(out, 8);
     return newton_schulz(w, batch, rows, cols, steps, parts, fin, st);
 }
 
@@ -318,12 +383,14 @@ int mg_muon_step(float* master, const float* grad, float* momentum, void* weight
     in.nesterov = nesterov;
     in.normSqOut = norm_sq_out;
     int parts = 0;
-    MG_TRY((prepare<float, true>(in, w, batch, rows, cols, &parts, st)));
+    const bool vec = cols % 4 == 0 && batch_stride % 4 == 0 && aligned_to(grad, 16) && aligned_to(momentum, 16);
+    MG_TRY((prepare<float, true>(in, w, batch, rows, cols, vec, &parts, st)));
     NsFinal fin{};
     fin.master = master;
     fin.weights = static_cast<__nv_bfloat16*>(weights);
     fin.ld = cols;
     fin.stride = batch_stride;
+    fin.vec = cols % 4 == 0 && batch_stride % 4 == 0 && aligned_to(master, 16) && aligned_to(weights, 8);
     fin.keep = 1.0f - lr * weight_decay;
     fin.rate = lr * scale;
     return newton_schulz(w, batch, rows, cols, steps, parts, fin, st);

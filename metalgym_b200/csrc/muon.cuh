@@ -1,11 +1,21 @@
 // The tcgen05 products of a Newton-Schulz step (muon.cu): fp16 operands, fp32
-// accumulation in tensor memory, one CTA per 128 x 128 output tile.
+// accumulation in tensor memory, persistent CTAs that walk 128 x BN output
+// tiles with the accumulator double-buffered in tensor memory, so that the
+// epilogue of one tile runs beside the products of the next.
 //
-//   kNsGram   G = X X^T or X^T X, symmetric: the tiles on and above the
-//             diagonal are computed, each written to both places
+//   kNsGram   G = X X^T or X^T X, symmetric: only tiles that reach the diagonal
+//             or lie above it are computed, and written to both places
 //   kNsPoly   B = b G + c G G, likewise symmetric
 //   kNsApply  X <- a X + B X or a X + X B, or in the last step what the caller
 //             wants of it
+//
+// Warp roles (320 threads): 0 TMA producer, 1 MMA issuer, 2-9 epilogue (warp w:
+// accumulator lanes 32 (w % 4) .., one half of the columns).
+// The epilogue takes 32 x 32 pieces from tensor memory through a swizzled
+// 4 KB slab of shared memory: a thread of tcgen05.ld has a row, and rows are
+// far apart in memory; out of the slab, eight lanes hold 32 consecutive columns
+// of a row, so that X (fp32 and fp16) and G move in whole 128- and 64-byte
+// lines. With a row a thread, the same epilogue took 30 us a launch at 128 x 512.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -27,25 +37,31 @@ struct NsFinal {
     float* master;
     __nv_bfloat16* weights;
     int64_t ld, stride;
+    int vec;           // every group of four columns of a row is 16-byte (fp32) and 8-byte (16-bit) aligned
     float keep, rate;  // master = master * keep - rate * X
 };
 
 struct NsProduct {
-    int M, N, K;
-    int ldo;              // row stride of out16, g16 and x32
-    __half* out16;        // [batch][M][ldo], scaled
-    const __half* g16;    // kNsPoly
-    float* x32;           // kNsApply
+    int M, N, K, batch;
+    int tilesM, tilesN;
+    int ldo;            // row stride of out16, g16 and x32 (a multiple of 8)
+    __half* out16;      // [batch][M][ldo], scaled
+    const __half* g16;  // kNsPoly
+    float* x32;         // kNsApply
     float a, b, c;
     int last;
     NsFinal fin;
     int* status;
 };
 
+template <int BN>
 struct NsTile {
-    static constexpr int BM = 128, BN = 128, BK = 64, STAGES = 4;
+    static constexpr int BM = 128, BK = 64, STAGES = BN == 256 ? 4 : 6;
     static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/;
+    static constexpr int EW = 8, THREADS = 64 + 32 * EW, SLAB = 4096;
+    static constexpr int SLAB_OFF = STAGES * STAGE_BYTES, BAR_OFF = SLAB_OFF + EW * SLAB;
+    static constexpr int TMEM_COLS = 2 * BN;
+    static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024 /*align*/;
 };
 
 // Instruction descriptor, kind::f16: fp16 A and B, fp32 accumulator, M = 128.
@@ -60,64 +76,205 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
         : "memory");
 }
 
-// 32 columns of one output row.
-template <int KIND>
-__device__ __forceinline__ void ns_epilogue(const NsProduct& p, int b, int row, int col, bool mirror, const float* v) {
-    const int n = min(32, p.N - col);
-    const int64_t base = (int64_t)b * p.M * p.ldo;
+// Tiles of one matrix, and the u-th of them; of a symmetric product only those
+// that do not lie wholly below the diagonal.
+template <int KIND, int BN>
+__host__ __device__ __forceinline__ int ns_tiles(int tilesM, int tilesN) {
+    if (KIND == kNsApply) return tilesM * tilesN;
+    int n = 0;
+    for (int i = 0; i < tilesM; i++) n += tilesN - i * 128 / BN;
+    return n;
+}
+template <int KIND, int BN>
+__device__ __forceinline__ void ns_tile_at(int u, int tilesN, int& i, int& j) {
     if (KIND == kNsApply) {
-        float* x = p.x32 + base + (int64_t)row * p.ldo + col;
-        __half* h = p.out16 + base + (int64_t)row * p.ldo + col;
-        const int64_t at = (int64_t)b * p.fin.stride + (int64_t)row * p.fin.ld + col;
-#pragma unroll
-        for (int i = 0; i < 32; i++) {
-            if (i >= n) break;
-            const float y = fmaf(p.a, x[i], v[i] * (kNsUnscale * kNsUnscale));
-            if (!p.last) {
-                x[i] = y;
-                h[i] = __float2half_rn(y * kNsScale);
-            } else if (p.fin.master) {
-                const float w = __fsub_rn(__fmul_rn(p.fin.master[at + i], p.fin.keep), __fmul_rn(p.fin.rate, y));
-                p.fin.master[at + i] = w;
-                p.fin.weights[at + i] = __float2bfloat16_rn(w);
-            } else if (p.fin.outBf16) {
-                static_cast<__nv_bfloat16*>(p.fin.out)[at + i] = __float2bfloat16_rn(y);
-            } else {
-                static_cast<__half*>(p.fin.out)[at + i] = __float2half_rn(y);
-            }
-        }
+        i = u / tilesN;
+        j = u % tilesN;
         return;
     }
+    i = 0;
+    while (u >= tilesN - i * 128 / BN) {
+        u -= tilesN - i * 128 / BN;
+        i++;
+    }
+    j = i * 128 / BN + u;
+}
+
+__device__ __forceinline__ uint32_t ns_slab_offset(int r, int k) { return (uint32_t)(r * 128 + ((k ^ (r & 7)) << 4)); }
+
+__device__ __forceinline__ uint2 pack_half4(float a, float b, float c, float d) {
+    const __half2 x = __floats2half2_rn(a, b), y = __floats2half2_rn(c, d);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
+}
+
+// Four columns (from col on) of output row `row`; v: the accumulator.
+template <int KIND>
+__device__ __forceinline__ void ns_store4(const NsProduct& p, int64_t at, int64_t finAt, int col, const float4& v,
+                                          const float4& x, const uint2& g, bool finVec) {
+    float y[4] = {v.x, v.y, v.z, v.w};
+    if constexpr (KIND == kNsApply) {
+        const float xv[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int i = 0; i < 32; i++) {
-        if (i >= n) break;
-        float y = v[i] * kNsUnscale;  // scaled by 2^10, as the operands are
-        if (KIND == kNsPoly) y = fmaf(p.c, y, p.b * __half2float(p.g16[base + (int64_t)row * p.ldo + col + i]));
-        const __half h = __float2half_rn(y);
-        p.out16[base + (int64_t)row * p.ldo + col + i] = h;
-        if (mirror) p.out16[base + (int64_t)(col + i) * p.ldo + row] = h;
+        for (int i = 0; i < 4; i++) y[i] = fmaf(p.a, xv[i], y[i] * (kNsUnscale * kNsUnscale));
+        if (!p.last) {
+            *reinterpret_cast<float4*>(p.x32 + at) = make_float4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<uint2*>(p.out16 + at) =
+                pack_half4(y[0] * kNsScale, y[1] * kNsScale, y[2] * kNsScale, y[3] * kNsScale);
+            return;
+        }
+        const int n = min(4, p.N - col);
+        if (p.fin.master) {
+            float* m = p.fin.master + finAt;
+            if (finVec && n == 4) {
+                const float4 o = *reinterpret_cast<const float4*>(m);
+                const float ov[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) y[i] = __fsub_rn(__fmul_rn(ov[i], p.fin.keep), __fmul_rn(p.fin.rate, y[i]));
+                *reinterpret_cast<float4*>(m) = make_float4(y[0], y[1], y[2], y[3]);
+                const __nv_bfloat162 a = __floats2bfloat162_rn(y[0], y[1]), b = __floats2bfloat162_rn(y[2], y[3]);
+                *reinterpret_cast<uint2*>(p.fin.weights + finAt) =
+                    make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (i < n) {
+                        const float w = __fsub_rn(__fmul_rn(m[i], p.fin.keep), __fmul_rn(p.fin.rate, y[i]));
+                        m[i] = w;
+                        p.fin.weights[finAt + i] = __float2bfloat16_rn(w);
+                    }
+            }
+            return;
+        }
+        if (p.fin.outBf16) {
+            __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.fin.out) + finAt;
+            if (finVec && n == 4) {
+                const __nv_bfloat162 a = __floats2bfloat162_rn(y[0], y[1]), b = __floats2bfloat162_rn(y[2], y[3]);
+                *reinterpret_cast<uint2*>(o) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (i < n) o[i] = __float2bfloat16_rn(y[i]);
+            }
+        } else {
+            __half* o = static_cast<__half*>(p.fin.out) + finAt;
+            if (finVec && n == 4) {
+                *reinterpret_cast<uint2*>(o) = pack_half4(y[0], y[1], y[2], y[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (i < n) o[i] = __float2half_rn(y[i]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) y[i] *= kNsUnscale;  // scaled by 2^10, as the operands are
+        if (KIND == kNsPoly) {
+            const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&g.x));
+            const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&g.y));
+            y[0] = fmaf(p.c, y[0], p.b * g0.x);
+            y[1] = fmaf(p.c, y[1], p.b * g0.y);
+            y[2] = fmaf(p.c, y[2], p.b * g1.x);
+            y[3] = fmaf(p.c, y[3], p.b * g1.y);
+        }
+        *reinterpret_cast<uint2*>(p.out16 + at) = pack_half4(y[0], y[1], y[2], y[3]);
     }
 }
 
-template <int KIND, bool A_MN, bool B_MN>
-__global__ void __launch_bounds__(128, 1)
+// A 32 x 32 piece at (row0, col0) of matrix b's output: lane r holds row r in v.
+// Of a symmetric product, pieces below the diagonal are left to their mirror
+// pieces above it, which write both: every entry is written once.
+template <int KIND>
+__device__ __forceinline__ void ns_piece(const NsProduct& p, int b, int row0, int col0, uint8_t* slab, const float* v) {
+    const int lane = threadIdx.x & 31;
+    if (KIND != kNsApply && col0 < row0) return;
+    __syncwarp();  // the slab's last readers are done
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+        *reinterpret_cast<float4*>(slab + ns_slab_offset(lane, k)) = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+    __syncwarp();
+    const int64_t base = (int64_t)b * p.M * p.ldo;
+    const int k = lane & 7, col = col0 + 4 * k;
+    const bool in = col < p.N;  // then the four columns lie inside ldo
+    const bool finVec = KIND == kNsApply && p.last && p.fin.vec;
+    if (in) {
+        // the loads of four rows go out before the first is used
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float4 x[4];
+            uint2 g[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int row = row0 + (4 * h + i) * 4 + (lane >> 3);
+                x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                g[i] = make_uint2(0u, 0u);
+                if (row < p.M) {
+                    if (KIND == kNsApply) x[i] = ld_f4_now(p.x32 + base + (int64_t)row * p.ldo + col);
+                    if (KIND == kNsPoly) g[i] = *reinterpret_cast<const uint2*>(p.g16 + base + (int64_t)row * p.ldo + col);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = (4 * h + i) * 4 + (lane >> 3), row = row0 + r;
+                if (row < p.M)
+                    ns_store4<KIND>(p, base + (int64_t)row * p.ldo + col, (int64_t)b * p.fin.stride + (int64_t)row * p.fin.ld + col,
+                                    col, *reinterpret_cast<const float4*>(slab + ns_slab_offset(r, k)), x[i], g[i], finVec);
+            }
+        }
+    }
+    if (KIND == kNsApply || col0 == row0) return;
+    // the mirrored piece, row col0 + lane: column row0 + r is this piece's (r, lane)
+    const int mrow = col0 + lane;
+    if (mrow < p.M) {
+        const int64_t at = base + (int64_t)mrow * p.ldo + row0;
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            if (row0 + 8 * q >= p.ldo) break;
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int r = 8 * q + i;
+                y[i] = *reinterpret_cast<const float*>(slab + ns_slab_offset(r, lane >> 2) + (lane & 3) * 4) * kNsUnscale;
+            }
+            if (KIND == kNsPoly) {  // G is symmetric: the same values as the direct piece's
+                const uint4 gw = *reinterpret_cast<const uint4*>(p.g16 + at + 8 * q);
+                const uint32_t w[4] = {gw.x, gw.y, gw.z, gw.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                    y[2 * i] = fmaf(p.c, y[2 * i], p.b * f.x);
+                    y[2 * i + 1] = fmaf(p.c, y[2 * i + 1], p.b * f.y);
+                }
+            }
+            const uint2 lo = pack_half4(y[0], y[1], y[2], y[3]), hi = pack_half4(y[4], y[5], y[6], y[7]);
+            *reinterpret_cast<uint4*>(p.out16 + at + 8 * q) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+    }
+}
+
+template <int KIND, int BN, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(NsTile<BN>::THREADS, 1)
     k_ns_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const NsProduct p) {
-    using S = NsTile;
-    mg_pdl_trigger();
-    if (KIND != kNsApply && blockIdx.x < blockIdx.y) return;  // the mirror of a tile above the diagonal
+    using S = NsTile<BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::STAGES * S::STAGE_BYTES);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::BAR_OFF);
     uint64_t* empty = full + S::STAGES;
-    uint64_t* done = empty + S::STAGES;
+    uint64_t* tfull = empty + S::STAGES;  // [2]
+    uint64_t* tempty = tfull + 2;         // [2]
+    uint64_t* done = tempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    mg_pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int m0 = blockIdx.y * S::BM, n0 = blockIdx.x * S::BN, b = blockIdx.z;
+    const int perMatrix = ns_tiles<KIND, BN>(p.tilesM, p.tilesN), units = perMatrix * p.batch;
     const int nk = (p.K + S::BK - 1) / S::BK;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; s++) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; a++) {
+            mbar_init(&tfull[a], 1);
+            mbar_init(&tempty[a], S::EW);
         }
         mbar_init(done, 1);
         fence_barrier_init();
@@ -125,7 +282,7 @@ __global__ void __launch_bounds__(128, 1)
         prefetch_tensormap(&tmB);
     }
     if (warp == 2) {
-        tmem_alloc(tmem_slot, S::BN);
+        tmem_alloc(tmem_slot, S::TMEM_COLS);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -134,69 +291,107 @@ __global__ void __launch_bounds__(128, 1)
     const uint32_t tmem = *tmem_slot;
     mg_pdl_wait();
 
-    if (warp == 0 && lane == 0) {
-        int issued = 0;
-        for (int kb = 0; kb < nk; kb++) {
-            const int s = kb % S::STAGES;
-            if (!mbar_wait(&empty[s], ((kb / S::STAGES) & 1) ^ 1, p.status, kDevTimeoutEmpty)) break;
-            issued = kb + 1;
-            uint8_t* sA = smem + s * S::STAGE_BYTES;
-            uint8_t* sB = sA + S::A_BYTES;
-            const int k0 = kb * S::BK;
-            mbar_arrive_expect_tx(&full[s], S::STAGE_BYTES);
-            if (A_MN) {
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
+                const int b = u / perMatrix;
+                int ti, tj;
+                ns_tile_at<KIND, BN>(u - b * perMatrix, p.tilesN, ti, tj);
+                const int m0 = ti * S::BM, n0 = tj * BN;
+                for (int kb = 0; kb < nk; kb++, it++) {
+                    const int s = it % S::STAGES;
+                    if (!mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1, p.status, kDevTimeoutEmpty)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t* sA = smem + s * S::STAGE_BYTES;
+                    uint8_t* sB = sA + S::A_BYTES;
+                    const int k0 = kb * S::BK;
+                    mbar_arrive_expect_tx(&full[s], S::STAGE_BYTES);
+                    if (A_MN) {
 #pragma unroll
-                for (int j = 0; j < S::BM / 64; j++) tma_load_3d(sA + j * 8192, &tmA, m0 + 64 * j, k0, b, &full[s]);
-            } else {
-                tma_load_3d(sA, &tmA, k0, m0, b, &full[s]);
-            }
-            if (B_MN) {
+                        for (int j = 0; j < S::BM / 64; j++) tma_load_3d(sA + j * 8192, &tmA, m0 + 64 * j, k0, b, &full[s]);
+                    } else {
+                        tma_load_3d(sA, &tmA, k0, m0, b, &full[s]);
+                    }
+                    if (B_MN) {
 #pragma unroll
-                for (int j = 0; j < S::BN / 64; j++) tma_load_3d(sB + j * 8192, &tmB, n0 + 64 * j, k0, b, &full[s]);
-            } else {
-                tma_load_3d(sB, &tmB, k0, n0, b, &full[s]);
+                        for (int j = 0; j < BN / 64; j++) tma_load_3d(sB + j * 8192, &tmB, n0 + 64 * j, k0, b, &full[s]);
+                    } else {  // boxes of 128 rows
+#pragma unroll
+                        for (int j = 0; j < BN / 128; j++) tma_load_3d(sB + j * 16384, &tmB, k0, n0 + 128 * j, b, &full[s]);
+                    }
+                }
             }
+            // every issued copy has landed before this CTA can exit
+            for (int k = it - S::STAGES < 0 ? 0 : it - S::STAGES; k < it; k++)
+                mbar_wait(&full[k % S::STAGES], (k / S::STAGES) & 1, p.status, kDevTimeoutFull);
         }
-        // every issued copy has landed before this CTA can exit
-        for (int kb = issued - S::STAGES < 0 ? 0 : issued - S::STAGES; kb < issued; kb++)
-            mbar_wait(&full[kb % S::STAGES], (kb / S::STAGES) & 1, p.status, kDevTimeoutFull);
-    } else if (warp == 1 && lane == 0) {
-        constexpr uint32_t idesc = idesc_f16_f32(S::BN, A_MN, B_MN);
-        for (int kb = 0; kb < nk; kb++) {
-            const int s = kb % S::STAGES;
-            if (!mbar_wait(&full[s], (kb / S::STAGES) & 1, p.status, kDevTimeoutFull)) break;
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_f16_f32(BN, A_MN, B_MN);
+            int it = 0, t = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < units && ok; u += gridDim.x, t++) {
+                const int a = t & 1;
+                if (!mbar_wait(&tempty[a], ((t >> 1) & 1) ^ 1, p.status, kDevTimeoutEmpty)) break;
+                tc_fence_after();
+                const uint32_t acc = tmem + (uint32_t)(a * BN);
+                for (int kb = 0; kb < nk; kb++, it++) {
+                    const int s = it % S::STAGES;
+                    if (!mbar_wait(&full[s], (it / S::STAGES) & 1, p.status, kDevTimeoutFull)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t aBase = smem_u32(smem + s * S::STAGE_BYTES), bBase = aBase + S::A_BYTES;
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++) {
+                        const uint64_t ad = A_MN ? smem_desc_sw128(aBase + kk * 2048, 8192, 1024)
+                                                 : smem_desc_sw128(aBase + kk * 32, 16, 1024);
+                        const uint64_t bd = B_MN ? smem_desc_sw128(bBase + kk * 2048, 8192, 1024)
+                                                 : smem_desc_sw128(bBase + kk * 32, 16, 1024);
+                        tc_mma_bf16(acc, ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);  // kind::f16: the types are idesc's
+                    }
+                    tc_commit(&empty[s]);
+                }
+                if (ok) tc_commit(&tfull[a]);
+            }
+            tc_commit(done);  // covers every MMA issued, also after a timeout
+        }
+    } else {
+        const int q = warp & 3, e = warp - 2, half = (e / 4) * (BN / 2);
+        uint8_t* slab = smem + S::SLAB_OFF + e * S::SLAB;
+        int t = 0;
+        for (int u = blockIdx.x; u < units; u += gridDim.x, t++) {
+            const int b = u / perMatrix, a = t & 1;
+            int ti, tj;
+            ns_tile_at<KIND, BN>(u - b * perMatrix, p.tilesN, ti, tj);
+            const int row0 = ti * S::BM + 32 * q, n0 = tj * BN + half;
+            if (!mbar_wait_warp(&tfull[a], (t >> 1) & 1, p.status, kDevTimeoutDone)) break;
             tc_fence_after();
-            const uint32_t aBase = smem_u32(smem + s * S::STAGE_BYTES), bBase = aBase + S::A_BYTES;
-#pragma unroll
-            for (int kk = 0; kk < 4; kk++) {
-                const uint64_t ad = A_MN ? smem_desc_sw128(aBase + kk * 2048, 8192, 1024)
-                                         : smem_desc_sw128(aBase + kk * 32, 16, 1024);
-                const uint64_t bd = B_MN ? smem_desc_sw128(bBase + kk * 2048, 8192, 1024)
-                                         : smem_desc_sw128(bBase + kk * 32, 16, 1024);
-                tc_mma_bf16(tmem, ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);  // kind::f16: the types are idesc's
-            }
-            tc_commit(&empty[s]);
-        }
-        tc_commit(done);  // covers every MMA issued, also after a timeout
-    }
-    __syncwarp();
-    const bool ready = mbar_wait_warp(done, 0, p.status, kDevTimeoutDone);
-    tc_fence_after();
-    const int row = m0 + warp * 32 + lane;
-    if (ready) {
+            const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN + half);
 #pragma unroll 1
-        for (int c = 0; c < S::BN / 32; c++) {
-            float v[32];
-            tmem_ld32(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(c * 32), v);
-            const int col = n0 + c * 32;
-            if (row < p.M && col < p.N) ns_epilogue<KIND>(p, b, row, col, blockIdx.x > blockIdx.y, v);
+            for (int c = 0; c < BN / 64; c++) {
+                float v[32];
+                tmem_ld32(acc + (uint32_t)(c * 32), v);
+                if (c == BN / 64 - 1) {  // the accumulator is free for the tile after next
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&tempty[a]);
+                }
+                if (row0 < p.M && n0 + 32 * c < p.N) ns_piece<KIND>(p, b, row0, n0 + 32 * c, slab, v);
+            }
         }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 2) {
+        mbar_wait(done, 0, p.status, kDevTimeoutDone);
         tc_fence_after();
-        tmem_dealloc(tmem, S::BN);
+        tmem_dealloc(tmem, S::TMEM_COLS);
     }
 }
 
