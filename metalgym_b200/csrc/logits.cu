@@ -305,14 +305,6 @@ __device__ __forceinline__ float warp_add(float x) {
     return x;
 }
 
-// The `rank`-th CTA's copy of a shared variable (distributed shared memory).
-template <class V>
-__device__ __forceinline__ const V* cluster_peer(const V* local, int rank) {
-    uint64_t remote;
-    asm("mapa.u64 %0, %1, %2;" : "=l"(remote) : "l"(reinterpret_cast<uint64_t>(local)), "r"(rank));
-    return reinterpret_cast<const V*>(remote);
-}
-
 // The row's statistics (and best runner) in every thread of its CTAs, merged in
 // one fixed order: lanes, warps, CTAs. With several parts the caller ends with
 // cluster_sync, so that no CTA leaves while another reads its part.

@@ -19,28 +19,12 @@
 
 #include "logits.cuh"
 #include "muon.cuh"
+#include "muon_small.cuh"
 #include "runtime.h"
 #include "metalgym/pdl.cuh"
 
 namespace mg {
 namespace {
-
-constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
-
-// ------------------------------------------------------------------ U and its norm
-
-// What turns the inputs into U: a copy (orthogonalise) or the momentum.
-struct MuonInput {
-    const void* x;  // orthogonalise: [batch][rows][ld]
-    int64_t ld, stride;
-    const float* grad;  // muon: dense rows
-    float* momentum;
-    const float* normPartial;
-    int nNorm;
-    float maxGradNorm, decay;
-    int nesterov;
-    float* normSqOut;
-};
 
 struct MuonShape {
     int rows, cols, ldx;  // ldx: row stride of X in the workspace
@@ -62,16 +46,12 @@ __global__ void __launch_bounds__(kPrepThreads)
     __shared__ double sSum[kPrepWarps];
     const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (MUON) {
-        if (warp == 0) {  // the clip factor, as the Adam step forms it
-            float sum = 0.0f;
-            for (int i = lane; i < in.nNorm; i += 32) sum = __fadd_rn(sum, in.normPartial[i]);
-            sum = warp_sum(sum);
+        if (warp == 0) {
+            float normSq;
+            const float f = muon_clip(in, &normSq);
             if (lane == 0) {
-                const float norm = __fsqrt_rn(sum);
-                sScale = (in.maxGradNorm > 0.0f && norm > in.maxGradNorm)
-                             ? __fdiv_rn(in.maxGradNorm, __fadd_rn(norm, 1e-6f))
-                             : 1.0f;
-                if (blockIdx.x == 0 && b == 0 && in.normSqOut) *in.normSqOut = sum;
+                sScale = f;
+                if (blockIdx.x == 0 && b == 0 && in.normSqOut) *in.normSqOut = normSq;
             }
         }
         __syncthreads();
@@ -303,6 +283,54 @@ int prepare(const MuonInput& in, const Workspace& w, int batch, int rows, int co
     return check_launch("k_muon_prepare");
 }
 
+// One kernel for a smaller side of at most 128 and a few steps (muon_small.cuh).
+bool small_enough(int rows, int cols, int steps) {
+    return std::min(rows, cols) <= kMuonSmallSide && steps <= kMuonSmallSteps;
+}
+
+template <int SP, bool WIDE, class T, bool MUON>
+int launch_small(const MuonInput& in, const NsProduct& p, int steps, bool vec, cudaStream_t st) {
+    auto kern = k_muon_small<SP, WIDE, T, MUON>;
+    static std::atomic<uint64_t> done{0};
+    MG_TRY(smem_limit_once(kern, MuonSmall::SMEM_BYTES, done));
+    // a CTA for each 128 of the long side, up to a cluster, while the matrices leave SMs for them
+    const int pieces = (std::max(p.M, p.N) + 127) / 128;
+    int parts = 1;
+    while (parts < kMuonSmallCluster && parts < pieces && (int64_t)p.batch * parts * 2 <= num_sms()) parts *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.batch * parts));
+    cfg.blockDim = dim3(kMuonSmallThreads);
+    cfg.dynamicSmemBytes = MuonSmall::SMEM_BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = parts;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = parts > 1 ? 2 : 1;
+    MG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, in, p, steps, vec ? 1 : 0, parts));
+    return check_launch("k_muon_small");
+}
+
+template <class T, bool MUON>
+int run_small(const MuonInput& in, const NsFinal& fin, int batch, int rows, int cols, int steps, bool vec, cudaStream_t st) {
+    NsProduct p{};
+    p.M = rows;
+    p.N = cols;
+    p.batch = batch;
+    p.ldo = round8(cols);
+    p.last = 1;
+    p.fin = fin;
+    p.status = status_ptr();
+    const bool narrow = std::min(rows, cols) <= 64;
+    if (rows <= cols)
+        return narrow ? launch_small<64, true, T, MUON>(in, p, steps, vec, st) : launch_small<128, true, T, MUON>(in, p, steps, vec, st);
+    return narrow ? launch_small<64, false, T, MUON>(in, p, steps, vec, st) : launch_small<128, false, T, MUON>(in, p, steps, vec, st);
+}
+
 bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % (unsigned)bytes) == 0; }
 
 }  // namespace
@@ -338,6 +366,19 @@ int mg_orthogonalize(const void* x, int dtype, int64_t ld, int64_t batch_stride,
     in.x = x;
     in.ld = ld;
     in.stride = batch_stride;
+    NsFinal fin{};
+    fin.out = out;
+    fin.outBf16 = out_dtype == MG_DTYPE_BF16;
+    fin.ld = ldo;
+    fin.stride = out_stride;
+    fin.vec = ldo % 4 == 0 && out_stride % 4 == 0 && aligned_to(out, 8);
+    if (small_enough(rows, cols, steps)) {
+        const int per = dtype == MG_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
+        const bool vec = ld % per == 0 && batch_stride % per == 0 && aligned_to(x, 16);
+        if (dtype == MG_DTYPE_F32) return run_small<float, false>(in, fin, batch, rows, cols, steps, vec, st);
+        if (dtype == MG_DTYPE_BF16) return run_small<__nv_bfloat16, false>(in, fin, batch, rows, cols, steps, vec, st);
+        return run_small<__half, false>(in, fin, batch, rows, cols, steps, vec, st);
+    }
     int parts = 0;
     const bool vec = cols % 4 == 0 && ld % 4 == 0 && batch_stride % 4 == 0 && aligned_to(x, dtype == MG_DTYPE_F32 ? 16 : 8);
     if (dtype == MG_DTYPE_F32)
@@ -346,12 +387,6 @@ int mg_orthogonalize(const void* x, int dtype, int64_t ld, int64_t batch_stride,
         MG_TRY((prepare<__nv_bfloat16, false>(in, w, batch, rows, cols, vec, &parts, st)));
     else
         MG_TRY((prepare<__half, false>(in, w, batch, rows, cols, vec, &parts, st)));
-    NsFinal fin{};
-    fin.out = out;
-    fin.outBf16 = out_dtype == MG_DTYPE_BF16;
-    fin.ld = ldo;
-    fin.stride = out_stride;
-    fin.vec = ldo % 4 == 0 && out_stride % 4 == 0 && aligned_to(out, 8);
     return newton_schulz(w, batch, rows, cols, steps, parts, fin, st);
 }
 
@@ -382,9 +417,7 @@ int mg_muon_step(float* master, const float* grad, float* momentum, void* weight
     in.decay = momentum_decay;
     in.nesterov = nesterov;
     in.normSqOut = norm_sq_out;
-    int parts = 0;
     const bool vec = cols % 4 == 0 && batch_stride % 4 == 0 && aligned_to(grad, 16) && aligned_to(momentum, 16);
-    MG_TRY((prepare<float, true>(in, w, batch, rows, cols, vec, &parts, st)));
     NsFinal fin{};
     fin.master = master;
     fin.weights = static_cast<__nv_bfloat16*>(weights);
@@ -393,6 +426,9 @@ int mg_muon_step(float* master, const float* grad, float* momentum, void* weight
     fin.vec = cols % 4 == 0 && batch_stride % 4 == 0 && aligned_to(master, 16) && aligned_to(weights, 8);
     fin.keep = 1.0f - lr * weight_decay;
     fin.rate = lr * scale;
+    if (small_enough(rows, cols, steps)) return run_small<float, true>(in, fin, batch, rows, cols, steps, vec, st);
+    int parts = 0;
+    MG_TRY((prepare<float, true>(in, w, batch, rows, cols, vec, &parts, st)));
     return newton_schulz(w, batch, rows, cols, steps, parts, fin, st);
 }
 

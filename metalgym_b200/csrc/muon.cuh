@@ -107,10 +107,11 @@ __device__ __forceinline__ uint2 pack_half4(float a, float b, float c, float d) 
     return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
 
-// Four columns (from col on) of output row `row`; v: the accumulator.
+// Four columns (from col on) of an output row; v: the accumulator, x, g and
+// master: what the epilogue reads there (x 0 where X is not kept).
 template <int KIND>
 __device__ __forceinline__ void ns_store4(const NsProduct& p, int64_t at, int64_t finAt, int col, const float4& v,
-                                          const float4& x, const uint2& g, bool finVec) {
+                                          const float4& x, const uint2& g, const float4& master, bool finVec) {
     float y[4] = {v.x, v.y, v.z, v.w};
     if constexpr (KIND == kNsApply) {
         const float xv[4] = {x.x, x.y, x.z, x.w};
@@ -126,8 +127,7 @@ __device__ __forceinline__ void ns_store4(const NsProduct& p, int64_t at, int64_
         if (p.fin.master) {
             float* m = p.fin.master + finAt;
             if (finVec && n == 4) {
-                const float4 o = *reinterpret_cast<const float4*>(m);
-                const float ov[4] = {o.x, o.y, o.z, o.w};
+                const float ov[4] = {master.x, master.y, master.z, master.w};
 #pragma unroll
                 for (int i = 0; i < 4; i++) y[i] = __fsub_rn(__fmul_rn(ov[i], p.fin.keep), __fmul_rn(p.fin.rate, y[i]));
                 *reinterpret_cast<float4*>(m) = make_float4(y[0], y[1], y[2], y[3]);
@@ -200,15 +200,18 @@ __device__ __forceinline__ void ns_piece(const NsProduct& p, int b, int row0, in
         // the loads of four rows go out before the first is used
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            float4 x[4];
+            float4 x[4], m[4];
             uint2 g[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int row = row0 + (4 * h + i) * 4 + (lane >> 3);
                 x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                m[i] = x[i];
                 g[i] = make_uint2(0u, 0u);
                 if (row < p.M) {
-                    if (KIND == kNsApply) x[i] = ld_f4_now(p.x32 + base + (int64_t)row * p.ldo + col);
+                    if (KIND == kNsApply && finVec && p.fin.master && col + 4 <= p.N)
+                        m[i] = ld_f4_now(p.fin.master + (int64_t)b * p.fin.stride + (int64_t)row * p.fin.ld + col);
+                    if (KIND == kNsApply && p.x32) x[i] = ld_f4_now(p.x32 + base + (int64_t)row * p.ldo + col);
                     if (KIND == kNsPoly) g[i] = *reinterpret_cast<const uint2*>(p.g16 + base + (int64_t)row * p.ldo + col);
                 }
             }
@@ -217,7 +220,7 @@ __device__ __forceinline__ void ns_piece(const NsProduct& p, int b, int row0, in
                 const int r = (4 * h + i) * 4 + (lane >> 3), row = row0 + r;
                 if (row < p.M)
                     ns_store4<KIND>(p, base + (int64_t)row * p.ldo + col, (int64_t)b * p.fin.stride + (int64_t)row * p.fin.ld + col,
-                                    col, *reinterpret_cast<const float4*>(slab + ns_slab_offset(r, k)), x[i], g[i], finVec);
+                                    col, *reinterpret_cast<const float4*>(slab + ns_slab_offset(r, k)), x[i], g[i], m[i], finVec);
             }
         }
     }

@@ -138,6 +138,46 @@ def test_orthogonalize(mg, batch, m, n, spectrum):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch,m,n,steps", [(2, 128, 512, 7), (1, 40, 200, 8), (3, 100, 30, 7), (1, 1, 9, 7), (1, 128, 128, 10), (2, 24, 24, 16)])
+def test_many_steps_of_small_matrices(mg, batch, m, n, steps):
+    """More steps than the one-kernel form takes: the tiled products at small sizes."""
+    gen = torch.Generator(device="cuda").manual_seed(m * n + steps)
+    x = torch.randn(batch, m, n, generator=gen, device="cuda")
+    space = workspace(mg, batch, m, n)
+    out = torch.empty(batch, m, n, dtype=torch.float16, device="cuda")
+    ok(mg, mg.mg_orthogonalize(x.data_ptr(), 0, n, m * n, out.data_ptr(), 2, n, m * n, batch, m, n, steps, space.data_ptr(), space.numel(), None))
+    assert status(mg) == 0
+    for i in range(batch):
+        want = newton_schulz(x[i], steps, False)
+        assert (out[i].double() - want).norm() <= allowance(x[i], want, steps) + 2.0 ** -12 * want.norm()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spectrum", ["normal", "low rank", "decaying"])
+@pytest.mark.parametrize("batch,m,n", [(1, 128, 5000), (1, 3001, 20), (2, 64, 1024), (1, 1000, 65), (100, 16, 24), (160, 130, 17), (2, 100, 129), (1, 128, 128)])
+def test_small_side_is_as_exact_as_fp32(mg, batch, m, n, spectrum):
+    """A smaller side of at most 128 takes products of 22-bit operands: at most 16 of them in a row, each off by the
+    operands' 2^-22 and by the cuts of the tensor cores' fp32 accumulator, 2^-23 in each of the 8 instructions of the
+    leading parts, 16 * (2^-22 + 8 * 2^-23) = 1.9e-5 of the products' norms. The products are the powers of G, at most
+    2, and P, whose norm is the largest ratio of a singular value of the result to that of X: the result is off by at
+    most 1.9e-5 times that growth. The master weights show the update without a 16-bit rounding."""
+    gen = torch.Generator(device="cuda").manual_seed(batch + m + n)
+    grad = torch.stack([matrix(gen, m, n, spectrum) for _ in range(batch)])
+    master, momentum = torch.zeros_like(grad), torch.zeros_like(grad)
+    weights = torch.zeros(batch, m, n, dtype=torch.bfloat16, device="cuda")
+    space = workspace(mg, batch, m, n)
+    ok(mg, mg.mg_muon_step(master.data_ptr(), grad.data_ptr(), momentum.data_ptr(), weights.data_ptr(), m * n, batch, m, n, None, 0, 0.0, -1.0,
+                           1.0, 0.0, 0, 0.0, 5, None, space.data_ptr(), space.numel(), None))
+    assert status(mg) == 0
+    for i in range(0, batch, max(1, batch // 5)):
+        want = newton_schulz(grad[i], 5, False)
+        x = grad[i].double() / grad[i].double().norm()
+        left, size, right = torch.linalg.svd(x, full_matrices=False)
+        growth = float((torch.einsum("ik,ij,kj->k", left, want, right) / size).max())
+        assert (master[i].double() - want).norm() <= 16 * (2.0 ** -22 + 8 * 2.0 ** -23) * growth * want.norm()
+
+
+@pytest.mark.gpu
 def test_singular_values_come_near_one(mg):
     """Five steps take a well-spread spectrum into [0.6, 1.25] (the quintic's band [0.68, 1.21] and 0.3 % for the roundings)."""
     gen = torch.Generator(device="cuda").manual_seed(1)
