@@ -107,83 +107,67 @@ __device__ __forceinline__ uint2 pack_half4(float a, float b, float c, float d) 
     return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
 
-// Four columns (from col on) of an output row; v: the accumulator, x, g and
-// master: what the epilogue reads there (x 0 where X is not kept).
-template <int KIND>
-__device__ __forceinline__ void ns_store4(const NsProduct& p, int64_t at, int64_t finAt, int col, const float4& v,
-                                          const float4& x, const uint2& g, const float4& master, bool finVec) {
+// Four columns (from col on) of a row of X; v: the accumulator, x and master:
+// what was read there (x 0 where X is not kept).
+__device__ __forceinline__ void ns_apply4(const NsProduct& p, int64_t at, int64_t finAt, int col, const float4& v, const float4& x,
+                                          const float4& master, bool finVec) {
     float y[4] = {v.x, v.y, v.z, v.w};
-    if constexpr (KIND == kNsApply) {
-        const float xv[4] = {x.x, x.y, x.z, x.w};
+    const float xv[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int i = 0; i < 4; i++) y[i] = fmaf(p.a, xv[i], y[i] * (kNsUnscale * kNsUnscale));
-        if (!p.last) {
-            *reinterpret_cast<float4*>(p.x32 + at) = make_float4(y[0], y[1], y[2], y[3]);
-            *reinterpret_cast<uint2*>(p.out16 + at) =
-                pack_half4(y[0] * kNsScale, y[1] * kNsScale, y[2] * kNsScale, y[3] * kNsScale);
-            return;
-        }
-        const int n = min(4, p.N - col);
-        if (p.fin.master) {
-            float* m = p.fin.master + finAt;
-            if (finVec && n == 4) {
-                const float ov[4] = {master.x, master.y, master.z, master.w};
+    for (int i = 0; i < 4; i++) y[i] = fmaf(p.a, xv[i], y[i] * (kNsUnscale * kNsUnscale));
+    if (!p.last) {
+        *reinterpret_cast<float4*>(p.x32 + at) = make_float4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<uint2*>(p.out16 + at) = pack_half4(y[0] * kNsScale, y[1] * kNsScale, y[2] * kNsScale, y[3] * kNsScale);
+        return;
+    }
+    const int n = min(4, p.N - col);
+    const bool vec = finVec && n == 4;
+    if (p.fin.master) {
+        float* m = p.fin.master + finAt;
+        if (vec) {
+            const float mv[4] = {master.x, master.y, master.z, master.w};
 #pragma unroll
-                for (int i = 0; i < 4; i++) y[i] = __fsub_rn(__fmul_rn(ov[i], p.fin.keep), __fmul_rn(p.fin.rate, y[i]));
-                *reinterpret_cast<float4*>(m) = make_float4(y[0], y[1], y[2], y[3]);
-                const __nv_bfloat162 a = __floats2bfloat162_rn(y[0], y[1]), b = __floats2bfloat162_rn(y[2], y[3]);
-                *reinterpret_cast<uint2*>(p.fin.weights + finAt) =
-                    make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (i < n) {
-                        const float w = __fsub_rn(__fmul_rn(m[i], p.fin.keep), __fmul_rn(p.fin.rate, y[i]));
-                        m[i] = w;
-                        p.fin.weights[finAt + i] = __float2bfloat16_rn(w);
-                    }
-            }
-            return;
-        }
-        if (p.fin.outBf16) {
-            __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.fin.out) + finAt;
-            if (finVec && n == 4) {
-                const __nv_bfloat162 a = __floats2bfloat162_rn(y[0], y[1]), b = __floats2bfloat162_rn(y[2], y[3]);
-                *reinterpret_cast<uint2*>(o) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (i < n) o[i] = __float2bfloat16_rn(y[i]);
-            }
+            for (int i = 0; i < 4; i++) y[i] = __fsub_rn(__fmul_rn(mv[i], p.fin.keep), __fmul_rn(p.fin.rate, y[i]));
+            *reinterpret_cast<float4*>(m) = make_float4(y[0], y[1], y[2], y[3]);
+            const __nv_bfloat162 a = __floats2bfloat162_rn(y[0], y[1]), b = __floats2bfloat162_rn(y[2], y[3]);
+            *reinterpret_cast<uint2*>(p.fin.weights + finAt) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
         } else {
-            __half* o = static_cast<__half*>(p.fin.out) + finAt;
-            if (finVec && n == 4) {
-                *reinterpret_cast<uint2*>(o) = pack_half4(y[0], y[1], y[2], y[3]);
-            } else {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    if (i < n) o[i] = __float2half_rn(y[i]);
-            }
+            for (int i = 0; i < 4; i++)
+                if (i < n) {
+                    const float w = __fsub_rn(__fmul_rn(m[i], p.fin.keep), __fmul_rn(p.fin.rate, y[i]));
+                    m[i] = w;
+                    p.fin.weights[finAt + i] = __float2bfloat16_rn(w);
+                }
+        }
+    } else if (p.fin.outBf16) {
+        __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.fin.out) + finAt;
+        if (vec) {
+            const __nv_bfloat162 a = __floats2bfloat162_rn(y[0], y[1]), b = __floats2bfloat162_rn(y[2], y[3]);
+            *reinterpret_cast<uint2*>(o) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (i < n) o[i] = __float2bfloat16_rn(y[i]);
         }
     } else {
+        __half* o = static_cast<__half*>(p.fin.out) + finAt;
+        if (vec) {
+            *reinterpret_cast<uint2*>(o) = pack_half4(y[0], y[1], y[2], y[3]);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) y[i] *= kNsUnscale;  // scaled by 2^10, as the operands are
-        if (KIND == kNsPoly) {
-            const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&g.x));
-            const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&g.y));
-            y[0] = fmaf(p.c, y[0], p.b * g0.x);
-            y[1] = fmaf(p.c, y[1], p.b * g0.y);
-            y[2] = fmaf(p.c, y[2], p.b * g1.x);
-            y[3] = fmaf(p.c, y[3], p.b * g1.y);
+            for (int i = 0; i < 4; i++)
+                if (i < n) o[i] = __float2half_rn(y[i]);
         }
-        *reinterpret_cast<uint2*>(p.out16 + at) = pack_half4(y[0], y[1], y[2], y[3]);
     }
 }
 
 // A 32 x 32 piece at (row0, col0) of matrix b's output: lane r holds row r in v.
 // Of a symmetric product, pieces below the diagonal are left to their mirror
-// pieces above it, which write both: every entry is written once.
-template <int KIND>
+// pieces above it, which write both: every entry is written once. BATCH: loads
+// of a lane that go out before the first is used.
+template <int KIND, int BATCH>
 __device__ __forceinline__ void ns_piece(const NsProduct& p, int b, int row0, int col0, uint8_t* slab, const float* v) {
     const int lane = threadIdx.x & 31;
     if (KIND != kNsApply && col0 < row0) return;
@@ -196,15 +180,15 @@ __device__ __forceinline__ void ns_piece(const NsProduct& p, int b, int row0, in
     const int k = lane & 7, col = col0 + 4 * k;
     const bool in = col < p.N;  // then the four columns lie inside ldo
     const bool finVec = KIND == kNsApply && p.last && p.fin.vec;
+    const bool mirror = KIND != kNsApply && col0 != row0;
     if (in) {
-        // the loads of four rows go out before the first is used
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            float4 x[4], m[4];
-            uint2 g[4];
+        for (int h = 0; h < 8 / BATCH; h++) {
+            float4 x[BATCH], m[BATCH];
+            uint2 g[BATCH];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int row = row0 + (4 * h + i) * 4 + (lane >> 3);
+            for (int i = 0; i < BATCH; i++) {
+                const int row = row0 + (BATCH * h + i) * 4 + (lane >> 3);
                 x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 m[i] = x[i];
                 g[i] = make_uint2(0u, 0u);
@@ -216,15 +200,36 @@ __device__ __forceinline__ void ns_piece(const NsProduct& p, int b, int row0, in
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int r = (4 * h + i) * 4 + (lane >> 3), row = row0 + r;
-                if (row < p.M)
-                    ns_store4<KIND>(p, base + (int64_t)row * p.ldo + col, (int64_t)b * p.fin.stride + (int64_t)row * p.fin.ld + col,
-                                    col, *reinterpret_cast<const float4*>(slab + ns_slab_offset(r, k)), x[i], g[i], m[i], finVec);
+            for (int i = 0; i < BATCH; i++) {
+                const int r = (BATCH * h + i) * 4 + (lane >> 3), row = row0 + r;
+                float4* cell = reinterpret_cast<float4*>(slab + ns_slab_offset(r, k));
+                float4 y = *cell;
+                if (KIND == kNsApply) {
+                    if (row < p.M)
+                        ns_apply4(p, base + (int64_t)row * p.ldo + col, (int64_t)b * p.fin.stride + (int64_t)row * p.fin.ld + col, col, y,
+                                  x[i], m[i], finVec);
+                } else {
+                    y.x *= kNsUnscale;  // scaled by 2^10, as the operands are
+                    y.y *= kNsUnscale;
+                    y.z *= kNsUnscale;
+                    y.w *= kNsUnscale;
+                    if (KIND == kNsPoly) {
+                        const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&g[i].x));
+                        const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&g[i].y));
+                        y.x = fmaf(p.c, y.x, p.b * g0.x);
+                        y.y = fmaf(p.c, y.y, p.b * g0.y);
+                        y.z = fmaf(p.c, y.z, p.b * g1.x);
+                        y.w = fmaf(p.c, y.w, p.b * g1.y);
+                    }
+                    if (row < p.M)
+                        *reinterpret_cast<uint2*>(p.out16 + base + (int64_t)row * p.ldo + col) = pack_half4(y.x, y.y, y.z, y.w);
+                    if (mirror) *cell = y;
+                }
             }
         }
     }
-    if (KIND == kNsApply || col0 == row0) return;
+    if (!mirror) return;
+    __syncwarp();
     // the mirrored piece, row col0 + lane: column row0 + r is this piece's (r, lane)
     const int mrow = col0 + lane;
     if (mrow < p.M) {
@@ -234,20 +239,8 @@ __device__ __forceinline__ void ns_piece(const NsProduct& p, int b, int row0, in
             if (row0 + 8 * q >= p.ldo) break;
             float y[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int r = 8 * q + i;
-                y[i] = *reinterpret_cast<const float*>(slab + ns_slab_offset(r, lane >> 2) + (lane & 3) * 4) * kNsUnscale;
-            }
-            if (KIND == kNsPoly) {  // G is symmetric: the same values as the direct piece's
-                const uint4 gw = *reinterpret_cast<const uint4*>(p.g16 + at + 8 * q);
-                const uint32_t w[4] = {gw.x, gw.y, gw.z, gw.w};
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-                    y[2 * i] = fmaf(p.c, y[2 * i], p.b * f.x);
-                    y[2 * i + 1] = fmaf(p.c, y[2 * i + 1], p.b * f.y);
-                }
-            }
+            for (int i = 0; i < 8; i++)
+                y[i] = *reinterpret_cast<const float*>(slab + ns_slab_offset(8 * q + i, lane >> 2) + (lane & 3) * 4);
             const uint2 lo = pack_half4(y[0], y[1], y[2], y[3]), hi = pack_half4(y[4], y[5], y[6], y[7]);
             *reinterpret_cast<uint4*>(p.out16 + at + 8 * q) = make_uint4(lo.x, lo.y, hi.x, hi.y);
         }
@@ -385,7 +378,7 @@ __global__ void __launch_bounds__(NsTile<BN>::THREADS, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&tempty[a]);
                 }
-                if (row0 < p.M && n0 + 32 * c < p.N) ns_piece<KIND>(p, b, row0, n0 + 32 * c, slab, v);
+                if (row0 < p.M && n0 + 32 * c < p.N) ns_piece<KIND, 8>(p, b, row0, n0 + 32 * c, slab, v);
             }
         }
     }

@@ -36,13 +36,13 @@ struct MuonInput {
     float* normSqOut;
 };
 
-constexpr int kMuonSmallSide = 128, kMuonSmallSteps = 6, kMuonSmallThreads = 256;
+constexpr int kMuonSmallSide = 128, kMuonSmallSteps = 6, kMuonSmallThreads = 512;
 constexpr int kMuonSmallCluster = 8;
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
 
 struct MuonSmall {
     static constexpr int MAT = 65536;  // a matrix's or a tile's two fp16 parts
-    static constexpr int SLAB_OFF = 3 * MAT, BAR_OFF = SLAB_OFF + 8 * 4096;
+    static constexpr int BAR_OFF = 3 * MAT;
     static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024 /*align*/;
 };
 
@@ -162,19 +162,39 @@ __device__ __forceinline__ void split_mma(uint32_t d, uint32_t a, uint32_t b, bo
     }
 }
 
+// 32 lanes x N consecutive fp32 columns of tensor memory, N = 16 or 32.
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t taddr, float* v) {
+    if constexpr (N == 32) {
+        tmem_ld32(taddr, v);
+    } else {
+        static_assert(N == 16, "16 or 32 columns");
+        uint32_t r[16];
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+              "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(taddr));
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; i++) v[i] = __uint_as_float(r[i]);
+    }
+}
+
 // SP: the smaller side padded, 64 or 128. WIDE: rows <= cols.
 template <int SP, bool WIDE, class T, bool MUON>
 __global__ void __launch_bounds__(kMuonSmallThreads, 1)
     k_muon_small(const MuonInput in, const NsProduct p, int steps, int vec, int parts) {
     using S = MuonSmall;
-    constexpr int KS = SP / 16, COLS = SP / 2;  // COLS: columns of an s x s matrix that a thread holds
+    constexpr int KS = SP / 16, COLS = SP / 4;  // COLS: columns of an s x s matrix that a thread holds
+    constexpr int WARPS = kMuonSmallThreads / 32;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *mG = smem, *mQ = smem + S::MAT, *mP = smem + 2 * S::MAT;
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + S::BAR_OFF);  // [2]
     double* sNorm = reinterpret_cast<double*>(bar + 2);
-    double* sSum = sNorm + 1;  // [8]
-    float* sScale = reinterpret_cast<float*>(sSum + 8);
+    double* sSum = sNorm + 1;  // [WARPS]
+    float* sScale = reinterpret_cast<float*>(sSum + WARPS);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sScale + 1);
     mg_pdl_trigger();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -235,22 +255,25 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
     constexpr int CELLS = SP * 16;
     auto cellIndex = [&](int j) { return WIDE || SP == 128 ? j : (j / (SP / 8)) * 16 + j % (SP / 8); };
 
-    // |U|^2 (and the momentum)
+    constexpr int PER = CELLS / kMuonSmallThreads;  // cells of a thread
+
+    // |U|^2 (and the momentum); the first piece stays in registers for its tile
     double sum = 0.0;
-    for (int i = first; i < end; i++)
-#pragma unroll 2
-        for (int j = tid; j < CELLS; j += kMuonSmallThreads) {
-            float u[8];
-            cell(i, cellIndex(j), true, u);
+    float held[PER][8];
+#pragma unroll 1
+    for (int i = end - 1; i >= first; i--)
 #pragma unroll
-            for (int k = 0; k < 8; k++) sum += (double)u[k] * (double)u[k];
+        for (int j = 0; j < PER; j++) {
+            cell(i, cellIndex(tid + j * kMuonSmallThreads), true, held[j]);
+#pragma unroll
+            for (int k = 0; k < 8; k++) sum += (double)held[j][k] * (double)held[j][k];
         }
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
     if (lane == 0) sSum[warp] = sum;
     __syncthreads();
     if (tid == 0) {
-        for (int w = 1; w < 8; w++) sum += sSum[w];
+        for (int w = 1; w < WARPS; w++) sum += sSum[w];
         *sNorm = sum;
     }
     if (parts > 1) {
@@ -262,15 +285,18 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
         sum = *sNorm;
     }
     const double inv = sum == 0.0 ? 0.0 : 1.0 / sqrt(sum);
-    // piece i of X into a tile
-    auto tile = [&](uint8_t* mat, int i) {
-#pragma unroll 2
-        for (int j = tid; j < CELLS; j += kMuonSmallThreads) {
-            const int g = cellIndex(j);
-            float u[8];
-            cell(i, g, false, u);
+    // piece i of X (from `held`, where its loads are, or were) into a tile
+    auto load = [&](int i) {
 #pragma unroll
-            for (int k = 0; k < 8; k++) u[k] = (float)((double)u[k] * inv) * kNsScale;
+        for (int j = 0; j < PER; j++) cell(i, cellIndex(tid + j * kMuonSmallThreads), false, held[j]);
+    };
+    auto tile = [&](uint8_t* mat) {
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int g = cellIndex(tid + j * kMuonSmallThreads);
+            float u[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) u[k] = (float)((double)held[j][k] * inv) * kNsScale;
             split_store8(mat, sw128_offset(g >> 4, g & 15), u);
         }
         handOver();
@@ -280,8 +306,9 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
     for (int i = first; i < end; i++) {
         const int k = (i - first) & 1;
         uint8_t* mat = k ? mP : mQ;
+        if (i > first) load(i);
         if (i - first >= 2) wait(k);
-        tile(mat, i);
+        tile(mat);
         if (tid == 0) {
             split_mma<!WIDE, !WIDE, SP, 8>(tmem, smem_u32(mat), smem_u32(mat), i > first);
             tc_commit(&bar[k]);
@@ -293,20 +320,17 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
     const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16);
     const bool holds = 32 * q < SP;  // warps 2 and 3 of four have no rows of a 64-row matrix
     if (holds) {
-#pragma unroll 1
-        for (int c = c0; c < c0 + COLS; c += 32) {
-            float v[32];
-            if (end > first) {
-                tmem_ld32(acc + (uint32_t)c, v);
-            } else {
+        float v[COLS];
+        if (end > first) {
+            tmem_load<COLS>(acc + (uint32_t)c0, v);
+        } else {
 #pragma unroll
-                for (int k = 0; k < 32; k++) v[k] = 0.0f;
-            }
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-                *reinterpret_cast<float4*>(mG + tile_offset(row, c / 4 + k)) =
-                    make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+            for (int k = 0; k < COLS; k++) v[k] = 0.0f;
         }
+#pragma unroll
+        for (int k = 0; k < COLS / 4; k++)
+            *reinterpret_cast<float4*>(mG + tile_offset(row, c0 / 4 + k)) =
+                make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
     }
     if (parts > 1) {
         // CTA k sums rows k SP / parts .. of all parts, in their order, and hands
@@ -357,112 +381,101 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
 
     // the steps
     const uint32_t aG = smem_u32(mG), aQ = smem_u32(mQ), aP = smem_u32(mP);
-    // an accumulator times f into a matrix
-    auto take = [&](uint32_t column, uint8_t* mat, float f) {
+    // an accumulator, scaled by 2^10 more than the matrix, into the matrix
+    auto take = [&](uint32_t column, uint8_t* mat) {
         if (!holds) return;
-#pragma unroll 1
-        for (int c = c0; c < c0 + COLS; c += 32) {
-            float v[32];
-            tmem_ld32(acc + column + (uint32_t)c, v);
+        float v[COLS];
+        tmem_load<COLS>(acc + column + (uint32_t)c0, v);
 #pragma unroll
-            for (int k = 0; k < 32; k++) v[k] *= f;
+        for (int k = 0; k < COLS; k++) v[k] *= kNsUnscale;
 #pragma unroll
-            for (int k = 0; k < 4; k++) split_store8(mat, sw128_offset(row, c / 8 + k), v + 8 * k);
+        for (int k = 0; k < COLS / 8; k++) split_store8(mat, sw128_offset(row, c0 / 8 + k), v + 8 * k);
+    };
+    auto multiply = [&](uint32_t column, uint32_t x, uint32_t y, int bit) {
+        if (tid == 0) {
+            split_mma<false, false, SP, KS>(tmem + column, x, y, false);
+            tc_commit(&bar[bit]);
         }
     };
+    // P's products run behind those that the next G waits for, and are taken up
+    // while the next product runs.
     for (int step = 0; step < steps; step++) {
         const bool more = step + 1 < steps;
-        if (tid == 0) {
-            split_mma<false, false, SP, KS>(tmem, aG, aG, false);
-            tc_commit(&bar[0]);
-        }
+        multiply(0, aG, aG, 0);
         wait(0);
         if (holds) {  // Q = a I + b G + c G^2
-#pragma unroll 1
-            for (int c = c0; c < c0 + COLS; c += 32) {
-                float v[32];
-                tmem_ld32(acc + (uint32_t)c, v);
+            float v[COLS];
+            tmem_load<COLS>(acc + (uint32_t)c0, v);
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    float g[8];
-                    split_load8(mG, sw128_offset(row, c / 8 + k), g);
+            for (int k = 0; k < COLS / 8; k++) {
+                float g[8];
+                split_load8(mG, sw128_offset(row, c0 / 8 + k), g);
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        float y = fmaf(kNsC * kNsUnscale, v[8 * k + i], kNsB * g[i]);  // times 2^10
-                        if (c + 8 * k + i == row && row < s) y += kNsA * kNsScale;
-                        g[i] = y;
-                    }
-                    split_store8(mQ, sw128_offset(row, c / 8 + k), g);
-                    if (step == 0) {  // P = Q
+                for (int i = 0; i < 8; i++) {
+                    float y = fmaf(kNsC * kNsUnscale, v[8 * k + i], kNsB * g[i]);  // times 2^10
+                    if (c0 + 8 * k + i == row && row < s) y += kNsA * kNsScale;
+                    g[i] = y;
+                }
+                split_store8(mQ, sw128_offset(row, c0 / 8 + k), g);
+                if (step == 0) {  // P = Q, scaled by 2^5 throughout
 #pragma unroll
-                        for (int i = 0; i < 8; i++) g[i] *= 0.03125f;
-                        split_store8(mP, sw128_offset(row, c / 8 + k), g);
-                    }
+                    for (int i = 0; i < 8; i++) g[i] *= 0.03125f;
+                    split_store8(mP, sw128_offset(row, c0 / 8 + k), g);
                 }
             }
         }
         handOver();
-        if (step == 0 && !more) break;
-        if (tid == 0) {
-            if (more) split_mma<false, false, SP, KS>(tmem, aQ, aG, false);
-            if (step > 0) split_mma<false, false, SP, KS>(tmem + 128, aQ, aP, false);
-            tc_commit(&bar[0]);
+        if (more) multiply(0, aQ, aG, 0);
+        if (step > 0) multiply(128, aQ, aP, 1);
+        if (more) {
+            wait(0);
+            take(0, mG);  // Q G, in G's place
+            handOver();
+            multiply(0, aQ, aG, 0);
         }
-        wait(0);
-        if (more) take(0, mG, kNsUnscale);             // Q G, in G's place
-        if (step > 0) take(128, mP, kNsUnscale);       // P: scaled by 2^5 throughout
-        handOver();
-        if (!more) break;
-        if (tid == 0) {
-            split_mma<false, false, SP, KS>(tmem, aQ, aG, false);
-            tc_commit(&bar[0]);
+        if (step > 0) {
+            wait(1);
+            take(128, mP);
         }
-        wait(0);
-        take(0, mG, kNsUnscale);  // Q G Q
+        if (more) {
+            wait(0);
+            take(0, mG);  // Q G Q
+        }
         handOver();
     }
 
-    // P X, piece by piece, the tiles alternating between G's and Q's places
+    // P X, piece by piece: the next piece's product beside this one's epilogue. The
+    // tiles take G's place, the epilogue's slabs Q's.
     constexpr int N = WIDE ? 128 : SP;
-    uint8_t* slab = smem + S::SLAB_OFF + warp * 4096;
+    uint8_t* slab = mQ + warp * 4096;
     auto issue = [&](int i) {
         const int k = (i - first) & 1;
-        const uint32_t x = k ? aQ : aG;
+        tile(mG);
         if (tid == 0) {
             if (WIDE)
-                split_mma<false, true, N, KS>(tmem + 128 * k, aP, x, false);
+                split_mma<false, true, N, KS>(tmem + 128 * k, aP, aG, false);
             else
-                split_mma<false, false, N, KS>(tmem + 128 * k, x, aP, false);
+                split_mma<false, false, N, KS>(tmem + 128 * k, aG, aP, false);
             tc_commit(&bar[k]);
         }
     };
     if (first < end) {
-        tile(mG, first);
+        load(first);
         issue(first);
     }
     for (int i = first; i < end; i++) {
         const int k = (i - first) & 1;
-        if (i + 1 < end) {
-            tile(k ? mG : mQ, i + 1);
-            issue(i + 1);
-        }
+        if (i + 1 < end) load(i + 1);
         wait(k);
-        const int row0 = 32 * q + (WIDE ? 0 : 128 * i);
-        if (row0 < rows && (!WIDE || 32 * q < SP)) {
-#pragma unroll 1
-            for (int c = (warp >> 2) * (N / 2); c < ((warp >> 2) + 1) * (N / 2); c += 32) {
-                const int col0 = c + (WIDE ? 128 * i : 0);
-                if (col0 >= cols) break;
-                float v[32];
-                tmem_ld32(acc + (uint32_t)(128 * k + c), v);
+        if (i + 1 < end) issue(i + 1);
+        const int row0 = 32 * q + (WIDE ? 0 : 128 * i), c = 32 * (warp >> 2), col0 = c + (WIDE ? 128 * i : 0);
+        if (row0 < rows && c < N && col0 < cols && (!WIDE || 32 * q < SP)) {
+            float v[32];
+            tmem_ld32(acc + (uint32_t)(128 * k + c), v);
 #pragma unroll
-                for (int j = 0; j < 32; j++) v[j] *= 32.0f;  // to the scale of ns_piece, 2^20
-                ns_piece<kNsApply>(p, b, row0, col0, slab, v);
-            }
+            for (int j = 0; j < 32; j++) v[j] *= 32.0f;  // to the scale of ns_piece, 2^20
+            ns_piece<kNsApply, 4>(p, b, row0, col0, slab, v);
         }
-        tc_fence_before();
-        __syncthreads();
-        tc_fence_after();
     }
     tc_fence_before();
     __syncthreads();
