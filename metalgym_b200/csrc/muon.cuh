@@ -9,8 +9,10 @@
 //   kNsApply  X <- a X + B X or a X + X B, or in the last step what the caller
 //             wants of it
 //
-// Warp roles (320 threads): 0 TMA producer, 1 MMA issuer, 2-9 epilogue (warp w:
-// accumulator lanes 32 (w % 4) .., one half of the columns).
+// Warp roles: 0 TMA producer, 1 MMA issuer, the others epilogue (warp w:
+// accumulator lanes 32 (w % 4) .., a part of the columns): 16 at 128-wide tiles,
+// where small matrices wait for it, 8 at 256-wide ones, where it runs beside
+// the next tile and shared memory is better spent on a fourth stage.
 // The epilogue takes 32 x 32 pieces from tensor memory through a swizzled
 // 4 KB slab of shared memory: a thread of tcgen05.ld has a row, and rows are
 // far apart in memory; out of the slab, eight lanes hold 32 consecutive columns
@@ -56,9 +58,10 @@ struct NsProduct {
 
 template <int BN>
 struct NsTile {
-    static constexpr int BM = 128, BK = 64, STAGES = BN == 256 ? 4 : 6;
+    static constexpr int BM = 128, BK = 64, STAGES = BN == 256 ? 4 : 5;
     static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int EW = 8, THREADS = 64 + 32 * EW, SLAB = 4096;
+    static constexpr int EW = BN == 256 ? 8 : 16, THREADS = 64 + 32 * EW, SLAB = 4096;
+    static constexpr int PIECES = BN / (8 * EW);  // 32-column pieces of an epilogue warp
     static constexpr int SLAB_OFF = STAGES * STAGE_BYTES, BAR_OFF = SLAB_OFF + EW * SLAB;
     static constexpr int TMEM_COLS = 2 * BN;
     static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024 /*align*/;
@@ -163,14 +166,37 @@ __device__ __forceinline__ void ns_apply4(const NsProduct& p, int64_t at, int64_
     }
 }
 
+// What the epilogue of a 32 x 32 piece reads: four columns of eight rows a lane
+// (eight lanes to a row). It does not depend on the product, so the loads go
+// out before the accumulator is waited for.
+template <int KIND>
+struct NsFetched {
+    float4 x[KIND == kNsApply ? 8 : 1];
+    uint2 g[KIND == kNsPoly ? 8 : 1];
+};
+template <int KIND>
+__device__ __forceinline__ void ns_fetch(const NsProduct& p, int b, int row0, int col0, NsFetched<KIND>& f) {
+    const int lane = threadIdx.x & 31, col = col0 + 4 * (lane & 7);
+    const int64_t at = ((int64_t)b * p.M + row0 + (lane >> 3)) * p.ldo + col;
+    if (KIND == kNsApply && !p.x32) return;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if (KIND == kNsApply) f.x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (KIND == kNsPoly) f.g[i] = make_uint2(0u, 0u);
+        if (col < p.N && row0 + 4 * i + (lane >> 3) < p.M) {
+            if (KIND == kNsApply) f.x[i] = ld_f4_now(p.x32 + at + (int64_t)(4 * i) * p.ldo);
+            if (KIND == kNsPoly) f.g[i] = *reinterpret_cast<const uint2*>(p.g16 + at + (int64_t)(4 * i) * p.ldo);
+        }
+    }
+}
+
 // A 32 x 32 piece at (row0, col0) of matrix b's output: lane r holds row r in v.
 // Of a symmetric product, pieces below the diagonal are left to their mirror
-// pieces above it, which write both: every entry is written once. BATCH: loads
-// of a lane that go out before the first is used.
-template <int KIND, int BATCH>
-__device__ __forceinline__ void ns_piece(const NsProduct& p, int b, int row0, int col0, uint8_t* slab, const float* v) {
+// pieces above it, which write both: every entry is written once.
+template <int KIND>
+__device__ __forceinline__ void ns_piece(const NsProduct& p, int b, int row0, int col0, uint8_t* slab, const float* v,
+                                         const NsFetched<KIND>& f) {
     const int lane = threadIdx.x & 31;
-    if (KIND != kNsApply && col0 < row0) return;
     __syncwarp();  // the slab's last readers are done
 #pragma unroll
     for (int k = 0; k < 8; k++)
@@ -178,44 +204,39 @@ __device__ __forceinline__ void ns_piece(const NsProduct& p, int b, int row0, in
     __syncwarp();
     const int64_t base = (int64_t)b * p.M * p.ldo;
     const int k = lane & 7, col = col0 + 4 * k;
-    const bool in = col < p.N;  // then the four columns lie inside ldo
     const bool finVec = KIND == kNsApply && p.last && p.fin.vec;
     const bool mirror = KIND != kNsApply && col0 != row0;
-    if (in) {
+    if (col < p.N) {  // then the four columns lie inside ldo
 #pragma unroll
-        for (int h = 0; h < 8 / BATCH; h++) {
-            float4 x[BATCH], m[BATCH];
-            uint2 g[BATCH];
+        for (int h = 0; h < 2; h++) {
+            float4 m[4];
+            if (KIND == kNsApply) {
 #pragma unroll
-            for (int i = 0; i < BATCH; i++) {
-                const int row = row0 + (BATCH * h + i) * 4 + (lane >> 3);
-                x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                m[i] = x[i];
-                g[i] = make_uint2(0u, 0u);
-                if (row < p.M) {
-                    if (KIND == kNsApply && finVec && p.fin.master && col + 4 <= p.N)
+                for (int i = 0; i < 4; i++) {
+                    const int row = row0 + (4 * h + i) * 4 + (lane >> 3);
+                    m[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (finVec && p.fin.master && col + 4 <= p.N && row < p.M)
                         m[i] = ld_f4_now(p.fin.master + (int64_t)b * p.fin.stride + (int64_t)row * p.fin.ld + col);
-                    if (KIND == kNsApply && p.x32) x[i] = ld_f4_now(p.x32 + base + (int64_t)row * p.ldo + col);
-                    if (KIND == kNsPoly) g[i] = *reinterpret_cast<const uint2*>(p.g16 + base + (int64_t)row * p.ldo + col);
                 }
             }
 #pragma unroll
-            for (int i = 0; i < BATCH; i++) {
-                const int r = (BATCH * h + i) * 4 + (lane >> 3), row = row0 + r;
+            for (int i = 0; i < 4; i++) {
+                const int r = (4 * h + i) * 4 + (lane >> 3), row = row0 + r;
                 float4* cell = reinterpret_cast<float4*>(slab + ns_slab_offset(r, k));
                 float4 y = *cell;
-                if (KIND == kNsApply) {
+                if constexpr (KIND == kNsApply) {
                     if (row < p.M)
                         ns_apply4(p, base + (int64_t)row * p.ldo + col, (int64_t)b * p.fin.stride + (int64_t)row * p.fin.ld + col, col, y,
-                                  x[i], m[i], finVec);
+                                  p.x32 ? f.x[4 * h + i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f), m[i], finVec);
                 } else {
                     y.x *= kNsUnscale;  // scaled by 2^10, as the operands are
                     y.y *= kNsUnscale;
                     y.z *= kNsUnscale;
                     y.w *= kNsUnscale;
-                    if (KIND == kNsPoly) {
-                        const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&g[i].x));
-                        const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&g[i].y));
+                    if constexpr (KIND == kNsPoly) {
+                        const uint2 gw = f.g[4 * h + i];
+                        const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&gw.x));
+                        const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&gw.y));
                         y.x = fmaf(p.c, y.x, p.b * g0.x);
                         y.y = fmaf(p.c, y.y, p.b * g0.y);
                         y.z = fmaf(p.c, y.z, p.b * g1.x);
@@ -358,28 +379,37 @@ __global__ void __launch_bounds__(NsTile<BN>::THREADS, 1)
             tc_commit(done);  // covers every MMA issued, also after a timeout
         }
     } else {
-        const int q = warp & 3, e = warp - 2, half = (e / 4) * (BN / 2);
+        bool gaveUp = false;  // a wait gave up
+        const int q = warp & 3, e = warp - 2, part = (e / 4) * (BN * 4 / S::EW);
         uint8_t* slab = smem + S::SLAB_OFF + e * S::SLAB;
         int t = 0;
         for (int u = blockIdx.x; u < units; u += gridDim.x, t++) {
             const int b = u / perMatrix, a = t & 1;
             int ti, tj;
             ns_tile_at<KIND, BN>(u - b * perMatrix, p.tilesN, ti, tj);
-            const int row0 = ti * S::BM + 32 * q, n0 = tj * BN + half;
-            if (!mbar_wait_warp(&tfull[a], (t >> 1) & 1, p.status, kDevTimeoutDone)) break;
-            tc_fence_after();
-            const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN + half);
+            const int row0 = ti * S::BM + 32 * q, n0 = tj * BN + part;
+            const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN + part);
 #pragma unroll 1
-            for (int c = 0; c < BN / 64; c++) {
+            for (int c = 0; c < S::PIECES; c++) {
+                const int col0 = n0 + 32 * c;
+                const bool wanted = row0 < p.M && col0 < p.N && (KIND == kNsApply || col0 >= row0);
+                NsFetched<KIND> f;
+                if (wanted) ns_fetch<KIND>(p, b, row0, col0, f);
+                if (c == 0) {
+                    if (!mbar_wait_warp(&tfull[a], (t >> 1) & 1, p.status, kDevTimeoutDone)) gaveUp = true;
+                    if (gaveUp) break;
+                    tc_fence_after();
+                }
                 float v[32];
                 tmem_ld32(acc + (uint32_t)(c * 32), v);
-                if (c == BN / 64 - 1) {  // the accumulator is free for the tile after next
+                if (c == S::PIECES - 1) {  // the accumulator is free for the tile after next
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&tempty[a]);
                 }
-                if (row0 < p.M && n0 + 32 * c < p.N) ns_piece<KIND, 8>(p, b, row0, n0 + 32 * c, slab, v);
+                if (wanted) ns_piece<KIND>(p, b, row0, col0, slab, v, f);
             }
+            if (gaveUp) break;
         }
     }
     tc_fence_before();

@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
             tmem_ld32(acc + (uint32_t)(128 * k + c), v);
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] *= 32.0f;  // to the scale of ns_piece, 2^20
-            ns_piece<kNsApply, 4>(p, b, row0, col0, slab, v);
+            ns_piece<kNsApply>(p, b, row0, col0, slab, v, NsFetched<kNsApply>{});
         }
     }
     tc_fence_before();
