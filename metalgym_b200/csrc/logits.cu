@@ -179,6 +179,11 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
+__device__ __forceinline__ float log2_fast(float x) {  // within 2^-22 (absolute near 1)
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // The largest of a warp's values (NaN ignored).
 __device__ __forceinline__ float warp_max(float x) {
     float y;
@@ -204,19 +209,6 @@ struct Softmax {
         if (!(s != s)) s = s * e;
         m = top;
         return e;
-    }
-    __device__ __forceinline__ void merge(const Softmax& o) {
-        if (o.m == -INFINITY && o.s == 0.0f) return;
-        if (m == -INFINITY && s == 0.0f) {
-            *this = o;
-            return;
-        }
-        const float top = fmaxf(m, o.m);
-        const float da = m - top, db = o.m - top, ea = exp2f(da), eb = exp2f(db);
-        const float ta = ea == 0.0f ? 0.0f : ea * (t + s * da), tb = eb == 0.0f ? 0.0f : eb * (o.t + o.s * db);
-        s = s * ea + o.s * eb;
-        t = ta + tb;
-        m = top;
     }
 };
 
@@ -280,7 +272,7 @@ struct Runner {
 };
 
 // Whether a's key is above b's (equal keys: the lower action). 32 bits decide
-// where they can: both keys are good to about 2^-21 of their size.
+// where they can: both keys are good to well within the margin.
 template <bool GREEDY>
 __device__ __forceinline__ bool beats(const Runner& a, const Runner& b) {
     if (a.action < 0 || b.action < 0) return a.action >= 0;
@@ -292,7 +284,16 @@ __device__ __forceinline__ bool beats(const Runner& a, const Runner& b) {
     return ka > kb || (ka == kb && a.action < b.action);
 }
 
-// What the CTAs of a row tell each other.
+__device__ __forceinline__ Runner runner_xor(const Runner& r, int d) {
+    Runner o;
+    o.key = __shfl_xor_sync(0xffffffffu, r.key, d);
+    o.logit = __shfl_xor_sync(0xffffffffu, r.logit, d);
+    o.bits = __shfl_xor_sync(0xffffffffu, r.bits, d);
+    o.action = __shfl_xor_sync(0xffffffffu, r.action, d);
+    return o;
+}
+
+// What the warps of a row tell each other.
 struct RowPart {
     Softmax v;
     Runner best;
@@ -309,44 +310,58 @@ __device__ __forceinline__ float warp_add(float x) {
 // one fixed order: lanes, warps, CTAs. With several parts the caller ends with
 // cluster_sync, so that no CTA leaves while another reads its part.
 template <int NT, bool RACE, bool GREEDY>
-__device__ inline void row_merge(RowPart& mine, RowPart* warps, RowPart* whole, int parts, int chosenRank) {
+__device__ inline void row_merge(RowPart& mine, RowPart* warps, int parts, int chosenRank) {
     mine.v.s = warp_add(mine.v.s);
     mine.v.t = warp_add(mine.v.t);
     if (RACE) {
 #pragma unroll 1
         for (int d = 16; d; d >>= 1) {
-            Runner o;
-            o.key = __shfl_xor_sync(0xffffffffu, mine.best.key, d);
-            o.logit = __shfl_xor_sync(0xffffffffu, mine.best.logit, d);
-            o.bits = __shfl_xor_sync(0xffffffffu, mine.best.bits, d);
-            o.action = __shfl_xor_sync(0xffffffffu, mine.best.action, d);
+            const Runner o = runner_xor(mine.best, d);
             if (beats<GREEDY>(o, mine.best)) mine.best = o;
         }
     }
     if (NT == 32) return;
-    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = mine;
-    __syncthreads();
-    auto join = [&](RowPart& all, const RowPart& o) {
-        all.v.merge(o.v);
-        if (RACE && beats<GREEDY>(o.best, all.best)) all.best = o.best;
-    };
-    if (threadIdx.x == 0) {
-        RowPart all = warps[0];
-#pragma unroll 1
-        for (int w = 1; w < kTeamWarps<NT>; w++) join(all, warps[w]);
-        *whole = all;
-    }
-    if (parts == 1) {
+    // a lane for each warp of the row's CTAs
+    constexpr int W = kTeamWarps<NT>;
+    static_assert(NT == 32 || W == 8, "eight warps a CTA: up to two slots a lane");
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) warps[threadIdx.x >> 5] = mine;
+    if (parts == 1)
         __syncthreads();
-        mine = *whole;
-        return;
+    else
+        cluster_sync();
+    Softmax v[2];
+    Runner best;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int slot = lane + 32 * k;
+        if (slot < parts * W) {
+            const RowPart* o = parts == 1 ? warps + slot : cluster_peer(warps, slot / W) + slot % W;
+            v[k] = o->v;
+            if (RACE && beats<GREEDY>(o->best, best)) best = o->best;
+        }
     }
-    cluster_sync();
-    RowPart all = *cluster_peer(whole, 0);
+    const float m = warp_max(fmaxf(v[0].m, v[1].m));
+    float s = 0.0f, t = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const float d = v[k].m > -INFINITY ? v[k].m - m : 0.0f, f = exp2_fast(d);
+        s += v[k].s * f;
+        if (f > 0.0f) t += f * (v[k].t + v[k].s * d);
+    }
+    mine.v.m = m;
+    mine.v.s = warp_add(s);
+    mine.v.t = warp_add(t);
+    if (RACE) {
 #pragma unroll 1
-    for (int k = 1; k < parts; k++) join(all, *cluster_peer(whole, k));
-    if (!RACE) all.chosen = cluster_peer(whole, chosenRank)->chosen;
-    mine = all;
+        for (int d = 16; d; d >>= 1) {
+            const Runner o = runner_xor(best, d);
+            if (beats<GREEDY>(o, best)) best = o;
+        }
+        mine.best = best;
+    } else if (parts > 1) {
+        mine.chosen = cluster_peer(warps, chosenRank)->chosen;
+    }
 }
 
 // Passes the team's part of a row, controlled but without the actions that
@@ -404,16 +419,15 @@ __device__ __forceinline__ void row_walk(const T* x, const RowControls& r, const
 // as 2^23 + k against 2^23 + 2^16 times that bound (1e-4 more than it, so that
 // rounding never hides a winner); only the few that pass take logarithms.
 template <class T, int NT, bool GREEDY>
-__global__ void __launch_bounds__(kCtaThreads<NT>)
+__global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
     k_logits_sample(const T* logits, int64_t ld, const mg_logit_controls c, uint32_t* rng, int32_t* action,
                     float* logProb, float* entropy, float* value, const TeamPart part) {
     mg_pdl_trigger();
     mg_pdl_wait();
     extern __shared__ uint32_t smem[];
     __shared__ uint32_t sums[kTeamWarps<NT>];
-    __shared__ __align__(8) unsigned char slots[(kTeamWarps<NT> + 1) * sizeof(RowPart)];
+    __shared__ __align__(8) unsigned char slots[kTeamWarps<NT> * sizeof(RowPart)];
     RowPart* warps = reinterpret_cast<RowPart*>(slots);
-    RowPart* whole = warps + kTeamWarps<NT>;
     int row, lo, hi;
     if (!team_part<NT>(part, row, lo, hi)) return;
     const RowControls r = row_controls(c, row);
@@ -464,6 +478,16 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
             if (f <= fmaf(limit, e, 8388608.0f)) pass |= 1u << i;
         });
         // the lanes' candidates, one a lane at a time, each against the bound that the ones before it left
+        auto still = [&](uint32_t bits) {  // those of them that pass under the bound as it is now
+            uint32_t out = 0;
+            const float now = fminf(bound * 65542.6f, 3e38f);
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const float f = (float)(race_bits(word, at(i)) >> 16), e = exp2_fast(log2_weight(l[i], mine.v.m));
+                if (f <= now * e) out |= 1u << i;
+            }
+            return out & bits;
+        };
         while (some && __any_sync(0xffffffffu, pass != 0)) {
             float ratio = 3e38f;
             if (pass) {
@@ -475,11 +499,12 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
                 const uint32_t h = race_bits(word, at(i));
                 const float e = exp2_fast(log2_weight(li, mine.v.m));
                 if (li > -INFINITY && (float)(h >> 16) <= bound * 65542.6f * e) {
-                    // -log(1 - v) from whichever of v and 1 - v is small
-                    const float time = h < 0x80000000u ? -log1pf(-((float)h + 0.5f) * 2.3283064e-10f)
-                                                       : -logf(((float)(~h) + 0.5f) * 2.3283064e-10f);
+                    // -log(1 - v): its series below 1 / 64 (the next term is 4e-6 of it), else from 1 - v
+                    const float u = ((float)h + 0.5f) * 2.3283064e-10f;
+                    const float time = u < 0.015625f ? u * fmaf(u, fmaf(u, 0.33333333f, 0.5f), 1.0f)
+                                                     : -kLn2 * log2_fast(((float)(~h) + 0.5f) * 2.3283064e-10f);
                     Runner o;
-                    o.key = li - logf(time);
+                    o.key = fmaf(-kLn2, log2_fast(time), li);
                     o.logit = li;
                     o.bits = h;
                     o.action = at(i);
@@ -490,7 +515,8 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
             const float least = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(ratio)));
             if (least < bound) {
                 bound = least;
-                if (NT > 32 && (threadIdx.x & 31) == 0) atomicMin(&sharedBound, float_order(log2f(least) - mine.v.m));
+                if (NT > 32 && (threadIdx.x & 31) == 0) atomicMin(&sharedBound, float_order(log2_fast(least) - mine.v.m));
+                if (N > 4 && __any_sync(0xffffffffu, (pass & (pass - 1)) != 0)) pass = still(pass);
             }
         }
     };
@@ -502,7 +528,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
             take(&l, [&](int) { return a; }, std::integral_constant<int, 1>());
         }
     }
-    row_merge<NT, true, GREEDY>(mine, warps, whole, part.parts, 0);
+    row_merge<NT, true, GREEDY>(mine, warps, part.parts, 0);
     if (tid == 0 && lo == 0) {
         const float ls = log2f(mine.v.s);
         const bool some = mine.best.action >= 0 || mine.v.s != mine.v.s;
@@ -528,7 +554,7 @@ struct LossArgs {
 // The row's statistics in one pass, its gradient in a second one that reads the
 // row again, from L2.
 template <class T, int NT>
-__global__ void __launch_bounds__(kCtaThreads<NT>)
+__global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
     k_logits_loss(const T* logits, int64_t ld, const mg_logit_controls c, T* dLogits, int64_t ldd, const TeamPart part,
                   const LossArgs L) {
     constexpr int VE = kGroup<T>;
@@ -536,9 +562,8 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
     mg_pdl_wait();
     extern __shared__ uint32_t smem[];
     __shared__ uint32_t sums[kTeamWarps<NT>];
-    __shared__ __align__(8) unsigned char slots[(kTeamWarps<NT> + 1) * sizeof(RowPart)];
+    __shared__ __align__(8) unsigned char slots[kTeamWarps<NT> * sizeof(RowPart)];
     RowPart* warps = reinterpret_cast<RowPart*>(slots);
-    RowPart* whole = warps + kTeamWarps<NT>;
     int row, lo, hi;
     if (!team_part<NT>(part, row, lo, hi)) return;
     const int actions = part.actions, tid = team_rank<NT>();
@@ -547,6 +572,10 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
     const T* x = logits + (int64_t)row * ld;
     T* d = dLogits + (int64_t)row * ldd;
     const int act = L.action[row];
+    // the row's other inputs in flight with its action
+    const float old = L.oldLogProb[row], advRaw = L.adv[row], ret = L.ret ? L.ret[row] : 0.0f;
+    const float adv0 = L.advStats ? L.advStats[0] : 0.0f, adv1 = L.advStats ? L.advStats[1] : 1.0f;
+    const float valueX = L.ret && lo == 0 ? to_f32(x[actions]) : 0.0f;
     const bool inside = act >= 0 && act < actions;
     if (!inside || !allowed(r, act)) {  // the same for every CTA of the row
         if (tid == 0 && lo == 0 && !inside && act != -1) record_error(L.status, kDevBadAction);
@@ -578,11 +607,11 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
             take(&l, 0, std::integral_constant<int, 1>());
         }
     }
-    row_merge<NT, false, false>(mine, warps, whole, part.parts, act / part.span);
+    row_merge<NT, false, false>(mine, warps, part.parts, act / part.span);
     const float m = mine.v.m, ls = log2f(mine.v.s), entropy = (ls - mine.v.t / mine.v.s) * kLn2;
-    const float logp = (log2_weight(mine.chosen, m) - ls) * kLn2, old = L.oldLogProb[row];
+    const float logp = (log2_weight(mine.chosen, m) - ls) * kLn2;
     const float ratio = expf(logp - old);
-    const float adv = L.advStats ? (L.adv[row] - L.advStats[0]) * L.advStats[1] : L.adv[row];
+    const float adv = L.advStats ? (advRaw - adv0) * adv1 : advRaw;
     const float one = ratio * adv, two = fminf(fmaxf(ratio, 1.0f - L.clip), 1.0f + L.clip) * adv;
     const float slope = one <= two ? -adv * ratio : 0.0f;
     // every thread has read the action's logit: the gradient may take its place
@@ -654,7 +683,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>)
         float* st = L.stats + (int64_t)row * 5;
         float vLoss = 0.0f;
         if (L.ret) {
-            const float err = to_f32(x[actions]) - L.ret[row];
+            const float err = valueX - ret;
             vLoss = 0.5f * L.valueCoef * err * err;
             from_f32(&d[actions], L.valueCoef * err * L.scale);
         }
