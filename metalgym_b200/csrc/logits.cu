@@ -79,7 +79,7 @@ constexpr int kUnit = 2048;
 constexpr int kControlGroups = 4;  // 16-byte loads of a thread in flight
 constexpr int kControlCtas = 5;    // CTAs an SM holds
 
-template <class T, int NT, bool BACKWARD>
+template <class T, int NT, bool BACKWARD, int WITH>
 __device__ __forceinline__ void control_part(const T* x, const T* src, T* y, const RowControls& r, HistoryTable& t,
                                              const mg_logit_controls& c, int row, int lo, int hi, uint32_t* sums) {
     constexpr int VE = kGroup<T>, U = kControlGroups;
@@ -110,9 +110,9 @@ __device__ __forceinline__ void control_part(const T* x, const T* src, T* y, con
             const int a = s.body + (g0 + u * NT) * VE;
             float v[VE];
             group_floats(raw[u], src, v);
-            if (!BACKWARD) {
-                group_bias_mask<VE>(r, a, 0u, v);
-            } else if (r.mask) {
+            if constexpr (!BACKWARD) {
+                group_bias_mask<WITH, VE>(r, a, 0u, v);
+            } else if ((WITH & kWithMask) && r.mask) {
                 const uint32_t ok = bit_window<VE>(r.mask, a);
 #pragma unroll
                 for (int i = 0; i < VE; i++) v[i] = (ok & (1u << i)) ? v[i] : 0.0f;
@@ -134,7 +134,7 @@ __device__ __forceinline__ void control_part(const T* x, const T* src, T* y, con
     }
 }
 
-template <class T, int NT, bool BACKWARD>
+template <class T, int NT, bool BACKWARD, int WITH>
 __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : kControlCtas)
     k_logits_control(const T* logits, int64_t ld, const mg_logit_controls c, const T* dOut, int64_t ldg, T* out,
                      int64_t ldo, const TeamPart part) {
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : kControlCtas)
     HistoryTable t = team_table<NT>(part, c, smem);
     auto run = [&](int row, int lo, int hi) {
         const T* x = logits + (int64_t)row * ld;
-        control_part<T, NT, BACKWARD>(x, BACKWARD ? dOut + (int64_t)row * ldg : x, out + (int64_t)row * ldo, row_controls(c, row),
+        control_part<T, NT, BACKWARD, WITH>(x, BACKWARD ? dOut + (int64_t)row * ldg : x, out + (int64_t)row * ldo, row_controls(c, row),
                                       t, c, row, lo, hi, sums);
     };
     if (NT == 32) {
@@ -366,32 +366,27 @@ __device__ inline void row_merge(RowPart& mine, RowPart* warps, int parts, int c
 
 // Passes the team's part of a row, controlled but without the actions that
 // occurred, to take(l, at, count): whole warps, 16 logits a lane while there
-// are as many, then a group a lane, then the edges.
-template <class T, int NT, class Take>
+// are as many, then a group a lane, then the edges. (The next loads are left to
+// the other warps: holding them in registers cost 7 % more than it hid.)
+template <class T, int NT, int WITH, class Take>
 __device__ __forceinline__ void row_walk(const T* x, const RowControls& r, const HistoryTable& t, const RowSpan& s, int lo,
                                          Take take) {
     constexpr int VE = kGroup<T>, U = 16 / VE;
     const int tid = team_rank<NT>();
     auto control = [&](const uint4& raw, int a, float* l) {
         group_floats(raw, x, l);
-        group_bias_mask<VE>(r, a, r.history ? bit_window<VE>(t.seen, a - lo) : 0u, l);
+        group_bias_mask<WITH, VE>(r, a, r.history ? bit_window<VE>(t.seen, a - lo) : 0u, l);
     };
     int g0 = 0;
-    if (s.groups >= NT * U) {
+    for (; g0 + NT * U <= s.groups; g0 += NT * U) {
+        const int a = s.body + (g0 + tid) * VE;
         uint4 raw[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) raw[u] = group_load(x + s.body + (u * NT + tid) * VE);
-        for (; g0 + NT * U <= s.groups; g0 += NT * U) {
-            const int a = s.body + (g0 + tid) * VE;
-            float l[16];
+        for (int u = 0; u < U; u++) raw[u] = group_load(x + a + u * NT * VE);
+        float l[16];
 #pragma unroll
-            for (int u = 0; u < U; u++) control(raw[u], a + u * NT * VE, l + u * VE);
-            if (g0 + 2 * NT * U <= s.groups) {  // the next loads while these logits are worked on
-#pragma unroll
-                for (int u = 0; u < U; u++) raw[u] = group_load(x + a + (NT * U + u * NT) * VE);
-            }
-            take(l, [&](int i) { return a + (i / VE) * (NT * VE) + i % VE; }, std::integral_constant<int, 16>());
-        }
+        for (int u = 0; u < U; u++) control(raw[u], a + u * NT * VE, l + u * VE);
+        take(l, [&](int i) { return a + (i / VE) * (NT * VE) + i % VE; }, std::integral_constant<int, 16>());
     }
     for (; g0 < s.groups; g0 += NT) {
         const int g = g0 + tid, a = s.body + g * VE;
@@ -418,7 +413,7 @@ __device__ __forceinline__ void row_walk(const T* x, const RowControls& r, const
 // takes the upper 16 bits of h, which the last step of mg_mix32 leaves alone,
 // as 2^23 + k against 2^23 + 2^16 times that bound (1e-4 more than it, so that
 // rounding never hides a winner); only the few that pass take logarithms.
-template <class T, int NT, bool GREEDY>
+template <class T, int NT, bool GREEDY, int WITH>
 __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
     k_logits_sample(const T* logits, int64_t ld, const mg_logit_controls c, uint32_t* rng, int32_t* action,
                     float* logProb, float* entropy, float* value, const TeamPart part) {
@@ -520,7 +515,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
             }
         }
     };
-    row_walk<T, NT>(x, r, t, s, lo, take);
+    row_walk<T, NT, WITH>(x, r, t, s, lo, take);
     if (r.history) {
         for (int j0 = 0, n = t.total(); j0 < n; j0 += NT) {
             const int j = j0 + tid, a = j < n ? (int)t.list[j] : 0;
@@ -553,7 +548,7 @@ struct LossArgs {
 
 // The row's statistics in one pass, its gradient in a second one that reads the
 // row again, from L2.
-template <class T, int NT>
+template <class T, int NT, int WITH>
 __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
     k_logits_loss(const T* logits, int64_t ld, const mg_logit_controls c, T* dLogits, int64_t ldd, const TeamPart part,
                   const LossArgs L) {
@@ -592,7 +587,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
     auto take = [&](const float* l, auto, auto count) {
         softmax_group<decltype(count)::value>(mine.v, l, [](float) {}, [](int, float) {});
     };
-    row_walk<T, NT>(x, r, t, s, lo, take);
+    row_walk<T, NT, WITH>(x, r, t, s, lo, take);
     if (r.history) {
         for (int j0 = 0, n = t.total(); j0 < n; j0 += NT) {
             const int j = j0 + tid;
@@ -641,7 +636,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
             const int a = s.body + (g0 + u * NT) * VE;
             float l[VE];
             group_floats(raw[u], x, l);
-            group_bias_mask<VE>(r, a, 0u, l);
+            group_bias_mask<WITH, VE>(r, a, 0u, l);
             const float2 k2 = make_float2(kLog2e, kLog2e), m2 = make_float2(-m, -m), ls2 = make_float2(-ls, -ls);
             const float2 s12 = make_float2(s1, s1), sh2 = make_float2(sh, sh);
 #pragma unroll
@@ -659,7 +654,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
 #pragma unroll
                 for (int i = 0; i < VE; i++) l[i] = a + i == act ? l[i] + s0 : l[i];
             }
-            if (r.mask && all_nan) {  // a NaN somewhere in the row: still 0 where the mask says so
+            if ((WITH & kWithMask) && r.mask && all_nan) {  // a NaN somewhere in the row: still 0 where the mask says so
                 const uint32_t ok = bit_window<VE>(r.mask, a);
 #pragma unroll
                 for (int i = 0; i < VE; i++) l[i] = (ok & (1u << i)) ? l[i] : 0.0f;
@@ -789,10 +784,16 @@ int row_parts(int rows, int actions, int size, int nt, bool twice) {
     return parts;
 }
 
-template <class T, int NT, bool BACKWARD>
+// The compiled controls that a call needs; `history`: the pass leaves out the
+// actions that occurred. Small action sets take the kernel with all of them.
+int needed_controls(const mg_logit_controls& c, bool history) {
+    return (c.bias ? kWithBias : 0) | (c.mask || (history && c.history) ? kWithMask : 0);
+}
+
+template <class T, int NT, bool BACKWARD, int WITH>
 int launch_control(const void* logits, int64_t ld, const mg_logit_controls& c, const void* dOut, int64_t ldg, void* out,
                    int64_t ldo, int rows, int actions, cudaStream_t st) {
-    auto kern = k_logits_control<T, NT, BACKWARD>;
+    auto kern = k_logits_control<T, NT, BACKWARD, WITH>;
     static std::atomic<uint64_t> done{0};
     MG_TRY(smem_limit_once(kern, kTableSmemMax, done));
     TeamPart p = plan(NT, rows, actions, 1, c.history_max);
@@ -812,15 +813,23 @@ int launch_control(const void* logits, int64_t ld, const mg_logit_controls& c, c
 template <class T, bool BACKWARD>
 int control(const void* logits, int64_t ld, const mg_logit_controls& c, const void* dOut, int64_t ldg, void* out, int64_t ldo,
             int rows, int actions, cudaStream_t st) {
-    return actions <= kWarpActions
-               ? launch_control<T, 32, BACKWARD>(logits, ld, c, dOut, ldg, out, ldo, rows, actions, st)
-               : launch_control<T, 256, BACKWARD>(logits, ld, c, dOut, ldg, out, ldo, rows, actions, st);
+    auto f = launch_control<T, 32, BACKWARD, BACKWARD ? kWithMask : kWithBias | kWithMask>;
+    if (actions > kWarpActions) {
+        switch (needed_controls(c, false)) {
+            case 0: f = launch_control<T, 256, BACKWARD, 0>; break;
+            case kWithMask: f = launch_control<T, 256, BACKWARD, kWithMask>; break;
+            default:  // (no bias in a gradient)
+                if constexpr (!BACKWARD)
+                    f = c.mask ? launch_control<T, 256, false, kWithBias | kWithMask> : launch_control<T, 256, false, kWithBias>;
+        }
+    }
+    return f(logits, ld, c, dOut, ldg, out, ldo, rows, actions, st);
 }
 
-template <class T, int NT, bool GREEDY>
+template <class T, int NT, bool GREEDY, int WITH>
 int launch_sample(const void* logits, int64_t ld, const mg_logit_controls& c, uint32_t* rng, int32_t* action, float* logProb,
                   float* entropy, float* value, int rows, int actions, cudaStream_t st) {
-    auto kern = k_logits_sample<T, NT, GREEDY>;
+    auto kern = k_logits_sample<T, NT, GREEDY, WITH>;
     static std::atomic<uint64_t> done{0};
     MG_TRY(smem_limit_once(kern, kTableSmemMax, done));
     const TeamPart p = plan(NT, rows, actions, NT == 32 ? 1 : row_parts(rows, actions, sizeof(T), NT, false), c.history_max);
@@ -828,21 +837,32 @@ int launch_sample(const void* logits, int64_t ld, const mg_logit_controls& c, ui
                            value, p);
 }
 
+template <class T, bool GREEDY>
+int sample_rows(const void* logits, int64_t ld, const mg_logit_controls& c, uint32_t* rng, int32_t* action, float* logProb,
+                float* entropy, float* value, int rows, int actions, cudaStream_t st) {
+    auto f = launch_sample<T, 32, GREEDY, 3>;
+    if (actions > kWarpActions) {
+        switch (needed_controls(c, true)) {
+            case 0: f = launch_sample<T, 256, GREEDY, 0>; break;
+            case 1: f = launch_sample<T, 256, GREEDY, 1>; break;
+            case 2: f = launch_sample<T, 256, GREEDY, 2>; break;
+            default: f = launch_sample<T, 256, GREEDY, 3>;
+        }
+    }
+    return f(logits, ld, c, rng, action, logProb, entropy, value, rows, actions, st);
+}
+
 template <class T>
 int sample(const void* logits, int64_t ld, const mg_logit_controls& c, uint32_t* rng, int32_t* action, float* logProb,
            float* entropy, float* value, int rows, int actions, cudaStream_t st) {
-    const bool warp = actions <= kWarpActions;
-    if (rng)
-        return warp ? launch_sample<T, 32, false>(logits, ld, c, rng, action, logProb, entropy, value, rows, actions, st)
-                    : launch_sample<T, 256, false>(logits, ld, c, rng, action, logProb, entropy, value, rows, actions, st);
-    return warp ? launch_sample<T, 32, true>(logits, ld, c, rng, action, logProb, entropy, value, rows, actions, st)
-                : launch_sample<T, 256, true>(logits, ld, c, rng, action, logProb, entropy, value, rows, actions, st);
+    return rng ? sample_rows<T, false>(logits, ld, c, rng, action, logProb, entropy, value, rows, actions, st)
+               : sample_rows<T, true>(logits, ld, c, rng, action, logProb, entropy, value, rows, actions, st);
 }
 
-template <class T, int NT>
+template <class T, int NT, int WITH>
 int launch_loss(const void* logits, int64_t ld, const mg_logit_controls& c, void* d, int64_t ldd, int rows, int actions,
                 const LossArgs& L, cudaStream_t st) {
-    auto kern = k_logits_loss<T, NT>;
+    auto kern = k_logits_loss<T, NT, WITH>;
     static std::atomic<uint64_t> done{0};
     MG_TRY(smem_limit_once(kern, kTableSmemMax, done));
     const TeamPart p = plan(NT, rows, actions, NT == 32 ? 1 : row_parts(rows, actions, sizeof(T), NT, true), c.history_max);
@@ -852,8 +872,16 @@ int launch_loss(const void* logits, int64_t ld, const mg_logit_controls& c, void
 template <class T>
 int loss(const void* logits, int64_t ld, const mg_logit_controls& c, void* d, int64_t ldd, int rows, int actions,
          const LossArgs& L, cudaStream_t st) {
-    return actions <= kWarpActions ? launch_loss<T, 32>(logits, ld, c, d, ldd, rows, actions, L, st)
-                                   : launch_loss<T, 256>(logits, ld, c, d, ldd, rows, actions, L, st);
+    auto f = launch_loss<T, 32, 3>;
+    if (actions > kWarpActions) {
+        switch (needed_controls(c, true)) {
+            case 0: f = launch_loss<T, 256, 0>; break;
+            case 1: f = launch_loss<T, 256, 1>; break;
+            case 2: f = launch_loss<T, 256, 2>; break;
+            default: f = launch_loss<T, 256, 3>;
+        }
+    }
+    return f(logits, ld, c, d, ldd, rows, actions, L, st);
 }
 
 }  // namespace
