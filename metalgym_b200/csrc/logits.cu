@@ -82,7 +82,7 @@ constexpr int kControlCtas = 5;    // CTAs an SM holds
 template <class T, int NT, bool BACKWARD, int WITH>
 __device__ __forceinline__ void control_part(const T* x, const T* src, T* y, const RowControls& r, HistoryTable& t,
                                              const mg_logit_controls& c, int row, int lo, int hi, uint32_t* sums) {
-    constexpr int VE = kGroup<T>, U = kControlGroups;
+    constexpr int VE = kGroup, U = kControlGroups * 16 / (VE * (int)sizeof(T));
     const int tid = team_rank<NT>();
     const bool vec = same_alignment(src, y);
     const RowSpan s = row_span(src, lo, hi);
@@ -100,7 +100,7 @@ __device__ __forceinline__ void control_part(const T* x, const T* src, T* y, con
         team_sync<NT>();
     }
     for (int g0 = tid; g0 < s.groups; g0 += NT * U) {
-        uint4 raw[U];
+        RawGroup<T> raw[U];
 #pragma unroll
         for (int u = 0; u < U; u++)
             if (g0 + u * NT < s.groups) raw[u] = group_load(src + s.body + (g0 + u * NT) * VE);
@@ -109,19 +109,19 @@ __device__ __forceinline__ void control_part(const T* x, const T* src, T* y, con
             if (g0 + u * NT >= s.groups) break;
             const int a = s.body + (g0 + u * NT) * VE;
             float v[VE];
-            group_floats(raw[u], src, v);
+            group_floats(raw[u], v);
             if constexpr (!BACKWARD) {
-                group_bias_mask<WITH, VE>(r, a, 0u, v);
+                group_bias_mask<WITH>(r, a, 0u, v);
             } else if ((WITH & kWithMask) && r.mask) {
-                const uint32_t ok = bit_window<VE>(r.mask, a);
+                const uint32_t ok = bit_window(r.mask, a);
 #pragma unroll
                 for (int i = 0; i < VE; i++) v[i] = (ok & (1u << i)) ? v[i] : 0.0f;
             }
-            group_store(y + a, vec, group_pack(v, src));
+            group_store(y + a, vec, v);
         }
     }
     if (s.edges() && tid < 32) {
-        const int a = s.edge<VE>(tid);
+        const int a = s.edge(tid);
         if (a >= 0) {
             const float raw = to_f32(src[a]);
             from_f32(&y[a], !BACKWARD ? bias_mask(r, raw, a) : allowed(r, a) ? raw : 0.0f);
@@ -371,16 +371,16 @@ __device__ inline void row_merge(RowPart& mine, RowPart* warps, int parts, int c
 template <class T, int NT, int WITH, class Take>
 __device__ __forceinline__ void row_walk(const T* x, const RowControls& r, const HistoryTable& t, const RowSpan& s, int lo,
                                          Take take) {
-    constexpr int VE = kGroup<T>, U = 16 / VE;
+    constexpr int VE = kGroup, U = 16 / VE;
     const int tid = team_rank<NT>();
-    auto control = [&](const uint4& raw, int a, float* l) {
-        group_floats(raw, x, l);
-        group_bias_mask<WITH, VE>(r, a, r.history ? bit_window<VE>(t.seen, a - lo) : 0u, l);
+    auto control = [&](const RawGroup<T>& raw, int a, float* l) {
+        group_floats(raw, l);
+        group_bias_mask<WITH>(r, a, r.history ? bit_window(t.seen, a - lo) : 0u, l);
     };
     int g0 = 0;
     for (; g0 + NT * U <= s.groups; g0 += NT * U) {
         const int a = s.body + (g0 + tid) * VE;
-        uint4 raw[U];
+        RawGroup<T> raw[U];
 #pragma unroll
         for (int u = 0; u < U; u++) raw[u] = group_load(x + a + u * NT * VE);
         float l[16];
@@ -400,7 +400,7 @@ __device__ __forceinline__ void row_walk(const T* x, const RowControls& r, const
         take(l, [&](int i) { return a + i; }, std::integral_constant<int, VE>());
     }
     if (s.edges() && tid < 32) {
-        const int a = s.edge<VE>(tid);
+        const int a = s.edge(tid);
         const float l = a < 0 || (r.history && t.has(a - lo)) ? -INFINITY : bias_mask(r, to_f32(x[a]), a);
         take(&l, [&](int) { return a; }, std::integral_constant<int, 1>());
     }
@@ -552,7 +552,7 @@ template <class T, int NT, int WITH>
 __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
     k_logits_loss(const T* logits, int64_t ld, const mg_logit_controls c, T* dLogits, int64_t ldd, const TeamPart part,
                   const LossArgs L) {
-    constexpr int VE = kGroup<T>;
+    constexpr int VE = kGroup;
     mg_pdl_trigger();
     mg_pdl_wait();
     extern __shared__ uint32_t smem[];
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
     };
     constexpr int U = 2;
     for (int g0 = tid; g0 < s.groups; g0 += NT * U) {
-        uint4 raw[U];
+        RawGroup<T> raw[U];
 #pragma unroll
         for (int u = 0; u < U; u++)
             if (g0 + u * NT < s.groups) raw[u] = group_load(x + s.body + (g0 + u * NT) * VE);
@@ -635,8 +635,8 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
             if (g0 + u * NT >= s.groups) break;
             const int a = s.body + (g0 + u * NT) * VE;
             float l[VE];
-            group_floats(raw[u], x, l);
-            group_bias_mask<WITH, VE>(r, a, 0u, l);
+            group_floats(raw[u], l);
+            group_bias_mask<WITH>(r, a, 0u, l);
             const float2 k2 = make_float2(kLog2e, kLog2e), m2 = make_float2(-m, -m), ls2 = make_float2(-ls, -ls);
             const float2 s12 = make_float2(s1, s1), sh2 = make_float2(sh, sh);
 #pragma unroll
@@ -655,15 +655,15 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
                 for (int i = 0; i < VE; i++) l[i] = a + i == act ? l[i] + s0 : l[i];
             }
             if ((WITH & kWithMask) && r.mask && all_nan) {  // a NaN somewhere in the row: still 0 where the mask says so
-                const uint32_t ok = bit_window<VE>(r.mask, a);
+                const uint32_t ok = bit_window(r.mask, a);
 #pragma unroll
                 for (int i = 0; i < VE; i++) l[i] = (ok & (1u << i)) ? l[i] : 0.0f;
             }
-            group_store(d + a, vec, group_pack(l, x));
+            group_store(d + a, vec, l);
         }
     }
     if (s.edges() && tid < 32) {
-        const int a = s.edge<VE>(tid);
+        const int a = s.edge(tid);
         if (a >= 0) from_f32(&d[a], allowed(r, a) ? gradient(bias_mask(r, to_f32(x[a]), a), a) : 0.0f);
     }
     if (r.history) {  // the actions that occurred, over what the pass wrote for them
@@ -774,13 +774,14 @@ int launch_rows(void (*kern)(KArgs...), const TeamPart& p, cudaStream_t st, cons
 
 // Parts of a row for the calls that need the whole row's statistics: more
 // while the CTAs do not fill the GPU (and a part keeps 4096 actions), and, for
-// the loss, so many that the rows in flight stay in half of L2.
+// the loss, so many that the rows in flight stay in L2 for its second pass (1000 x 50001
+// fp32: 220 us at four parts, 188 at two, 228 at one, whose rows are 118 MB).
 int row_parts(int rows, int actions, int size, int nt, bool twice) {
     int parts = 1;
     const int fill = 4 * num_sms();
     while (parts < 8 && (int64_t)rows * parts < fill && actions / (2 * parts) >= 4096) parts *= 2;
     if (twice)
-        while (parts < 8 && (int64_t)num_sms() * (1024 / nt) / parts * actions * size > (48 << 20)) parts *= 2;
+        while (parts < 8 && (int64_t)num_sms() * (1024 / nt) / parts * actions * size > (100 << 20)) parts *= 2;
     return parts;
 }
 

@@ -186,59 +186,68 @@ __device__ __forceinline__ float seen_gradient(const RowControls& r, float g, fl
 }
 
 // ------------------------------------------------------------------ groups
-// A row (or a part [lo, hi) of it) is read in groups of 16 bytes, one vector
-// load each, cut at 16-byte boundaries of memory; the up to kGroup - 1
-// actions before the first boundary and behind the last one, the edges, are
-// done one by one by the first warp of the team.
+// A row (or a part [lo, hi) of it) is read in groups of eight actions, by vector
+// loads, from the first 16-byte boundary of memory on; the up to 7 actions
+// before it and behind the last whole group, the edges, are done one by one by
+// the first warp of the team. (Eight fp32 logits are two loads: four to a
+// group would look up mask, table and bias twice as often.)
+
+constexpr int kGroup = 8;
 
 template <class T>
-constexpr int kGroup = 16 / (int)sizeof(T);
+struct RawGroup {
+    uint4 w[kGroup * sizeof(T) / 16];
+};
 
 struct RowSpan {
     int body, groups;    // first action of group 0, number of groups
     int lo, head, tail;  // actions before the groups, and behind them
     // The action of lane `lane` of the edges, or -1.
-    template <int VE>
     __device__ __forceinline__ int edge(int lane) const {
         if (lane < head) return lo + lane;
-        return lane >= 16 && lane - 16 < tail ? body + groups * VE + lane - 16 : -1;
+        return lane >= 16 && lane - 16 < tail ? body + groups * kGroup + lane - 16 : -1;
     }
     __device__ __forceinline__ bool edges() const { return (head | tail) != 0; }
 };
 
 template <class T>
 __device__ __forceinline__ RowSpan row_span(const T* row, int lo, int hi) {
-    constexpr int VE = kGroup<T>;
     const int past = (int)((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
     RowSpan s;
     s.lo = lo;
-    s.head = min(hi - lo, past ? VE - past : 0);
+    s.head = min(hi - lo, past ? (int)(16 / sizeof(T)) - past : 0);
     s.body = lo + s.head;
-    s.groups = (hi - s.body) / VE;
-    s.tail = hi - s.body - s.groups * VE;
+    s.groups = (hi - s.body) / kGroup;
+    s.tail = hi - s.body - s.groups * kGroup;
     return s;
 }
 
 template <class T>
-__device__ __forceinline__ uint4 group_load(const T* p) {
-    return *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ RawGroup<T> group_load(const T* p) {
+    RawGroup<T> g;
+#pragma unroll
+    for (int i = 0; i < (int)(kGroup * sizeof(T) / 16); i++) g.w[i] = reinterpret_cast<const uint4*>(p)[i];
+    return g;
 }
-__device__ __forceinline__ void group_floats(const uint4& w, const float*, float* x) {
-    x[0] = __uint_as_float(w.x);
-    x[1] = __uint_as_float(w.y);
-    x[2] = __uint_as_float(w.z);
-    x[3] = __uint_as_float(w.w);
+__device__ __forceinline__ void group_floats(const RawGroup<float>& g, float* x) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        x[4 * i] = __uint_as_float(g.w[i].x);
+        x[4 * i + 1] = __uint_as_float(g.w[i].y);
+        x[4 * i + 2] = __uint_as_float(g.w[i].z);
+        x[4 * i + 3] = __uint_as_float(g.w[i].w);
+    }
 }
-__device__ __forceinline__ void group_floats(const uint4& w, const __nv_bfloat16*, float* x) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ void group_floats(const RawGroup<__nv_bfloat16>& g, float* x) {
+    const uint32_t u[4] = {g.w[0].x, g.w[0].y, g.w[0].z, g.w[0].w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         x[2 * i] = __uint_as_float(u[i] << 16);
         x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
 }
-__device__ __forceinline__ void group_floats(const uint4& w, const __half*, float* x) {
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ void group_floats(const RawGroup<__half>& g, float* x) {
+    const uint32_t u[4] = {g.w[0].x, g.w[0].y, g.w[0].z, g.w[0].w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
@@ -246,52 +255,50 @@ __device__ __forceinline__ void group_floats(const uint4& w, const __half*, floa
         x[2 * i + 1] = f.y;
     }
 }
-__device__ __forceinline__ uint4 group_pack(const float* v, const float*) {
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+
+// Writes a full group; `vec`: p is 16-byte aligned.
+__device__ __forceinline__ void group_store(float* p, bool vec, const float* v) {
+    if (vec) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kGroup; i++) p[i] = v[i];
 }
-__device__ __forceinline__ uint4 group_pack(const float* v, const __nv_bfloat16*) {
+__device__ __forceinline__ void group_store16(void* p, bool vec, const uint32_t* u) {
+    if (vec) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kGroup; i++) static_cast<unsigned short*>(p)[i] = (unsigned short)(u[i >> 1] >> ((i & 1) * 16));
+}
+__device__ __forceinline__ void group_store(__nv_bfloat16* p, bool vec, const float* v) {
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
         u[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    return make_uint4(u[0], u[1], u[2], u[3]);
+    group_store16(p, vec, u);
 }
-__device__ __forceinline__ uint4 group_pack(const float* v, const __half*) {
+__device__ __forceinline__ void group_store(__half* p, bool vec, const float* v) {
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
         u[i] = *reinterpret_cast<const uint32_t*>(&h);
     }
-    return make_uint4(u[0], u[1], u[2], u[3]);
+    group_store16(p, vec, u);
 }
 
-// Writes a full group; `vec`: p is 16-byte aligned.
-template <class T>
-__device__ __forceinline__ void group_store(T* p, bool vec, const uint4& w) {
-    if (vec) {
-        *reinterpret_cast<uint4*>(p) = w;
-        return;
-    }
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < kGroup<T>; i++) {
-        if (sizeof(T) == 4)
-            reinterpret_cast<uint32_t*>(p)[i] = u[i & 3];
-        else
-            reinterpret_cast<unsigned short*>(p)[i] = (unsigned short)(u[(i >> 1) & 3] >> ((i & 1) * 16));
-    }
-}
-
-// VE bits of a bit row from bit `at` on (all of them inside the row; those
-// above VE are not cleared).
-template <int VE>
+// The bits of a group in a bit row, from bit `at` on (all of them inside the
+// row; the bits above them are not cleared).
 __device__ __forceinline__ uint32_t bit_window(const uint32_t* words, int at) {
     const int sh = at & 31;
     const uint32_t* w = words + (at >> 5);
-    return __funnelshift_r(w[0], sh + VE > 32 ? w[1] : 0u, sh);
+    return __funnelshift_r(w[0], sh + kGroup > 32 ? w[1] : 0u, sh);
 }
 
 // What a kernel is compiled for: 0 neither bias nor mask, +1 a bias, +2 a mask or
@@ -301,13 +308,13 @@ constexpr int kWithBias = 1, kWithMask = 2;
 
 // Bias and mask of a full group of actions from a on (-inf where the mask says
 // so, and where `skip` has a bit).
-template <int WITH, int VE>
+template <int WITH>
 __device__ __forceinline__ void group_bias_mask(const RowControls& r, int a, uint32_t skip, float* x) {
     if (((WITH & kWithBias) != 0) && r.bias) {
         const float* b = r.bias + a;
         if ((reinterpret_cast<uintptr_t>(b) & 15) == 0) {
 #pragma unroll
-            for (int i = 0; i < VE; i += 4) {
+            for (int i = 0; i < kGroup; i += 4) {
                 const float4 q = *reinterpret_cast<const float4*>(b + i);
                 x[i] = __fadd_rn(x[i], q.x);
                 x[i + 1] = __fadd_rn(x[i + 1], q.y);
@@ -316,13 +323,13 @@ __device__ __forceinline__ void group_bias_mask(const RowControls& r, int a, uin
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < VE; i++) x[i] = __fadd_rn(x[i], b[i]);
+            for (int i = 0; i < kGroup; i++) x[i] = __fadd_rn(x[i], b[i]);
         }
     }
     if constexpr ((WITH & kWithMask) != 0) {
-        const uint32_t out = r.mask ? skip | ~bit_window<VE>(r.mask, a) : skip;
+        const uint32_t out = r.mask ? skip | ~bit_window(r.mask, a) : skip;
 #pragma unroll
-        for (int i = 0; i < VE; i++) x[i] = (out & (1u << i)) ? -INFINITY : x[i];
+        for (int i = 0; i < kGroup; i++) x[i] = (out & (1u << i)) ? -INFINITY : x[i];
     }
 }
 
