@@ -162,10 +162,43 @@ int launch_tiled(const CUtensorMap& ta, const CUtensorMap& tb, NsProduct p, cuda
     return check_launch("k_ns_product");
 }
 
+template <int KIND, bool A_MN, bool B_MN>
+int launch_split(const CUtensorMap& ta, const CUtensorMap& tb, NsProduct p, int splits, cudaStream_t st) {
+    using S = NsTile<128>;
+    auto kern = k_ns_split<KIND, A_MN, B_MN>;
+    static std::atomic<uint64_t> done{0};
+    MG_TRY(smem_limit_once(kern, S::SMEM_BYTES, done));
+    p.tilesM = (p.M + 127) / 128;
+    p.tilesN = (p.N + 127) / 128;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(ns_tiles<KIND, 128>(p.tilesM, p.tilesN) * p.batch * splits));
+    cfg.blockDim = dim3(S::THREADS);
+    cfg.dynamicSmemBytes = S::SMEM_BYTES;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = splits;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    MG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, ta, tb, p, splits));
+    return check_launch("k_ns_split");
+}
+
 // 256-wide tiles where they fill the GPU: half the operand bytes per product
-// of 128-wide ones, which below a wave leave too many SMs idle.
+// of 128-wide ones, which below a wave leave too many SMs idle. Symmetric
+// products of few tiles split a long K over a cluster.
 template <int KIND, bool A_MN, bool B_MN>
 int launch_product(const CUtensorMap& ta, const CUtensorMap& tb, const NsProduct& p, cudaStream_t st) {
+    if constexpr (KIND != kNsApply) {
+        const int64_t tiles = (int64_t)ns_tiles<KIND, 128>((p.M + 127) / 128, (p.N + 127) / 128) * p.batch;
+        int splits = 1;
+        while (splits < 4 && tiles * splits * 2 <= num_sms() && (p.K + 63) / 64 >= 4 * splits) splits *= 2;
+        if (splits > 1) return launch_split<KIND, A_MN, B_MN>(ta, tb, p, splits, st);
+    }
     const int64_t tiles = (int64_t)ns_tiles<KIND, 256>((p.M + 127) / 128, (p.N + 255) / 256) * p.batch;
     return tiles >= num_sms() ? launch_tiled<KIND, 256, A_MN, B_MN>(ta, tb, p, st)
                               : launch_tiled<KIND, 128, A_MN, B_MN>(ta, tb, p, st);

@@ -421,4 +421,169 @@ __global__ void __launch_bounds__(NsTile<BN>::THREADS, 1)
     }
 }
 
+// G or B of few tiles with K split over the CTAs of a cluster, one 128 x 128
+// tile per cluster: a tile's operands come at about 55 bytes a cycle and SM
+// from L2, 590 cycles for a K block whose products take 256, so that few tiles
+// with a long K leave most of that rate unused. Every CTA leaves its part of
+// the sum in the slabs; CTA r then adds the parts of rows 32 r / splits .. of
+// each piece, in their order, and writes them.
+template <int KIND, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(NsTile<128>::THREADS, 1)
+    k_ns_split(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const NsProduct p, int splits) {
+    using S = NsTile<128>;
+    static_assert(KIND != kNsApply, "symmetric products");
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::BAR_OFF);
+    uint64_t* empty = full + S::STAGES;
+    uint64_t* done = empty + S::STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    mg_pdl_trigger();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x % splits, unit = blockIdx.x / splits;
+    const int perMatrix = ns_tiles<KIND, 128>(p.tilesM, p.tilesN), b = unit / perMatrix;
+    int ti, tj;
+    ns_tile_at<KIND, 128>(unit - b * perMatrix, p.tilesN, ti, tj);
+    const int m0 = ti * 128, n0 = tj * 128;
+    const int blocks = (p.K + S::BK - 1) / S::BK;
+    const int kFirst = (int)((int64_t)blocks * rank / splits), kEnd = (int)((int64_t)blocks * (rank + 1) / splits);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::STAGES; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(done, 1);
+        fence_barrier_init();
+        prefetch_tensormap(&tmA);
+        prefetch_tensormap(&tmB);
+    }
+    if (warp == 2) {
+        tmem_alloc(tmem_slot, 128);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    mg_pdl_wait();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            for (int kb = kFirst; kb < kEnd; kb++, it++) {
+                const int s = it % S::STAGES;
+                if (!mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1, p.status, kDevTimeoutEmpty)) break;
+                uint8_t* sA = smem + s * S::STAGE_BYTES;
+                uint8_t* sB = sA + S::A_BYTES;
+                const int k0 = kb * S::BK;
+                mbar_arrive_expect_tx(&full[s], S::STAGE_BYTES);
+                if (A_MN) {
+                    tma_load_3d(sA, &tmA, m0, k0, b, &full[s]);
+                    tma_load_3d(sA + 8192, &tmA, m0 + 64, k0, b, &full[s]);
+                } else {
+                    tma_load_3d(sA, &tmA, k0, m0, b, &full[s]);
+                }
+                if (B_MN) {
+                    tma_load_3d(sB, &tmB, n0, k0, b, &full[s]);
+                    tma_load_3d(sB + 8192, &tmB, n0 + 64, k0, b, &full[s]);
+                } else {
+                    tma_load_3d(sB, &tmB, k0, n0, b, &full[s]);
+                }
+            }
+            // every issued copy has landed before this CTA can exit
+            for (int k = it - S::STAGES < 0 ? 0 : it - S::STAGES; k < it; k++)
+                mbar_wait(&full[k % S::STAGES], (k / S::STAGES) & 1, p.status, kDevTimeoutFull);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_f16_f32(128, A_MN, B_MN);
+            for (int it = 0; it < kEnd - kFirst; it++) {
+                const int s = it % S::STAGES;
+                if (!mbar_wait(&full[s], (it / S::STAGES) & 1, p.status, kDevTimeoutFull)) break;
+                tc_fence_after();
+                const uint32_t aBase = smem_u32(smem + s * S::STAGE_BYTES), bBase = aBase + S::A_BYTES;
+#pragma unroll
+                for (int kk = 0; kk < 4; kk++) {
+                    const uint64_t ad = A_MN ? smem_desc_sw128(aBase + kk * 2048, 8192, 1024)
+                                             : smem_desc_sw128(aBase + kk * 32, 16, 1024);
+                    const uint64_t bd = B_MN ? smem_desc_sw128(bBase + kk * 2048, 8192, 1024)
+                                             : smem_desc_sw128(bBase + kk * 32, 16, 1024);
+                    tc_mma_bf16(tmem, ad, bd, idesc, (it > 0 || kk > 0) ? 1u : 0u);
+                }
+                tc_commit(&empty[s]);
+            }
+            tc_commit(done);  // covers every MMA issued, also after a timeout
+        }
+    }
+    const int e = warp - 2, q = warp & 3, row0 = m0 + 32 * q, col0 = n0 + 32 * (e / 4);
+    const bool wanted = e >= 0 && row0 < p.M && col0 < p.N && col0 >= row0, mirror = wanted && col0 != row0;
+    uint8_t* slab = smem + S::SLAB_OFF + (e < 0 ? 0 : e) * S::SLAB;
+    if (wanted) {
+        mbar_wait_warp(done, 0, p.status, kDevTimeoutDone);
+        tc_fence_after();
+        float v[32];
+        tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(32 * (e / 4)), v);
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            *reinterpret_cast<float4*>(slab + ns_slab_offset(lane, k)) = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+    }
+    __syncwarp();
+    cluster_sync();
+    const int share = 32 / splits, first = rank * share;  // rows of a piece that this CTA writes
+    const int64_t base = (int64_t)b * p.M * p.ldo;
+    if (wanted) {
+        const int k = lane & 7, col = col0 + 4 * k;
+        for (int r = first + (lane >> 3); r < first + share; r += 4) {
+            const int row = row0 + r;
+            const bool in = row < p.M && col < p.N;
+            uint2 gw = make_uint2(0u, 0u);
+            if (KIND == kNsPoly && in) gw = *reinterpret_cast<const uint2*>(p.g16 + base + (int64_t)row * p.ldo + col);
+            const uint32_t off = ns_slab_offset(r, k);
+            float4 y = *reinterpret_cast<const float4*>(cluster_peer(slab, 0) + off);
+            for (int z = 1; z < splits; z++) {
+                const float4 o = *reinterpret_cast<const float4*>(cluster_peer(slab, z) + off);
+                y.x += o.x;
+                y.y += o.y;
+                y.z += o.z;
+                y.w += o.w;
+            }
+            y.x *= kNsUnscale;
+            y.y *= kNsUnscale;
+            y.z *= kNsUnscale;
+            y.w *= kNsUnscale;
+            if (KIND == kNsPoly) {
+                const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&gw.x));
+                const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&gw.y));
+                y.x = fmaf(p.c, y.x, p.b * g0.x);
+                y.y = fmaf(p.c, y.y, p.b * g0.y);
+                y.z = fmaf(p.c, y.z, p.b * g1.x);
+                y.w = fmaf(p.c, y.w, p.b * g1.y);
+            }
+            if (in) *reinterpret_cast<uint2*>(p.out16 + base + (int64_t)row * p.ldo + col) = pack_half4(y.x, y.y, y.z, y.w);
+            // (rows `first` .. of this CTA's slab are read by nobody else)
+            if (mirror) *reinterpret_cast<float4*>(slab + off) = y;
+        }
+        __syncwarp();
+        const int mrow = col0 + lane;  // the mirrored piece, as in ns_piece
+        if (mirror && mrow < p.M) {
+            for (int r = first; r < first + share && row0 + r < p.ldo; r += 8) {
+                float y[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    y[i] = *reinterpret_cast<const float*>(slab + ns_slab_offset(r + i, lane >> 2) + (lane & 3) * 4);
+                const uint2 lo = pack_half4(y[0], y[1], y[2], y[3]), hi = pack_half4(y[4], y[5], y[6], y[7]);
+                *reinterpret_cast<uint4*>(p.out16 + base + (int64_t)mrow * p.ldo + row0 + r) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            }
+        }
+    }
+    cluster_sync();  // no CTA leaves while another reads its slabs
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        mbar_wait(done, 0, p.status, kDevTimeoutDone);
+        tc_fence_after();
+        tmem_dealloc(tmem, 128);
+    }
+}
+
 }  // namespace mg
