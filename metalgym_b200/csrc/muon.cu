@@ -189,19 +189,19 @@ int launch_split(const CUtensorMap& ta, const CUtensorMap& tb, NsProduct p, int 
 }
 
 // 256-wide tiles where they fill the GPU: half the operand bytes per product
-// of 128-wide ones, which below a wave leave too many SMs idle. Symmetric
-// products of few tiles split a long K over a cluster.
+// of 128-wide ones, which below a wave leave too many SMs idle. Few tiles split
+// a K of four blocks or more over a cluster, while the clusters fit the GPU at
+// once (measured: clusters of four on 144 of 148 SMs run in two waves).
 template <int KIND, bool A_MN, bool B_MN>
 int launch_product(const CUtensorMap& ta, const CUtensorMap& tb, const NsProduct& p, cudaStream_t st) {
-    if constexpr (KIND != kNsApply) {
-        const int64_t tiles = (int64_t)ns_tiles<KIND, 128>((p.M + 127) / 128, (p.N + 127) / 128) * p.batch;
-        int splits = 1;
-        while (splits < 4 && tiles * splits * 2 <= num_sms() && (p.K + 63) / 64 >= 4 * splits) splits *= 2;
-        if (splits > 1) return launch_split<KIND, A_MN, B_MN>(ta, tb, p, splits, st);
-    }
-    const int64_t tiles = (int64_t)ns_tiles<KIND, 256>((p.M + 127) / 128, (p.N + 255) / 256) * p.batch;
-    return tiles >= num_sms() ? launch_tiled<KIND, 256, A_MN, B_MN>(ta, tb, p, st)
-                              : launch_tiled<KIND, 128, A_MN, B_MN>(ta, tb, p, st);
+    const int64_t tiles = (int64_t)ns_tiles<KIND, 128>((p.M + 127) / 128, (p.N + 127) / 128) * p.batch;
+    const int blocks = (p.K + 63) / 64;
+    int splits = 1;
+    while (splits < 4 && tiles * splits * 2 <= num_sms() * 7 / 8 && blocks >= 4 && blocks >= 2 * splits) splits *= 2;
+    if (splits > 1) return launch_split<KIND, A_MN, B_MN>(ta, tb, p, splits, st);
+    const int64_t wide = (int64_t)ns_tiles<KIND, 256>((p.M + 127) / 128, (p.N + 255) / 256) * p.batch;
+    return wide >= num_sms() ? launch_tiled<KIND, 256, A_MN, B_MN>(ta, tb, p, st)
+                             : launch_tiled<KIND, 128, A_MN, B_MN>(ta, tb, p, st);
 }
 
 struct Workspace {

@@ -421,17 +421,16 @@ __global__ void __launch_bounds__(NsTile<BN>::THREADS, 1)
     }
 }
 
-// G or B of few tiles with K split over the CTAs of a cluster, one 128 x 128
+// Products of few tiles with K split over the CTAs of a cluster, one 128 x 128
 // tile per cluster: a tile's operands come at about 55 bytes a cycle and SM
 // from L2, 590 cycles for a K block whose products take 256, so that few tiles
 // with a long K leave most of that rate unused. Every CTA leaves its part of
 // the sum in the slabs; CTA r then adds the parts of rows 32 r / splits .. of
-// each piece, in their order, and writes them.
+// each piece, in their order, and writes them. (512 x 2048: 178 -> 128 us.)
 template <int KIND, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(NsTile<128>::THREADS, 1)
     k_ns_split(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const NsProduct p, int splits) {
     using S = NsTile<128>;
-    static_assert(KIND != kNsApply, "symmetric products");
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::BAR_OFF);
@@ -516,7 +515,8 @@ __global__ void __launch_bounds__(NsTile<128>::THREADS, 1)
         }
     }
     const int e = warp - 2, q = warp & 3, row0 = m0 + 32 * q, col0 = n0 + 32 * (e / 4);
-    const bool wanted = e >= 0 && row0 < p.M && col0 < p.N && col0 >= row0, mirror = wanted && col0 != row0;
+    const bool wanted = e >= 0 && row0 < p.M && col0 < p.N && (KIND == kNsApply || col0 >= row0);
+    const bool mirror = KIND != kNsApply && wanted && col0 != row0, finVec = KIND == kNsApply && p.last && p.fin.vec;
     uint8_t* slab = smem + S::SLAB_OFF + (e < 0 ? 0 : e) * S::SLAB;
     if (wanted) {
         mbar_wait_warp(done, 0, p.status, kDevTimeoutDone);
@@ -537,7 +537,13 @@ __global__ void __launch_bounds__(NsTile<128>::THREADS, 1)
             const int row = row0 + r;
             const bool in = row < p.M && col < p.N;
             uint2 gw = make_uint2(0u, 0u);
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), m = x;
+            const int64_t finAt = (int64_t)b * p.fin.stride + (int64_t)row * p.fin.ld + col;
             if (KIND == kNsPoly && in) gw = *reinterpret_cast<const uint2*>(p.g16 + base + (int64_t)row * p.ldo + col);
+            if (KIND == kNsApply && in) {
+                x = ld_f4_now(p.x32 + base + (int64_t)row * p.ldo + col);
+                if (finVec && p.fin.master && col + 4 <= p.N) m = ld_f4_now(p.fin.master + finAt);
+            }
             const uint32_t off = ns_slab_offset(r, k);
             float4 y = *reinterpret_cast<const float4*>(cluster_peer(slab, 0) + off);
             for (int z = 1; z < splits; z++) {
@@ -546,6 +552,10 @@ __global__ void __launch_bounds__(NsTile<128>::THREADS, 1)
                 y.y += o.y;
                 y.z += o.z;
                 y.w += o.w;
+            }
+            if (KIND == kNsApply) {
+                if (in) ns_apply4(p, base + (int64_t)row * p.ldo + col, finAt, col, y, x, m, finVec);
+                continue;
             }
             y.x *= kNsUnscale;
             y.y *= kNsUnscale;
