@@ -285,12 +285,12 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
         sum = *sNorm;
     }
     const double inv = sum == 0.0 ? 0.0 : 1.0 / sqrt(sum);
-    // piece i of X (from `held`, where its loads are, or were) into a tile
+    // the piece of X in `held` into a tile; piece `next` is loaded behind it
     auto load = [&](int i) {
 #pragma unroll
         for (int j = 0; j < PER; j++) cell(i, cellIndex(tid + j * kMuonSmallThreads), false, held[j]);
     };
-    auto tile = [&](uint8_t* mat) {
+    auto tile = [&](uint8_t* mat, int next) {
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             const int g = cellIndex(tid + j * kMuonSmallThreads);
@@ -298,6 +298,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
 #pragma unroll
             for (int k = 0; k < 8; k++) u[k] = (float)((double)held[j][k] * inv) * kNsScale;
             split_store8(mat, sw128_offset(g >> 4, g & 15), u);
+            if (next < end) cell(next, g, false, held[j]);
         }
         handOver();
     };
@@ -306,9 +307,8 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
     for (int i = first; i < end; i++) {
         const int k = (i - first) & 1;
         uint8_t* mat = k ? mP : mQ;
-        if (i > first) load(i);
         if (i - first >= 2) wait(k);
-        tile(mat);
+        tile(mat, i + 1);
         if (tid == 0) {
             split_mma<!WIDE, !WIDE, SP, 8>(tmem, smem_u32(mat), smem_u32(mat), i > first);
             tc_commit(&bar[k]);
@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
     uint8_t* slab = mQ + warp * 4096;
     auto issue = [&](int i) {
         const int k = (i - first) & 1;
-        tile(mG);
+        tile(mG, i + 1);
         if (tid == 0) {
             if (WIDE)
                 split_mma<false, true, N, KS>(tmem + 128 * k, aP, aG, false);
@@ -465,7 +465,6 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
     }
     for (int i = first; i < end; i++) {
         const int k = (i - first) & 1;
-        if (i + 1 < end) load(i + 1);
         wait(k);
         if (i + 1 < end) issue(i + 1);
         const int row0 = 32 * q + (WIDE ? 0 : 128 * i), c = 32 * (warp >> 2), col0 = c + (WIDE ? 128 * i : 0);
