@@ -396,7 +396,9 @@ typedef struct mg_logit_controls {
 /* out[r][a] = controlled logit, in the logits' type. logits [rows][ld] and out
  * [rows][ldo] of `dtype` (mg_dtype); columns from `actions` on are neither
  * read nor written. controls may be NULL (a copy). out may be logits itself
- * (then ldo = ld); any other overlap is not allowed. */
+ * (then ldo = ld); any other overlap is not allowed. At most
+ * MG_LOGITS_MAX_ACTIONS actions. As everywhere, the buffers belong to the
+ * current device. */
 int mg_logits_control(const void* logits, int dtype, int64_t ld, const mg_logit_controls* controls, void* out,
                       int64_t ldo, int rows, int actions, mg_stream_t stream);
 /* Its gradient with respect to the raw logits: d_logits = d_out times the
@@ -418,8 +420,8 @@ int mg_logits_control_backward(const void* logits, int dtype, int64_t ld, const 
  * probability, and the draw of a row does not depend on how it is split over
  * threads. rng NULL: the largest controlled logit. Equal ones: the lowest
  * index. A row without an allowed action gets action -1, log-probability 0
- * and entropy 0. A NaN at an allowed action is never drawn and makes the
- * row's log-probability and entropy NaN. */
+ * and entropy 0. A NaN or +infinity at an allowed action makes the row's
+ * log-probability and entropy NaN; a NaN is never drawn. */
 int mg_logits_sample(const void* logits, int dtype, int64_t ld, const mg_logit_controls* controls, uint32_t* rng,
                      int32_t* action, float* log_prob, float* entropy, float* value, int rows, int actions,
                      mg_stream_t stream);

@@ -191,20 +191,20 @@ __device__ __forceinline__ float warp_max(float x) {
     return y;
 }
 
-// log2(e^l) - m. Every use takes the same m, so that the rounding of m (the
-// largest logit in these units) is the same for all and falls out of
-// probabilities and their logarithms; the product is not rounded (FMA). Kept
-// finite, so that e^-inf = 0 times it is 0 (a NaN stays one).
-__device__ __forceinline__ float log2_weight(float l, float m) { return max_nan(fmaf(l, kLog2e, -m), -1e30f); }
+// l - m for a logit and the running maximum, kept finite, so that e^-inf = 0
+// times it is 0 (a NaN stays one). Subtracted before anything is scaled: logits
+// up to the type's largest and lowest numbers stay in range.
+__device__ __forceinline__ float below(float l, float m) { return max_nan(l - m, -1e30f); }
+__device__ __forceinline__ float exp_fast(float d) { return exp2_fast(d * kLog2e); }
 
-// Running softmax statistics in units of log2: the maximum m, s = sum 2^d, t =
-// sum 2^d d with d = log2_weight(l, m); entropy = ln 2 (log2 s - t / s). In the
-// passes m is the same in the threads of a warp, s and t are a thread's.
+// Running softmax statistics: the maximum m, s = sum e^d, t = sum e^d d with d =
+// l - m; entropy = log s - t / s. In the passes m is the same in the threads of
+// a warp, s and t are a thread's.
 struct Softmax {
     float m = -INFINITY, s = 0.0f, t = 0.0f;
     // Raises m (a whole warp) and returns the factor that carried s over.
     __device__ __forceinline__ float raise(float top) {
-        const float d = m - top, e = m > -INFINITY ? exp2_fast(d) : 0.0f;
+        const float d = below(m, top), e = exp_fast(d);
         t = e > 0.0f ? e * (t + s * d) : 0.0f;
         if (!(s != s)) s = s * e;
         m = top;
@@ -220,7 +220,7 @@ __device__ __forceinline__ bool softmax_group(Softmax& v, const float* x, Raised
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < N; i++) top = fmaxf(top, x[i]);
-    top = warp_max(top) * kLog2e;
+    top = warp_max(top);
     if (top > v.m) raised(v.raise(top));
     if (v.m == -INFINITY) {  // a NaN still shows
 #pragma unroll
@@ -232,17 +232,17 @@ __device__ __forceinline__ bool softmax_group(Softmax& v, const float* x, Raised
     const float2 k2 = make_float2(kLog2e, kLog2e), m2 = make_float2(-v.m, -v.m);
 #pragma unroll
     for (int i = 0; i + 1 < N; i += 2) {  // two at a time (f32x2)
-        float2 d = f2fma_rn(make_float2(x[i], x[i + 1]), k2, m2);
+        float2 d = f2add_rn(make_float2(x[i], x[i + 1]), m2);
         d.x = max_nan(d.x, -1e30f);
         d.y = max_nan(d.y, -1e30f);
-        const float2 w = make_float2(exp2_fast(d.x), exp2_fast(d.y));
+        const float2 k = f2mul_rn(d, k2), w = make_float2(exp2_fast(k.x), exp2_fast(k.y));
         s2 = f2add_rn(s2, w);
         t2 = f2fma_rn(w, d, t2);
         each(i, w.x);
         each(i + 1, w.y);
     }
     if (N & 1) {
-        const float d = log2_weight(x[N - 1], v.m), w = exp2_fast(d);
+        const float d = below(x[N - 1], v.m), w = exp_fast(d);
         s2.x += w;
         t2.x = fmaf(w, d, t2.x);
         each(N - 1, w);
@@ -345,7 +345,7 @@ __device__ inline void row_merge(RowPart& mine, RowPart* warps, int parts, int c
     float s = 0.0f, t = 0.0f;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        const float d = v[k].m > -INFINITY ? v[k].m - m : 0.0f, f = exp2_fast(d);
+        const float d = v[k].m > -INFINITY ? below(v[k].m, m) : 0.0f, f = exp_fast(d);
         s += v[k].s * f;
         if (f > 0.0f) t += f * (v[k].t + v[k].s * d);
     }
@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
     if (!GREEDY) rngNext(word);
     RowPart mine;
     float bound = 3e38f;  // the warp's best ratio E / e^(l - m)
-    __shared__ int sharedBound;  // the CTA's, as an ordered log2 (E / e^l)
+    __shared__ int sharedBound;  // the CTA's, as an ordered log(E / e^l)
     if (NT > 32 && !GREEDY) {
         if (threadIdx.x == 0) sharedBound = 0x7f800000;
         __syncthreads();
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
         auto raised = [&](float f) { bound = f > 0.0f ? fminf(bound / f, 3e38f) : 3e38f; };
         const bool some = softmax_group<N>(mine.v, l, raised, [&](int i, float e) {
             if (i == 0) {
-                if (NT > 32) bound = fminf(bound, exp2_fast(ordered_float(*(volatile int*)&sharedBound) + mine.v.m));
+                if (NT > 32) bound = fminf(bound, exp_fast(ordered_float(*(volatile int*)&sharedBound) + mine.v.m));
                 limit = fminf(bound * 65542.6f, 3e38f);  // 2^16 (1 + 1e-4)
             }
             uint32_t h = word + (uint32_t)at(i) * 0x9E3779B9u;
@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
             const float now = fminf(bound * 65542.6f, 3e38f);
 #pragma unroll
             for (int i = 0; i < N; i++) {
-                const float f = (float)(race_bits(word, at(i)) >> 16), e = exp2_fast(log2_weight(l[i], mine.v.m));
+                const float f = (float)(race_bits(word, at(i)) >> 16), e = exp_fast(below(l[i], mine.v.m));
                 if (f <= now * e) out |= 1u << i;
             }
             return out & bits;
@@ -492,7 +492,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
 #pragma unroll
                 for (int k = 1; k < N; k++) li = k == i ? l[k] : li;
                 const uint32_t h = race_bits(word, at(i));
-                const float e = exp2_fast(log2_weight(li, mine.v.m));
+                const float e = exp_fast(below(li, mine.v.m));
                 if (li > -INFINITY && (float)(h >> 16) <= bound * 65542.6f * e) {
                     // -log(1 - v): its series below 1 / 64 (the next term is 4e-6 of it), else from 1 - v
                     const float u = ((float)h + 0.5f) * 2.3283064e-10f;
@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
             const float least = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(ratio)));
             if (least < bound) {
                 bound = least;
-                if (NT > 32 && (threadIdx.x & 31) == 0) atomicMin(&sharedBound, float_order(log2_fast(least) - mine.v.m));
+                if (NT > 32 && (threadIdx.x & 31) == 0) atomicMin(&sharedBound, float_order(kLn2 * log2_fast(least) - mine.v.m));
                 if (N > 4 && __any_sync(0xffffffffu, (pass & (pass - 1)) != 0)) pass = still(pass);
             }
         }
@@ -525,11 +525,11 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
     }
     row_merge<NT, true, GREEDY>(mine, warps, part.parts, 0);
     if (tid == 0 && lo == 0) {
-        const float ls = log2f(mine.v.s);
+        const float ls = logf(mine.v.s);
         const bool some = mine.best.action >= 0 || mine.v.s != mine.v.s;
         action[row] = mine.best.action;
-        logProb[row] = some ? (log2_weight(mine.best.logit, mine.v.m) - ls) * kLn2 : 0.0f;
-        if (entropy) entropy[row] = some ? (ls - mine.v.t / mine.v.s) * kLn2 : 0.0f;
+        logProb[row] = some ? below(mine.best.logit, mine.v.m) - ls : 0.0f;
+        if (entropy) entropy[row] = some ? ls - mine.v.t / mine.v.s : 0.0f;
         if (value) value[row] = to_f32(x[part.actions]);
         if (!GREEDY) rng[row] = word;
     }
@@ -603,8 +603,8 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
         }
     }
     row_merge<NT, false, false>(mine, warps, part.parts, act / part.span);
-    const float m = mine.v.m, ls = log2f(mine.v.s), entropy = (ls - mine.v.t / mine.v.s) * kLn2;
-    const float logp = (log2_weight(mine.chosen, m) - ls) * kLn2;
+    const float m = mine.v.m, ls = logf(mine.v.s), entropy = ls - mine.v.t / mine.v.s;
+    const float logp = below(mine.chosen, m) - ls;
     const float ratio = expf(logp - old);
     const float adv = L.advStats ? (advRaw - adv0) * adv1 : advRaw;
     const float one = ratio * adv, two = fminf(fmaxf(ratio, 1.0f - L.clip), 1.0f + L.clip) * adv;
@@ -616,12 +616,12 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
         cluster_sync();
     else
         __syncthreads();
-    // dl = scale (slope (1[a = act] - p) + ent p (ln p + H)) = p (s1 log2 p + (ent H - slope) scale), + s0 at act
-    const float s0 = slope * L.scale, s1 = L.entropyCoef * L.scale * kLn2, sh = fmaf(L.entropyCoef * L.scale, entropy, -s0);
+    // dl = scale (slope (1[a = act] - p) + ent p (ln p + H)) = p (s1 log p + (ent H - slope) scale), + s0 at act
+    const float s0 = slope * L.scale, s1 = L.entropyCoef * L.scale, sh = fmaf(L.entropyCoef * L.scale, entropy, -s0);
     const bool vec = same_alignment(x, d), all_nan = !(fabsf(sh) < INFINITY && fabsf(s1) < INFINITY);
     auto gradient = [&](float l, int a) {
-        const float q = log2_weight(l, m) - ls;
-        const float g = exp2_fast(q) * fmaf(s1, q, sh);
+        const float q = below(l, m) - ls;
+        const float g = exp_fast(q) * fmaf(s1, q, sh);
         return a == act ? g + s0 : g;
     };
     constexpr int U = 2;
@@ -641,11 +641,11 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
             const float2 s12 = make_float2(s1, s1), sh2 = make_float2(sh, sh);
 #pragma unroll
             for (int i = 0; i < VE; i += 2) {
-                float2 q = f2fma_rn(make_float2(l[i], l[i + 1]), k2, m2);
+                float2 q = f2add_rn(make_float2(l[i], l[i + 1]), m2);
                 q.x = max_nan(q.x, -1e30f);
                 q.y = max_nan(q.y, -1e30f);
                 q = f2add_rn(q, ls2);
-                const float2 p = make_float2(exp2_fast(q.x), exp2_fast(q.y));
+                const float2 k = f2mul_rn(q, k2), p = make_float2(exp2_fast(k.x), exp2_fast(k.y));
                 const float2 o = f2mul_rn(p, f2fma_rn(s12, q, sh2));
                 l[i] = o.x;
                 l[i + 1] = o.y;

@@ -386,6 +386,42 @@ def test_nan_and_minus_infinity_at_allowed_actions(mg):
     assert 0 <= a[3] < 40
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("actions", [5, 40, 3000])
+def test_logits_at_the_ends_of_the_type(mg, kind, actions):
+    """Rows of the type's lowest number (a mask some programs write), of large offsets and of wide spreads: the softmax of
+    equal logits is uniform whatever their size, and an entry far below the others has no weight."""
+    code, dtype = TYPES[kind]
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x = torch.full((6, actions), low, dtype=dtype)
+    x[1, 2] = 0.0
+    x[2] = high
+    x[3] = low
+    x[3, 1] = high
+    x[4] = 1000.0
+    x[4, :2] = 1008.0
+    x[5, ::2] = -math.inf
+    words = torch.arange(1, 7, dtype=torch.int32, device="cuda")
+    xd = x.cuda()
+    act, lp, ent = torch.empty(6, dtype=torch.int32, device="cuda"), torch.empty(6, device="cuda"), torch.empty(6, device="cuda")
+    ok(mg, mg.mg_logits_sample(xd.data_ptr(), code, actions, None, words.data_ptr(), act.data_ptr(), lp.data_ptr(), ent.data_ptr(), None, 6,
+                               actions, None))
+    assert status(mg) == 0
+    a = act.cpu().numpy()
+    assert np.all((a >= 0) & (a < actions)) and a[1] == 2 and a[3] == 1 and a[5] % 2 == 1
+    ref, h, _ = softmax_reference(x.float().numpy())
+    e = delta(actions, 8.0)
+    assert np.all(np.abs(lp.cpu().numpy() - ref[np.arange(6), a]) <= e + 2.0 ** -21)
+    assert np.all(np.abs(ent.cpu().numpy() - h) <= e * 17 + 2.0 ** -21)
+    d, st, z = torch.empty(6, actions, dtype=dtype, device="cuda"), torch.empty(6, 5, device="cuda"), torch.ones(6, device="cuda")
+    ok(mg, mg.mg_logits_policy_loss(xd.data_ptr(), code, actions, None, act.data_ptr(), z.data_ptr(), None, None, lp.data_ptr(), d.data_ptr(),
+                                    actions, st.data_ptr(), 6, actions, 0.2, 0.5, 0.0, 1.0, None))
+    assert status(mg) == 0
+    want = np.exp(ref) - (np.arange(actions) == a[:, None])
+    assert np.all(np.abs(d.double().cpu().numpy() - want) <= 4 * e + torch.finfo(dtype).eps / 2 + 2.0 ** -20)
+
+
 # ------------------------------------------------------------------ loss
 
 
