@@ -34,9 +34,9 @@ constexpr int kPrepThreads = 256;
 constexpr int kPrepWarps = kPrepThreads / 32;
 constexpr int kPrepMaxParts = 1024;  // CTAs (and norm partials) per matrix at most
 
-// U into X32 (not yet divided by its norm) and one 64-bit sum of squares a CTA:
-// the squares of any finite fp32 U neither overflow nor vanish in 64 bits. A
-// warp takes a row, a lane V columns at a time.
+// U into X32 (not yet divided by its norm) and one 64-bit sum of squares a CTA,
+// in which the squares of any finite fp32 U neither overflow nor vanish. A
+// thread takes V columns of a row at a time.
 template <class T, bool MUON, int V>
 __global__ void __launch_bounds__(kPrepThreads)
     k_muon_prepare(const MuonInput in, MuonShape s, float* x32, double* partial) {
@@ -103,8 +103,7 @@ __global__ void __launch_bounds__(kPrepThreads)
             *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(u);
         else
             dst[0] = u[0];
-#pragma unroll
-        for (int k = 0; k < V; k++) sum += (double)u[k] * (double)u[k];
+        sum += square_sum<V>(u);
     }
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -132,16 +131,13 @@ __global__ void __launch_bounds__(kPrepThreads)
     __syncthreads();
     sum = sSum[0];
     for (int w = 1; w < kPrepWarps; w++) sum += sSum[w];
-    const double inv = sum == 0.0 ? 0.0 : 1.0 / sqrt(sum);
+    const InverseNorm inv(sum);
     const int64_t total = (int64_t)s.rows * s.ldx / 4;
     float4* x = reinterpret_cast<float4*>(x32 + (int64_t)b * s.rows * s.ldx);
     uint2* h = reinterpret_cast<uint2*>(x16 + (int64_t)b * s.rows * s.ldx);
     for (int64_t i = (int64_t)blockIdx.x * kPrepThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kPrepThreads) {
         float4 v = x[i];  // (the padding's values are never read as operands)
-        v.x = (float)((double)v.x * inv);
-        v.y = (float)((double)v.y * inv);
-        v.z = (float)((double)v.z * inv);
-        v.w = (float)((double)v.w * inv);
+        v = make_float4(inv(v.x), inv(v.y), inv(v.z), inv(v.w));
         x[i] = v;
         h[i] = pack_half4(v.x * kNsScale, v.y * kNsScale, v.z * kNsScale, v.w * kNsScale);
     }

@@ -46,6 +46,36 @@ struct MuonSmall {
     static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024 /*align*/;
 };
 
+// The sum of N squares. 64-bit conversions run at 16 a cycle and SM, so that
+// they, not the loads, would set the pace of a pass (3 of 8 us per 128 x 128
+// piece): squares are summed in fp32 wherever that neither overflows nor loses
+// small ones, and a CTA's sums in 64 bits.
+template <int N>
+__device__ __forceinline__ double square_sum(const float* u) {
+    float f = 0.0f;
+#pragma unroll
+    for (int k = 0; k < N; k++) f = fmaf(u[k], u[k], f);
+    if (f > 1e-25f && f < 1e30f) return (double)f;
+    double d = 0.0;
+#pragma unroll
+    for (int k = 0; k < N; k++) d += (double)u[k] * (double)u[k];
+    return d;
+}
+
+// x -> x / norm by fp32 products that stay in range for every norm: 1 / norm =
+// p q m with p and q powers of two (0 for a zero norm).
+struct InverseNorm {
+    float p, q, m;
+    __device__ __forceinline__ explicit InverseNorm(double squares) {
+        int e = 0;
+        m = squares == 0.0 ? 0.0f : (float)frexp(1.0 / sqrt(squares), &e);  // NaN and infinity stay NaN and 0
+        const int first = max(-126, min(126, e));
+        p = ldexpf(1.0f, first);
+        q = ldexpf(1.0f, max(-126, min(126, e - first)));
+    }
+    __device__ __forceinline__ float operator()(float x) const { return ((x * p) * q) * m; }
+};
+
 // The clip factor of mg_adam_step from the norm partials (one warp; lane 0's
 // value counts). The squared norm goes to *normSq.
 __device__ __forceinline__ float muon_clip(const MuonInput& in, float* normSq) {
@@ -265,8 +295,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             cell(i, cellIndex(tid + j * kMuonSmallThreads), true, held[j]);
-#pragma unroll
-            for (int k = 0; k < 8; k++) sum += (double)held[j][k] * (double)held[j][k];
+            sum += square_sum<8>(held[j]);
         }
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
@@ -284,7 +313,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
         __syncthreads();
         sum = *sNorm;
     }
-    const double inv = sum == 0.0 ? 0.0 : 1.0 / sqrt(sum);
+    const InverseNorm inv(sum);
     // the piece of X in `held` into a tile; piece `next` is loaded behind it
     auto load = [&](int i) {
 #pragma unroll
@@ -296,7 +325,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
             const int g = cellIndex(tid + j * kMuonSmallThreads);
             float u[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++) u[k] = (float)((double)held[j][k] * inv) * kNsScale;
+            for (int k = 0; k < 8; k++) u[k] = inv(held[j][k]) * kNsScale;
             split_store8(mat, sw128_offset(g >> 4, g & 15), u);
             if (next < end) cell(next, g, false, held[j]);
         }
