@@ -653,3 +653,46 @@ def test_stream_capture_and_repeat(mg):
     for got, want in zip(captured, plain):
         assert torch.equal(got, want)
     assert status(mg) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,actions", [(300, 70), (40, 9000), (3, 60000)])
+def test_two_calls_at_once_and_a_repeat(mg, rows, actions):
+    """Loss and draw of the same logits on two streams together, twice: the bits of the calls made one after the other."""
+    rng = np.random.default_rng(rows)
+    c = make_controls(rng, rows, actions, ("mask", "bias", "history"))
+    dev = {}
+    cs = controls_struct(c, dev)
+    xn = logits_of(rng, rows, actions, "bf16")
+    action, old, adv = loss_inputs(rng, xn.float().numpy(), c, rows, actions)
+    x = xn.cuda()
+    t = [torch.from_numpy(v).cuda() for v in (action, adv, old)]
+    first = torch.arange(1, rows + 1, dtype=torch.int32, device="cuda")
+
+    def loss(stream):
+        d, st = torch.zeros_like(x), torch.zeros(rows, 5, device="cuda")
+        torch.cuda.synchronize()
+        return d, st, lambda: ok(mg, mg.mg_logits_policy_loss(
+            x.data_ptr(), 1, actions, cs, t[0].data_ptr(), t[1].data_ptr(), None, None, t[2].data_ptr(), d.data_ptr(), actions, st.data_ptr(),
+            rows, actions, 0.2, 0.5, 0.01, 1.0, stream))
+
+    def draw(stream):
+        w, a, lp = first.clone(), torch.zeros(rows, dtype=torch.int32, device="cuda"), torch.zeros(rows, device="cuda")
+        torch.cuda.synchronize()
+        return w, a, lp, lambda: ok(mg, mg.mg_logits_sample(x.data_ptr(), 1, actions, cs, w.data_ptr(), a.data_ptr(), lp.data_ptr(), None, None,
+                                                            rows, actions, stream))
+
+    one, two = loss(None), draw(None)
+    one[-1]()
+    torch.cuda.synchronize()
+    two[-1]()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(2):
+        three, four = loss(streams[0].cuda_stream), draw(streams[1].cuda_stream)
+        three[-1]()
+        four[-1]()
+        torch.cuda.synchronize()
+        for a, b in zip((*one[:-1], *two[:-1]), (*three[:-1], *four[:-1])):
+            assert torch.equal(a, b)
+    assert status(mg) == 0

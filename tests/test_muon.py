@@ -256,6 +256,72 @@ def test_muon_step(mg, batch, m, n, nesterov, clip):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(64, 200), (200, 300)])
+@pytest.mark.parametrize("offset", [0, 1, 3])
+def test_buffers_off_vector_alignment(mg, m, n, offset):
+    """Matrices whose first element, rows or distance from one to the next are not 16-byte aligned: the aligned call's bits."""
+    gen = torch.Generator(device="cuda").manual_seed(offset + m)
+    batch, results = 2, []
+    grad = torch.randn(batch, m, n, generator=gen, device="cuda")
+    master, momentum = torch.randn(batch, m, n, generator=gen, device="cuda"), torch.randn(batch, m, n, generator=gen, device="cuda")
+    space = workspace(mg, batch, m, n)
+    for shift, stride in ((0, m * n), (offset, m * n + offset)):
+        def place(t, dtype=torch.float32):
+            flat = torch.full((shift + batch * stride + 8,), 3.0, dtype=dtype, device="cuda")
+            view = torch.as_strided(flat, (batch, m, n), (stride, n, 1), shift)
+            view.copy_(t)
+            return flat, view
+
+        (fm, vm), (fg, vg), (fo, vo), (fw, vw) = place(master), place(grad), place(momentum), place(master, torch.bfloat16)
+        ok(mg, mg.mg_muon_step(vm.data_ptr(), vg.data_ptr(), vo.data_ptr(), vw.data_ptr(), stride, batch, m, n, None, 0, 0.0, 0.01, 1.0, 0.9, 1,
+                               0.0, 5, None, space.data_ptr(), space.numel(), None))
+        out, view = place(master, torch.float16)
+        ok(mg, mg.mg_orthogonalize(vw.data_ptr(), 1, n, stride, view.data_ptr(), 2, n, stride, batch, m, n, 5, space.data_ptr(), space.numel(), None))
+        assert status(mg) == 0
+        for flat in (fm, fg, fo, fw, out):  # what lies around the matrices stays
+            assert (flat[:shift] == 3).all() and (flat[shift + (batch - 1) * stride + m * n:] == 3).all()
+            assert (flat[shift + m * n: shift + stride] == 3).all()
+        results.append([t.clone() for t in (vm, vo, vw, view)])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(128, 512), (300, 520)])
+def test_captured_step_replays(mg, m, n):
+    """A captured optimiser step replayed three times does what three calls do."""
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    start = [torch.randn(2, m, n, generator=gen, device="cuda") for _ in range(3)]
+    norm = torch.full((1,), 50.0, device="cuda")
+    space = [workspace(mg, 2, m, n) for _ in range(2)]
+
+    def buffers():
+        master, grad, momentum = (t.clone() for t in start)
+        return master, grad, momentum, master.bfloat16()
+
+    def call(b, s, stream):
+        ok(mg, mg.mg_muon_step(b[0].data_ptr(), b[1].data_ptr(), b[2].data_ptr(), b[3].data_ptr(), m * n, 2, m, n, norm.data_ptr(), 1, 0.5, 0.01,
+                               1.0, 0.9, 1, 0.1, 5, None, s.data_ptr(), s.numel(), stream))
+
+    plain, held = buffers(), buffers()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        graph.capture_begin()
+        call(held, space[1], side.cuda_stream)
+        graph.capture_end()
+        for _ in range(3):
+            graph.replay()
+    for _ in range(3):
+        call(plain, space[0], None)
+    torch.cuda.synchronize()
+    assert status(mg) == 0
+    for a, b in zip(plain, held):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_two_streams_two_workspaces_and_a_graph(mg):
     """Two calls at once with a workspace each, and a captured graph replayed beside one of them: the same bits as alone."""
     gen = torch.Generator(device="cuda").manual_seed(3)
