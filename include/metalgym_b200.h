@@ -419,8 +419,8 @@ int mg_logits_control_backward(const void* logits, int dtype, int64_t ld, const 
  * of rates e^l, the first of which rings in a with the softmax's
  * probability, and the draw of a row does not depend on how it is split over
  * threads. rng NULL: the largest controlled logit. Equal ones: the lowest
- * index. A row without an allowed action gets action -1, log-probability 0
- * and entropy 0. A NaN or +infinity at an allowed action makes the row's
+ * index. A row without an allowed action of a logit above -inf gets action
+ * -1, log-probability 0 and entropy 0. A NaN or +infinity at an allowed action makes the row's
  * log-probability and entropy NaN; a NaN is never drawn. */
 int mg_logits_sample(const void* logits, int dtype, int64_t ld, const mg_logit_controls* controls, uint32_t* rng,
                      int32_t* action, float* log_prob, float* entropy, float* value, int rows, int actions,
@@ -433,8 +433,8 @@ int mg_logits_sample(const void* logits, int dtype, int64_t ld, const mg_logit_c
  * and its gradient goes to column `actions` of d_logits (ld, ldd > actions).
  * Other columns of d_logits are left as they were. adv_stats as in
  * mg_policy_loss. A row whose action is -1 (padding, or drawn from a row that
- * allowed nothing) or not allowed by the mask gets zeros in its gradient and
- * its statistics; any other action outside [0, actions) does too, and is
+ * allowed nothing), not allowed by the mask or of a logit -inf gets zeros in
+ * its gradient and its statistics; any other action outside [0, actions) does too, and is
  * recorded in the device status word. d_logits may be logits itself (then
  * ldd = ld). */
 int mg_logits_policy_loss(const void* logits, int dtype, int64_t ld, const mg_logit_controls* controls,

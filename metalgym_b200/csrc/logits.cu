@@ -41,10 +41,11 @@ struct TeamPart {
 template <int NT>
 __device__ __forceinline__ bool team_part(const TeamPart& p, int& row, int& lo, int& hi) {
     if (NT == 32) {
-        row = blockIdx.x * kWarpRows + (threadIdx.x >> 5);
+        const unsigned r = blockIdx.x * kWarpRows + (threadIdx.x >> 5);  // (past 2^31 in the last CTA of 2^31 - 1 rows)
+        row = (int)r;
         lo = 0;
         hi = p.actions;
-        return row < p.rows;
+        return r < (unsigned)p.rows;
     }
     row = blockIdx.x / p.parts;
     lo = min(p.actions, (int)(blockIdx.x % p.parts) * p.span);
@@ -572,11 +573,14 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
     const float adv0 = L.advStats ? L.advStats[0] : 0.0f, adv1 = L.advStats ? L.advStats[1] : 1.0f;
     const float valueX = L.ret && lo == 0 ? to_f32(x[actions]) : 0.0f;
     const bool inside = act >= 0 && act < actions;
-    if (!inside || !allowed(r, act)) {  // the same for every CTA of the row
-        if (tid == 0 && lo == 0 && !inside && act != -1) record_error(L.status, kDevBadAction);
+    auto leaveOut = [&] {
         for (int a = lo + tid; a < hi; a += NT) from_f32(&d[a], 0.0f);
         if (lo == 0 && L.ret && tid == 0) from_f32(&d[actions], 0.0f);
         if (lo == 0 && tid < 5) L.stats[(int64_t)row * 5 + tid] = 0.0f;
+    };
+    if (!inside || !allowed(r, act)) {  // the same for every CTA of the row
+        if (tid == 0 && lo == 0 && !inside && act != -1) record_error(L.status, kDevBadAction);
+        leaveOut();
         return;
     }
     if (r.history)
@@ -616,6 +620,10 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
         cluster_sync();
     else
         __syncthreads();
+    if (mine.chosen == -INFINITY) {  // an action that the policy never takes
+        leaveOut();
+        return;
+    }
     // dl = scale (slope (1[a = act] - p) + ent p (ln p + H)) = p (s1 log p + (ent H - slope) scale), + s0 at act
     const float s0 = slope * L.scale, s1 = L.entropyCoef * L.scale, sh = fmaf(L.entropyCoef * L.scale, entropy, -s0);
     const bool vec = same_alignment(x, d), all_nan = !(fabsf(sh) < INFINITY && fabsf(s1) < INFINITY);

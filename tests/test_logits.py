@@ -599,6 +599,47 @@ def test_actions_outside_the_set_are_recorded(mg):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("actions", [9, 5000, 40000])
+def test_loss_leaves_out_actions_of_logit_minus_infinity(mg, actions):
+    """Rows whose action has the logit -inf (one of them with nothing else either), or was masked by the type's lowest
+    number beside others: zeros in the first two, the ordinary loss in the third."""
+    x = torch.zeros(3, actions + 1, device="cuda")
+    x[0, 4] = -math.inf
+    x[1, :actions] = -math.inf
+    x[2, 5:actions] = torch.finfo(torch.float32).min
+    action = torch.tensor([4, 2, 1], dtype=torch.int32, device="cuda")
+    one, old = torch.ones(3, device="cuda"), torch.full((3,), -math.log(5.0), device="cuda")
+    d, st = torch.full((3, actions + 1), 7.0, device="cuda"), torch.full((3, 5), 7.0, device="cuda")
+    ok(mg, mg.mg_logits_policy_loss(x.data_ptr(), 0, actions + 1, None, action.data_ptr(), one.data_ptr(), None, one.data_ptr(), old.data_ptr(),
+                                    d.data_ptr(), actions + 1, st.data_ptr(), 3, actions, 0.2, 0.5, 0.0, 1.0, None))
+    assert status(mg) == 0
+    assert not d[:2].any() and not st[:2].any()
+    want = torch.zeros(actions + 1, device="cuda")
+    want[:5] = 0.2  # p of the five, less 1 at the action; ratio 1, advantage 1; the value's 0.5 * (0 - 1)
+    want[1] -= 1.0
+    want[actions] = -0.5
+    torch.testing.assert_close(d[2], want, rtol=0, atol=1e-6)
+    torch.testing.assert_close(st[2], torch.tensor([-1.0, 0.25, math.log(5.0), 0.0, 0.0], device="cuda"), rtol=0, atol=2e-6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,actions", [(3, 50), (2, 4000)])
+def test_history_without_lengths_and_wider_rows(mg, rows, actions):
+    """history_len NULL takes history_max entries of every row, of rows that lie further apart than that."""
+    rng = np.random.default_rng(actions)
+    wide = rng.integers(0, actions, (rows, 30)).astype(np.int32)
+    c = dict(history=wide, history_max=11, frequency=np.full(rows, 0.5, F))
+    x = logits_of(rng, rows, actions, "f32")
+    want, _, count = control_reference(x.numpy(), c)
+    assert count.sum() == 11 * rows
+    dev = {}
+    xd, out = x.cuda(), torch.empty(rows, actions, device="cuda")
+    ok(mg, mg.mg_logits_control(xd.data_ptr(), 0, actions, controls_struct(c, dev), out.data_ptr(), actions, rows, actions, None))
+    assert status(mg) == 0
+    torch.testing.assert_close(out.cpu(), torch.from_numpy(want), rtol=0, atol=0)
+
+
+@pytest.mark.gpu
 def test_rows_past_32_bit_offsets(mg):
     """The last row of a tensor of more than 2^32 bytes (and 2^31 elements)."""
     ld = 1 << 21
