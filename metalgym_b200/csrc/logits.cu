@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
         const float g = exp_fast(q) * fmaf(s1, q, sh);
         return a == act ? g + s0 : g;
     };
-    constexpr int U = 2;
+    constexpr int U = sizeof(T) == 4 ? 1 : 2;  // (two groups of fp32: 189 us at 1000 x 50001, one 178)
     for (int g0 = tid; g0 < s.groups; g0 += NT * U) {
         RawGroup<T> raw[U];
 #pragma unroll
