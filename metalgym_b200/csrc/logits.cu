@@ -443,6 +443,42 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
     const RowSpan s = row_span(x, lo, hi);
     const int tid = team_rank<NT>();
 
+    // Action a of logit l > -inf in the race: the lane's best runner, and its ratio E / e^(l - m).
+    auto enter = [&](float l, int a) {
+        const uint32_t h = race_bits(word, a);
+        // -log(1 - v): its series below 1 / 64 (the next term is 4e-6 of it), else from 1 - v
+        const float u = ((float)h + 0.5f) * 2.3283064e-10f;
+        const float time = u < 0.015625f ? u * fmaf(u, fmaf(u, 0.33333333f, 0.5f), 1.0f)
+                                         : -kLn2 * log2_fast(((float)(~h) + 0.5f) * 2.3283064e-10f);
+        Runner o;
+        o.key = fmaf(-kLn2, log2_fast(time), l);
+        o.logit = l;
+        o.bits = h;
+        o.action = a;
+        if (beats<false>(o, mine.best)) mine.best = o;
+        return time / exp_fast(below(l, mine.v.m));
+    };
+    // The warp's bound from its lanes' ratios, told to the CTA.
+    auto tighten = [&](float ratio) {
+        const float least = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(ratio)));
+        if (!(least < bound)) return false;
+        bound = least;
+        if (NT > 32 && (threadIdx.x & 31) == 0) atomicMin(&sharedBound, float_order(kLn2 * log2_fast(least) - mine.v.m));
+        return true;
+    };
+    // One action a lane sets a first bound: without one, all 16 logits of every
+    // lane would pass it in the first round (12 us of a CTA's time).
+    if (!GREEDY && s.groups >= NT) {
+        const int a = s.body + tid * kGroup;
+        const float l = r.history && t.has(a - lo) ? -INFINITY : bias_mask(r, to_f32(x[a]), a);
+        const float top = warp_max(l);
+        if (top > -INFINITY) {
+            mine.v.m = top;
+            tighten(l > -INFINITY ? fminf(enter(l, a), 3e38f) : 3e38f);
+        }
+        team_sync<NT>();
+    }
+
     // N logits (every lane of the warp calls it; -inf where a lane has none):
     // the i-th is of action at(i)
     auto take = [&](const float* l, auto at, auto count) {
@@ -492,28 +528,9 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
                 float li = l[0];
 #pragma unroll
                 for (int k = 1; k < N; k++) li = k == i ? l[k] : li;
-                const uint32_t h = race_bits(word, at(i));
-                const float e = exp_fast(below(li, mine.v.m));
-                if (li > -INFINITY && (float)(h >> 16) <= bound * 65542.6f * e) {
-                    // -log(1 - v): its series below 1 / 64 (the next term is 4e-6 of it), else from 1 - v
-                    const float u = ((float)h + 0.5f) * 2.3283064e-10f;
-                    const float time = u < 0.015625f ? u * fmaf(u, fmaf(u, 0.33333333f, 0.5f), 1.0f)
-                                                     : -kLn2 * log2_fast(((float)(~h) + 0.5f) * 2.3283064e-10f);
-                    Runner o;
-                    o.key = fmaf(-kLn2, log2_fast(time), li);
-                    o.logit = li;
-                    o.bits = h;
-                    o.action = at(i);
-                    if (beats<false>(o, mine.best)) mine.best = o;
-                    ratio = time / e;
-                }
+                if (li > -INFINITY) ratio = fminf(enter(li, at(i)), 3e38f);
             }
-            const float least = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(ratio)));
-            if (least < bound) {
-                bound = least;
-                if (NT > 32 && (threadIdx.x & 31) == 0) atomicMin(&sharedBound, float_order(kLn2 * log2_fast(least) - mine.v.m));
-                if (N > 4 && __any_sync(0xffffffffu, (pass & (pass - 1)) != 0)) pass = still(pass);
-            }
+            if (tighten(ratio) && N > 4 && __any_sync(0xffffffffu, (pass & (pass - 1)) != 0)) pass = still(pass);
         }
     };
     row_walk<T, NT, WITH>(x, r, t, s, lo, take);
