@@ -737,3 +737,19 @@ def test_two_calls_at_once_and_a_repeat(mg, rows, actions):
         for a, b in zip((*one[:-1], *two[:-1]), (*three[:-1], *four[:-1])):
             assert torch.equal(a, b)
     assert status(mg) == 0
+
+
+@pytest.mark.gpu
+def test_documented_example_runs(mg):
+    """The Python block of the integration guide: it runs, draws only allowed actions, and its gradient is finite."""
+    from pathlib import Path
+
+    text = (Path(__file__).resolve().parent.parent / "INTEGRATION.md").read_text()
+    blocks = [b.split("```")[0] for b in text.split("```python")[1:]]
+    block = next(b for b in blocks if "mg_logits_sample" in b)
+    names = {}
+    exec(compile(block, "example", "exec"), names)
+    assert status(mg) == 0
+    assert not (names["action"] % 2).any() and (names["action"] >= 0).all()
+    assert names["grad"].isfinite().all() and names["grad"].any() and names["master"].isfinite().all()
+    assert torch.equal(names["w"], names["master"].bfloat16())
