@@ -143,15 +143,15 @@ __global__ void __launch_bounds__(kPrepThreads)
     }
 }
 
-template <int KIND, int BN, bool A_MN, bool B_MN>
+template <int KIND, int BN, int BM, bool A_MN, bool B_MN>
 int launch_tiled(const CUtensorMap& ta, const CUtensorMap& tb, NsProduct p, cudaStream_t st) {
-    using S = NsTile<BN>;
-    auto kern = k_ns_product<KIND, BN, A_MN, B_MN>;
+    using S = NsTile<BN, BM>;
+    auto kern = k_ns_product<KIND, BN, BM, A_MN, B_MN>;
     static std::atomic<uint64_t> done{0};
     MG_TRY(smem_limit_once(kern, S::SMEM_BYTES, done));
-    p.tilesM = (p.M + S::BM - 1) / S::BM;
+    p.tilesM = (p.M + BM - 1) / BM;
     p.tilesN = (p.N + BN - 1) / BN;
-    const int64_t units = (int64_t)ns_tiles<KIND, BN>(p.tilesM, p.tilesN) * p.batch;
+    const int64_t units = (int64_t)ns_tiles<KIND, BN, BM>(p.tilesM, p.tilesN) * p.batch;
     if (units > INT32_MAX) return fail(MG_ERR_ARGUMENT, "newton_schulz: too many tiles");
     const int grid = (int)std::min<int64_t>(units, num_sms());
     MG_CUDA_TRY(MG_LAUNCH(kern, grid, S::THREADS, S::SMEM_BYTES, st, ta, tb, p));
@@ -184,20 +184,27 @@ int launch_split(const CUtensorMap& ta, const CUtensorMap& tb, NsProduct p, int 
     return check_launch("k_ns_split");
 }
 
-// 256-wide tiles where they fill the GPU: half the operand bytes per product
-// of 128-wide ones, which below a wave leave too many SMs idle. Few tiles split
-// a K of four blocks or more over a cluster, while the clusters fit the GPU at
-// once (measured: clusters of four on 144 of 148 SMs run in two waves).
+// Few tiles split a K of four blocks or more over a cluster, while the clusters
+// fit the GPU at once (measured: clusters of four on 144 of 148 SMs run in two
+// waves). Otherwise the tile with the fewest cycles: whole rounds over the SMs,
+// of 590, 870 and 1164 cycles a K block for 128 x 128, 128 x 256 and 256 x 256
+// (their operand bytes at the 55 a cycle that L2 gives an SM), and an epilogue
+// behind the last tile, or behind every tile of 256 x 256.
 template <int KIND, bool A_MN, bool B_MN>
 int launch_product(const CUtensorMap& ta, const CUtensorMap& tb, const NsProduct& p, cudaStream_t st) {
     const int64_t tiles = (int64_t)ns_tiles<KIND, 128>((p.M + 127) / 128, (p.N + 127) / 128) * p.batch;
-    const int blocks = (p.K + 63) / 64;
+    const int64_t sms = num_sms(), blocks = (p.K + 63) / 64;
     int splits = 1;
-    while (splits < 4 && tiles * splits * 2 <= num_sms() * 7 / 8 && blocks >= 4 && blocks >= 2 * splits) splits *= 2;
+    while (splits < 4 && tiles * splits * 2 <= sms * 7 / 8 && blocks >= 4 && blocks >= 2 * splits) splits *= 2;
     if (splits > 1) return launch_split<KIND, A_MN, B_MN>(ta, tb, p, splits, st);
     const int64_t wide = (int64_t)ns_tiles<KIND, 256>((p.M + 127) / 128, (p.N + 255) / 256) * p.batch;
-    return wide >= num_sms() ? launch_tiled<KIND, 256, A_MN, B_MN>(ta, tb, p, st)
-                             : launch_tiled<KIND, 128, A_MN, B_MN>(ta, tb, p, st);
+    const int64_t square = (int64_t)ns_tiles<KIND, 256, 256>((p.M + 255) / 256, (p.N + 255) / 256) * p.batch;
+    auto rounds = [&](int64_t n) { return (n + sms - 1) / sms; };
+    const int64_t cost128 = rounds(tiles) * 590 * blocks + 3000, costWide = rounds(wide) * 870 * blocks + 5000;
+    const int64_t costSquare = rounds(square) * (1164 * blocks + 9000);
+    if (costSquare < costWide && costSquare < cost128) return launch_tiled<KIND, 256, 256, A_MN, B_MN>(ta, tb, p, st);
+    return costWide < cost128 ? launch_tiled<KIND, 256, 128, A_MN, B_MN>(ta, tb, p, st)
+                              : launch_tiled<KIND, 128, 128, A_MN, B_MN>(ta, tb, p, st);
 }
 
 struct Workspace {

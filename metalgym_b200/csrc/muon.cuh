@@ -3,6 +3,10 @@
 // tiles with the accumulator double-buffered in tensor memory, so that the
 // epilogue of one tile runs beside the products of the next.
 //
+// (256 x 256 tiles of large matrices have one accumulator set: their operands
+// come at 64 bytes a product cycle and SM instead of 96, which L2 does not
+// sustain, and that is worth more than the overlap.)
+//
 //   kNsGram   G = X X^T or X^T X, symmetric: only tiles that reach the diagonal
 //             or lie above it are computed, and written to both places
 //   kNsPoly   B = b G + c G G, likewise symmetric
@@ -56,14 +60,17 @@ struct NsProduct {
     int* status;
 };
 
-template <int BN>
+// A tile of BM x BN, BM = 128, or 256 in two halves that share B (one
+// accumulator set: 512 columns are all of tensor memory).
+template <int BN, int BM = 128>
 struct NsTile {
-    static constexpr int BM = 128, BK = 64, STAGES = BN == 256 ? 4 : 5;
+    static constexpr int BK = 64, HALVES = BM / 128, ACCS = HALVES == 1 ? 2 : 1;
+    static constexpr int STAGES = BM == 256 ? 3 : BN == 256 ? 4 : 5;
     static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int EW = BN == 256 ? 8 : 16, THREADS = 64 + 32 * EW, SLAB = 4096;
-    static constexpr int PIECES = BN / (8 * EW);  // 32-column pieces of an epilogue warp
+    static constexpr int PIECES = BN / (8 * EW);  // 32-column pieces of an epilogue warp and half
     static constexpr int SLAB_OFF = STAGES * STAGE_BYTES, BAR_OFF = SLAB_OFF + EW * SLAB;
-    static constexpr int TMEM_COLS = 2 * BN;
+    static constexpr int TMEM_COLS = ACCS * HALVES * BN;
     static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024 /*align*/;
 };
 
@@ -81,14 +88,14 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
 
 // Tiles of one matrix, and the u-th of them; of a symmetric product only those
 // that do not lie wholly below the diagonal.
-template <int KIND, int BN>
+template <int KIND, int BN, int BM = 128>
 __host__ __device__ __forceinline__ int ns_tiles(int tilesM, int tilesN) {
     if (KIND == kNsApply) return tilesM * tilesN;
     int n = 0;
-    for (int i = 0; i < tilesM; i++) n += tilesN - i * 128 / BN;
+    for (int i = 0; i < tilesM; i++) n += tilesN - i * BM / BN;
     return n;
 }
-template <int KIND, int BN>
+template <int KIND, int BN, int BM = 128>
 __device__ __forceinline__ void ns_tile_at(int u, int tilesN, int& i, int& j) {
     if (KIND == kNsApply) {
         i = u / tilesN;
@@ -96,11 +103,11 @@ __device__ __forceinline__ void ns_tile_at(int u, int tilesN, int& i, int& j) {
         return;
     }
     i = 0;
-    while (u >= tilesN - i * 128 / BN) {
-        u -= tilesN - i * 128 / BN;
+    while (u >= tilesN - i * BM / BN) {
+        u -= tilesN - i * BM / BN;
         i++;
     }
-    j = i * 128 / BN + u;
+    j = i * BM / BN + u;
 }
 
 __device__ __forceinline__ uint32_t ns_slab_offset(int r, int k) { return (uint32_t)(r * 128 + ((k ^ (r & 7)) << 4)); }
@@ -268,28 +275,28 @@ __device__ __forceinline__ void ns_piece(const NsProduct& p, int b, int row0, in
     }
 }
 
-template <int KIND, int BN, bool A_MN, bool B_MN>
-__global__ void __launch_bounds__(NsTile<BN>::THREADS, 1)
+template <int KIND, int BN, int BM, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(NsTile<BN, BM>::THREADS, 1)
     k_ns_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const NsProduct p) {
-    using S = NsTile<BN>;
+    using S = NsTile<BN, BM>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::BAR_OFF);
     uint64_t* empty = full + S::STAGES;
-    uint64_t* tfull = empty + S::STAGES;  // [2]
-    uint64_t* tempty = tfull + 2;         // [2]
-    uint64_t* done = tempty + 2;
+    uint64_t* tfull = empty + S::STAGES;  // [ACCS]
+    uint64_t* tempty = tfull + S::ACCS;   // [ACCS]
+    uint64_t* done = tempty + S::ACCS;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     mg_pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int perMatrix = ns_tiles<KIND, BN>(p.tilesM, p.tilesN), units = perMatrix * p.batch;
+    const int perMatrix = ns_tiles<KIND, BN, BM>(p.tilesM, p.tilesN), units = perMatrix * p.batch;
     const int nk = (p.K + S::BK - 1) / S::BK;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; s++) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int a = 0; a < 2; a++) {
+        for (int a = 0; a < S::ACCS; a++) {
             mbar_init(&tfull[a], 1);
             mbar_init(&tempty[a], S::EW);
         }
@@ -315,8 +322,8 @@ __global__ void __launch_bounds__(NsTile<BN>::THREADS, 1)
             for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
                 const int b = u / perMatrix;
                 int ti, tj;
-                ns_tile_at<KIND, BN>(u - b * perMatrix, p.tilesN, ti, tj);
-                const int m0 = ti * S::BM, n0 = tj * BN;
+                ns_tile_at<KIND, BN, BM>(u - b * perMatrix, p.tilesN, ti, tj);
+                const int m0 = ti * BM, n0 = tj * BN;
                 for (int kb = 0; kb < nk; kb++, it++) {
                     const int s = it % S::STAGES;
                     if (!mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1, p.status, kDevTimeoutEmpty)) {
@@ -329,9 +336,10 @@ __global__ void __launch_bounds__(NsTile<BN>::THREADS, 1)
                     mbar_arrive_expect_tx(&full[s], S::STAGE_BYTES);
                     if (A_MN) {
 #pragma unroll
-                        for (int j = 0; j < S::BM / 64; j++) tma_load_3d(sA + j * 8192, &tmA, m0 + 64 * j, k0, b, &full[s]);
-                    } else {
-                        tma_load_3d(sA, &tmA, k0, m0, b, &full[s]);
+                        for (int j = 0; j < BM / 64; j++) tma_load_3d(sA + j * 8192, &tmA, m0 + 64 * j, k0, b, &full[s]);
+                    } else {  // boxes of 128 rows
+#pragma unroll
+                        for (int j = 0; j < S::HALVES; j++) tma_load_3d(sA + j * 16384, &tmA, k0, m0 + 128 * j, b, &full[s]);
                     }
                     if (B_MN) {
 #pragma unroll
@@ -352,10 +360,10 @@ __global__ void __launch_bounds__(NsTile<BN>::THREADS, 1)
             int it = 0, t = 0;
             bool ok = true;
             for (int u = blockIdx.x; u < units && ok; u += gridDim.x, t++) {
-                const int a = t & 1;
-                if (!mbar_wait(&tempty[a], ((t >> 1) & 1) ^ 1, p.status, kDevTimeoutEmpty)) break;
+                const int a = t % S::ACCS;
+                if (!mbar_wait(&tempty[a], ((t / S::ACCS) & 1) ^ 1, p.status, kDevTimeoutEmpty)) break;
                 tc_fence_after();
-                const uint32_t acc = tmem + (uint32_t)(a * BN);
+                const uint32_t acc = tmem + (uint32_t)(a * S::HALVES * BN);
                 for (int kb = 0; kb < nk; kb++, it++) {
                     const int s = it % S::STAGES;
                     if (!mbar_wait(&full[s], (it / S::STAGES) & 1, p.status, kDevTimeoutFull)) {
@@ -366,11 +374,15 @@ __global__ void __launch_bounds__(NsTile<BN>::THREADS, 1)
                     const uint32_t aBase = smem_u32(smem + s * S::STAGE_BYTES), bBase = aBase + S::A_BYTES;
 #pragma unroll
                     for (int kk = 0; kk < 4; kk++) {
-                        const uint64_t ad = A_MN ? smem_desc_sw128(aBase + kk * 2048, 8192, 1024)
-                                                 : smem_desc_sw128(aBase + kk * 32, 16, 1024);
                         const uint64_t bd = B_MN ? smem_desc_sw128(bBase + kk * 2048, 8192, 1024)
                                                  : smem_desc_sw128(bBase + kk * 32, 16, 1024);
-                        tc_mma_bf16(acc, ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);  // kind::f16: the types are idesc's
+#pragma unroll
+                        for (int h = 0; h < S::HALVES; h++) {
+                            const uint64_t ad = A_MN ? smem_desc_sw128(aBase + h * 16384 + kk * 2048, 8192, 1024)
+                                                     : smem_desc_sw128(aBase + h * 16384 + kk * 32, 16, 1024);
+                            // kind::f16: the types are idesc's
+                            tc_mma_bf16(acc + (uint32_t)(h * BN), ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+                        }
                     }
                     tc_commit(&empty[s]);
                 }
@@ -384,25 +396,25 @@ __global__ void __launch_bounds__(NsTile<BN>::THREADS, 1)
         uint8_t* slab = smem + S::SLAB_OFF + e * S::SLAB;
         int t = 0;
         for (int u = blockIdx.x; u < units; u += gridDim.x, t++) {
-            const int b = u / perMatrix, a = t & 1;
+            const int b = u / perMatrix, a = t % S::ACCS;
             int ti, tj;
-            ns_tile_at<KIND, BN>(u - b * perMatrix, p.tilesN, ti, tj);
-            const int row0 = ti * S::BM + 32 * q, n0 = tj * BN + part;
-            const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN + part);
+            ns_tile_at<KIND, BN, BM>(u - b * perMatrix, p.tilesN, ti, tj);
+            const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * S::HALVES * BN + part);
 #pragma unroll 1
-            for (int c = 0; c < S::PIECES; c++) {
-                const int col0 = n0 + 32 * c;
+            for (int c = 0; c < S::HALVES * S::PIECES; c++) {
+                const int h = c / S::PIECES, at = 32 * (c % S::PIECES);
+                const int row0 = ti * BM + 128 * h + 32 * q, col0 = tj * BN + part + at;
                 const bool wanted = row0 < p.M && col0 < p.N && (KIND == kNsApply || col0 >= row0);
                 NsFetched<KIND> f;
                 if (wanted) ns_fetch<KIND>(p, b, row0, col0, f);
                 if (c == 0) {
-                    if (!mbar_wait_warp(&tfull[a], (t >> 1) & 1, p.status, kDevTimeoutDone)) gaveUp = true;
+                    if (!mbar_wait_warp(&tfull[a], (t / S::ACCS) & 1, p.status, kDevTimeoutDone)) gaveUp = true;
                     if (gaveUp) break;
                     tc_fence_after();
                 }
                 float v[32];
-                tmem_ld32(acc + (uint32_t)(c * 32), v);
-                if (c == S::PIECES - 1) {  // the accumulator is free for the tile after next
+                tmem_ld32(acc + (uint32_t)(h * BN + at), v);
+                if (c == S::HALVES * S::PIECES - 1) {  // the accumulator is free for the next tile that uses it
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&tempty[a]);

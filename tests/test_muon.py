@@ -138,6 +138,23 @@ def test_orthogonalize(mg, batch, m, n, spectrum):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch,m,n,steps", [(8, 1024, 1030, 2), (8, 1100, 1000, 2), (1, 1500, 2600, 2), (1, 2500, 1700, 2), (6, 520, 1300, 3)])
+def test_matrices_of_many_tiles(mg, batch, m, n, steps):
+    """Enough tiles for every tile shape and several to a CTA, edges inside them."""
+    gen = torch.Generator(device="cuda").manual_seed(m * n + steps)
+    x = torch.randn(batch, m, n, generator=gen, device="cuda")
+    space = workspace(mg, batch, m, n)
+    out = torch.empty(batch, m, n, dtype=torch.float16, device="cuda")
+    ok(mg, mg.mg_orthogonalize(x.data_ptr(), 0, n, m * n, out.data_ptr(), 2, n, m * n, batch, m, n, steps, space.data_ptr(), space.numel(), None))
+    assert status(mg) == 0
+    for i in range(0, batch, max(1, batch - 1)):
+        want = newton_schulz(x[i], steps, False)
+        off = (out[i].double() - want).abs()
+        assert off.norm() <= allowance(x[i], want, steps) + 2.0 ** -12 * want.norm()
+        assert off.max() <= 0.05 * want.abs().max()  # no tile is wrong or missing
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("batch,m,n,steps", [(2, 128, 512, 7), (1, 40, 200, 8), (3, 100, 30, 7), (1, 1, 9, 7), (1, 128, 128, 10), (2, 24, 24, 16)])
 def test_many_steps_of_small_matrices(mg, batch, m, n, steps):
     """More steps than the one-kernel form takes: the tiled products at small sizes."""
