@@ -327,6 +327,7 @@ __device__ inline void row_merge(RowPart& mine, RowPart* warps, int parts, int c
     static_assert(NT == 32 || W == 8, "eight warps a CTA: up to two slots a lane");
     const int lane = threadIdx.x & 31;
     if (lane == 0) warps[threadIdx.x >> 5] = mine;
+    __syncwarp();  // (the cluster's barrier takes whole warps)
     if (parts == 1)
         __syncthreads();
     else
@@ -551,6 +552,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
         if (value) value[row] = to_f32(x[part.actions]);
         if (!GREEDY) rng[row] = word;
     }
+    __syncwarp();
     if (NT > 32 && part.parts > 1) cluster_sync();
 }
 
@@ -631,12 +633,13 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
     const float one = ratio * adv, two = fminf(fmaxf(ratio, 1.0f - L.clip), 1.0f + L.clip) * adv;
     const float slope = one <= two ? -adv * ratio : 0.0f;
     // every thread has read the action's logit: the gradient may take its place
-    if (NT == 32)
-        __syncwarp();
-    else if (part.parts > 1)
-        cluster_sync();
-    else
-        __syncthreads();
+    __syncwarp();
+    if (NT > 32) {
+        if (part.parts > 1)
+            cluster_sync();
+        else
+            __syncthreads();
+    }
     if (mine.chosen == -INFINITY) {  // an action that the policy never takes
         leaveOut();
         return;

@@ -247,6 +247,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
     auto wait = [&](int i) {
         mbar_wait(&bar[i], phase[i], p.status, kDevTimeoutDone);
         phase[i] ^= 1u;
+        __syncwarp();  // loads from tensor memory take whole warps
         tc_fence_after();
     };
     // what the threads wrote to shared memory and read from tensor memory, before the next products
@@ -305,6 +306,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
         for (int w = 1; w < WARPS; w++) sum += sSum[w];
         *sNorm = sum;
     }
+    __syncwarp();
     if (parts > 1) {
         cluster_sync();
         sum = 0.0;
@@ -364,6 +366,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
     if (parts > 1) {
         // CTA k sums rows k SP / parts .. of all parts, in their order, and hands
         // them back to all: nobody else reads or writes those rows meanwhile
+        __syncwarp();
         cluster_sync();
         const int mine = SP / parts;
         for (int j = tid; j < mine * SP / 4; j += kMuonSmallThreads) {
@@ -385,6 +388,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
             for (int k = 0; k < kMuonSmallCluster; k++)
                 if (k < parts) *reinterpret_cast<float4*>(const_cast<uint8_t*>(cluster_peer(mG, k)) + off) = t;
         }
+        __syncwarp();
         cluster_sync();
     } else {
         __syncthreads();
