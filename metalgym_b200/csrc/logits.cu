@@ -499,7 +499,10 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
         auto raised = [&](float f) { bound = f > 0.0f ? fminf(bound / f, 3e38f) : 3e38f; };
         const bool some = softmax_group<N>(mine.v, l, raised, [&](int i, float e) {
             if (i == 0) {
-                if (NT > 32) bound = fminf(bound, exp_fast(ordered_float(*(volatile int*)&sharedBound) + mine.v.m));
+                if (NT > 32) {  // (3e-7 |m|: the roundings of the sums with m, so that the bound is never too low)
+                    const float other = ordered_float(*(volatile int*)&sharedBound) + mine.v.m;
+                    bound = fminf(bound, exp_fast(fmaf(3e-7f, fabsf(mine.v.m), other)));
+                }
                 limit = fminf(bound * 65542.6f, 3e38f);  // 2^16 (1 + 1e-4)
             }
             uint32_t h = word + (uint32_t)at(i) * 0x9E3779B9u;

@@ -370,6 +370,22 @@ def test_draws_follow_the_softmax(mg, actions):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("offset", [0.0, 3000.0, -65536.0])
+def test_draws_at_large_offsets(mg, offset):
+    """A common offset of the logits (which fp32 still resolves) moves no draw: the definition's winner in 64 bits."""
+    rng = np.random.default_rng(4)
+    rows, actions = 400, 9000
+    x = (rng.integers(-800, 800, (rows, actions)) / 128.0 + offset).astype(F)  # exact in fp32 at every offset
+    words = rng.integers(1, 1 << 32, rows, dtype=np.uint64)
+    xd, rd = torch.from_numpy(x).cuda(), torch.from_numpy(words.astype(np.uint32).view(np.int32).copy()).cuda()
+    act, lp = torch.empty(rows, dtype=torch.int32, device="cuda"), torch.empty(rows, device="cuda")
+    ok(mg, mg.mg_logits_sample(xd.data_ptr(), 0, actions, None, rd.data_ptr(), act.data_ptr(), lp.data_ptr(), None, None, rows, actions, None))
+    assert status(mg) == 0
+    want = (x.astype(np.float64) - np.log(race(next_word(words), actions))).argmax(1)
+    assert np.array_equal(act.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
 def test_nan_and_minus_infinity_at_allowed_actions(mg):
     x = torch.zeros(4, 40, device="cuda")
     x[0, 7] = math.nan
