@@ -649,7 +649,8 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
     }
     // dl = scale (slope (1[a = act] - p) + ent p (ln p + H)) = p (s1 log p + (ent H - slope) scale), + s0 at act
     const float s0 = slope * L.scale, s1 = L.entropyCoef * L.scale, sh = fmaf(L.entropyCoef * L.scale, entropy, -s0);
-    const bool vec = same_alignment(x, d), all_nan = !(fabsf(sh) < INFINITY && fabsf(s1) < INFINITY);
+    // (1e8: times the bounded logarithm, 1e30, a larger s1 could overflow, and 0 times that is NaN)
+    const bool vec = same_alignment(x, d), all_nan = !(fabsf(sh) < INFINITY && fabsf(s1) < 1e8f);
     auto gradient = [&](float l, int a) {
         const float q = below(l, m) - ls;
         const float g = exp_fast(q) * fmaf(s1, q, sh);

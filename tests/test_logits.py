@@ -639,6 +639,27 @@ def test_loss_leaves_out_actions_of_logit_minus_infinity(mg, actions):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("actions", [5, 2000])
+def test_masked_gradients_are_zero_for_large_coefficients(mg, actions):
+    """An entropy coefficient whose product with a masked action's logarithm overflows: zeros there all the same, and in
+    a uniform row 0 at the others but for the roundings of p (ln p + H): 8 steps of the logarithm, times the coefficient."""
+    mask = np.zeros((1, (actions + 31) // 32), np.uint32)
+    mask[0, 0] = 0b1011
+    dev = {}
+    cs = controls_struct(dict(mask=mask), dev)
+    x = torch.zeros(2, actions, device="cuda")
+    action, zero = torch.tensor([0, 3], dtype=torch.int32, device="cuda"), torch.zeros(2, device="cuda")
+    d, st = torch.full((2, actions), 7.0, device="cuda"), torch.empty(2, 5, device="cuda")
+    ok(mg, mg.mg_logits_policy_loss(x.data_ptr(), 0, actions, cs, action.data_ptr(), zero.data_ptr(), None, None, zero.data_ptr(),
+                                    d.data_ptr(), actions, st.data_ptr(), 2, actions, 0.2, 0.5, 1e9, 1.0, None))
+    assert status(mg) == 0
+    allowed = torch.zeros(actions, dtype=torch.bool, device="cuda")
+    allowed[[0, 1, 3]] = True
+    assert not d[:, ~allowed].any()
+    assert (d[:, allowed].abs() <= 1e9 * 8 * 2.0 ** -23 * math.log(3.0)).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,actions", [(3, 50), (2, 4000)])
 def test_history_without_lengths_and_wider_rows(mg, rows, actions):
     """history_len NULL takes history_max entries of every row, of rows that lie further apart than that."""
