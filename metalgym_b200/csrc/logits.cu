@@ -970,6 +970,8 @@ int mg_logits_sample(const void* logits, int dtype, int64_t ld, const mg_logit_c
     mg_logit_controls c;
     MG_TRY(check_common("logits_sample", logits, dtype, ld, controls, rows, actions, actions + (value ? 1 : 0), &c));
     MG_CHECK_ARG(action && log_prob, "logits_sample: null action or log_prob");
+    MG_CHECK_ARG(aligned(rng, 4) && aligned(action, 4) && aligned(log_prob, 4) && aligned(entropy, 4) && aligned(value, 4),
+                 "logits_sample: a buffer is not aligned to its type");
     return MG_BY_TYPE(dtype, sample)(logits, ld, c, rng, action, log_prob, entropy, value, rows, actions,
                                             reinterpret_cast<cudaStream_t>(stream));
 }
@@ -982,6 +984,9 @@ int mg_logits_policy_loss(const void* logits, int dtype, int64_t ld, const mg_lo
     const int columns = actions + (ret ? 1 : 0);
     MG_TRY(check_common("logits_policy_loss", logits, dtype, ld, controls, rows, actions, columns, &c));
     MG_CHECK_ARG(action && adv && old_log_prob && stats, "logits_policy_loss: null argument");
+    MG_CHECK_ARG(aligned(action, 4) && aligned(adv, 4) && aligned(adv_stats, 4) && aligned(ret, 4) && aligned(old_log_prob, 4) &&
+                     aligned(stats, 4),
+                 "logits_policy_loss: a buffer is not aligned to its type");
     MG_CHECK_ARG(d_logits && aligned(d_logits, type_size(dtype)), "logits_policy_loss: null or misaligned d_logits");
     MG_CHECK_ARG(ldd >= columns, "logits_policy_loss: ldd smaller than the row");
     MG_CHECK_ARG(d_logits != logits || ldd == ld, "logits_policy_loss: in place needs ldd = ld");

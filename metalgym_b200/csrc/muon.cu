@@ -432,8 +432,9 @@ int mg_muon_step(float* master, const float* grad, float* momentum, void* weight
                  void* workspace, size_t workspace_bytes, mg_stream_t stream) {
     MG_CHECK_ARG(master && grad && momentum && weights, "muon_step: null argument");
     MG_TRY(check_shape("muon_step", batch, rows, cols));
-    MG_CHECK_ARG(aligned_to(master, 4) && aligned_to(grad, 4) && aligned_to(momentum, 4) && aligned_to(weights, 2),
-                 "muon_step: a matrix is not aligned to its type");
+    MG_CHECK_ARG(aligned_to(master, 4) && aligned_to(grad, 4) && aligned_to(momentum, 4) && aligned_to(weights, 2) &&
+                     aligned_to(norm_partial, 4) && aligned_to(norm_sq_out, 4),
+                 "muon_step: a buffer is not aligned to its type");
     MG_CHECK_ARG(batch == 1 || batch_stride >= (int64_t)rows * cols, "muon_step: the matrices of the batch overlap");
     MG_CHECK_ARG(n_norm_partials >= 0 && (norm_partial || n_norm_partials == 0), "muon_step: null norm_partial");
     MG_CHECK_ARG(n_norm_partials > 0 || (!(max_grad_norm > 0.0f) && !norm_sq_out),

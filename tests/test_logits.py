@@ -176,6 +176,20 @@ def test_bad_arguments_are_refused(name):
         assert getattr(lib, name)(*dict(good_call(name), controls=ctypes.byref(c)).values()) == 1, spoil
 
 
+@pytest.mark.parametrize("name", ["mg_logits_sample", "mg_logits_policy_loss"])
+def test_misaligned_buffers_are_refused(name):
+    import metalgym_b200
+
+    lib = metalgym_b200.lib()
+    keys = dict(mg_logits_sample=["rng", "action", "log_prob", "entropy", "value"],
+                mg_logits_policy_loss=["action", "adv", "adv_stats", "ret", "old", "stats", "d_logits"])[name]
+    for key in keys:
+        args = good_call(name)
+        args[key] = (1 << 22) + 1
+        assert getattr(lib, name)(*args.values()) == 1, key
+        assert b"aligned" in lib.mg_last_error()
+
+
 def test_controls_layout_matches_the_header(tmp_path):
     """The ctypes structure has the C struct's size and offsets."""
     import subprocess

@@ -107,6 +107,14 @@ def test_bad_arguments_are_refused():
         assert lib.mg_last_error()
 
 
+def test_misaligned_norms_are_refused():
+    import metalgym_b200
+
+    for spoil in (dict(norms=(1 << 22) + 2), dict(norm_out=(1 << 22) + 1)):
+        assert metalgym_b200.lib().mg_muon_step(*dict(bad_step(), **spoil).values()) == 1, spoil
+        assert b"aligned" in metalgym_b200.lib().mg_last_error()
+
+
 SHAPES = [(1, 1, 1), (2, 1, 77), (1, 300, 1), (3, 5, 100), (2, 64, 64), (1, 65, 63), (4, 128, 512), (4, 512, 128), (2, 127, 129),
           (1, 129, 127), (1, 128, 1000), (2, 333, 1001), (1, 1001, 333), (1, 256, 1024), (2, 200, 40), (1, 640, 640), (9, 16, 24)]
 
