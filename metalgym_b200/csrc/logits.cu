@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : kControlCtas)
     HistoryTable t = team_table<NT>(part, c, smem);
     auto run = [&](int row, int lo, int hi) {
         const T* x = logits + (int64_t)row * ld;
-        control_part<T, NT, BACKWARD, WITH>(x, BACKWARD ? dOut + (int64_t)row * ldg : x, out + (int64_t)row * ldo, row_controls(c, row),
+        control_part<T, NT, BACKWARD, WITH>(x, BACKWARD ? dOut + (int64_t)row * ldg : x, out + (int64_t)row * ldo, row_controls(c, row, part.actions),
                                       t, c, row, lo, hi, sums);
     };
     if (NT == 32) {
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
     RowPart* warps = reinterpret_cast<RowPart*>(slots);
     int row, lo, hi;
     if (!team_part<NT>(part, row, lo, hi)) return;
-    const RowControls r = row_controls(c, row);
+    const RowControls r = row_controls(c, row, part.actions);
     HistoryTable t = team_table<NT>(part, c, smem);
     if (r.history)
         history_fill<NT>(t, c.history + (int64_t)row * c.history_stride, row_history_len(c, row), lo, hi, c.history_max, sums);
@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
     int row, lo, hi;
     if (!team_part<NT>(part, row, lo, hi)) return;
     const int actions = part.actions, tid = team_rank<NT>();
-    const RowControls r = row_controls(c, row);
+    const RowControls r = row_controls(c, row, part.actions);
     HistoryTable t = team_table<NT>(part, c, smem);
     const T* x = logits + (int64_t)row * ld;
     T* d = dLogits + (int64_t)row * ldd;
