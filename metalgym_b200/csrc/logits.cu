@@ -18,11 +18,10 @@
 namespace mg {
 namespace {
 
-// A team reads one row, or one part of it: a warp (eight rows a CTA) up to
-// kWarpActions actions, else a CTA of NT threads, with the row's parts in the
+// A team reads one row, or one part of it: a warp (eight rows a CTA) where rows
+// are short and many, else a CTA of NT threads, with the row's parts in the
 // CTAs of a cluster where rows are few or so long that the rows being read
 // would not stay in L2 for the loss's second pass.
-constexpr int kWarpActions = 1024;
 constexpr int kWarpRows = 8;  // rows of a CTA of warp teams
 
 template <int NT>
@@ -778,7 +777,7 @@ size_t table_smem(const TeamPart& p) {
     return (size_t)p.tableBytes * (NT == 32 ? kWarpRows : 1);
 }
 
-// the largest table (2^18 actions, 2^14 entries); eight of kWarpActions actions take less
+// the largest table (2^18 actions, 2^14 entries); a CTA's eight of warp teams take less
 constexpr int kTableSmemMax = 216 * 1024;
 
 // A launch of rows x parts CTAs (or warp teams), the parts of a row in one cluster.
@@ -817,8 +816,24 @@ int row_parts(int rows, int actions, int size, int nt, bool twice) {
     return parts;
 }
 
+// Whether a warp takes a row. A CTA spends about 3000 instructions on a row
+// whatever its length (merging warps, barriers), a warp waits out its loads one
+// after the other: up to 256 actions a warp is never slower; longer rows take a
+// CTA while CTAs have SMs of their own (draw of 256 x 1000 with all controls:
+// 15.2 us, 20.5 by warps), and a warp where rows are many for their length
+// (8000 x 2048, draw 49 us, 90 by CTAs; control 45 / 72; loss 41 / 55; but
+// 1024 x 4096, loss 18.4 / 16.4, control 24.6 / 20.5), unless the eight history tables
+// would leave an SM few warps.
+bool warp_teams(int rows, int actions, int historyMax, bool loss) {
+    if (actions <= 256) return true;
+    if (rows <= 4 * num_sms()) return false;
+    if (actions <= 1024) return true;
+    const int64_t most = loss ? std::min<int64_t>(rows / 2, 2816) : std::min<int64_t>(2 * (int64_t)rows, 4096);
+    return actions <= most && (!historyMax || HistoryTable::bytes(actions, historyMax) * kWarpRows <= 40 * 1024);
+}
+
 // The compiled controls that a call needs; `history`: the pass leaves out the
-// actions that occurred. Small action sets take the kernel with all of them.
+// actions that occurred. Warp teams take the kernel with all of them.
 int needed_controls(const mg_logit_controls& c, bool history) {
     return (c.bias ? kWithBias : 0) | (c.mask || (history && c.history) ? kWithMask : 0);
 }
@@ -847,7 +862,7 @@ template <class T, bool BACKWARD>
 int control(const void* logits, int64_t ld, const mg_logit_controls& c, const void* dOut, int64_t ldg, void* out, int64_t ldo,
             int rows, int actions, cudaStream_t st) {
     auto f = launch_control<T, 32, BACKWARD, BACKWARD ? kWithMask : kWithBias | kWithMask>;
-    if (actions > kWarpActions) {
+    if (!warp_teams(rows, actions, c.history ? c.history_max : 0, false)) {
         switch (needed_controls(c, false)) {
             case 0: f = launch_control<T, 256, BACKWARD, 0>; break;
             case kWithMask: f = launch_control<T, 256, BACKWARD, kWithMask>; break;
@@ -874,7 +889,7 @@ template <class T, bool GREEDY>
 int sample_rows(const void* logits, int64_t ld, const mg_logit_controls& c, uint32_t* rng, int32_t* action, float* logProb,
                 float* entropy, float* value, int rows, int actions, cudaStream_t st) {
     auto f = launch_sample<T, 32, GREEDY, 3>;
-    if (actions > kWarpActions) {
+    if (!warp_teams(rows, actions, c.history_max, false)) {
         switch (needed_controls(c, true)) {
             case 0: f = launch_sample<T, 256, GREEDY, 0>; break;
             case 1: f = launch_sample<T, 256, GREEDY, 1>; break;
@@ -906,7 +921,7 @@ template <class T>
 int loss(const void* logits, int64_t ld, const mg_logit_controls& c, void* d, int64_t ldd, int rows, int actions,
          const LossArgs& L, cudaStream_t st) {
     auto f = launch_loss<T, 32, 3>;
-    if (actions > kWarpActions) {
+    if (!warp_teams(rows, actions, c.history_max, true)) {
         switch (needed_controls(c, true)) {
             case 0: f = launch_loss<T, 256, 0>; break;
             case 1: f = launch_loss<T, 256, 1>; break;

@@ -556,6 +556,17 @@ def test_policy_loss(mg, rows, actions, pad, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,actions,pad", [(640, 1000, 3), (1300, 2100, 1), (2400, 1100, 5)])
+def test_many_rows(mg, monkeypatch, rows, actions, pad, kind):
+    """So many rows that a warp takes each."""
+    monkeypatch.setitem(globals(), "KINDS", [KINDS[0], KINDS[3]])
+    test_control_and_gradient(mg, rows, actions, pad, kind)
+    test_sample(mg, rows, actions, pad, kind)
+    test_policy_loss(mg, rows, actions, pad, kind)
+
+
+@pytest.mark.gpu
 def test_loss_gradient_against_differences(mg):
     """d(sum of row losses) / d(raw logit) by central differences of the 64-bit loss, penalties included."""
     rng = np.random.default_rng(9)
