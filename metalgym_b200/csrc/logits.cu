@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 5)
         const float g = exp_fast(q) * fmaf(s1, q, sh);
         return a == act ? g + s0 : g;
     };
-    constexpr int U = sizeof(T) == 4 ? 1 : 2;  // (two groups of fp32: 189 us at 1000 x 50001, one 178)
+    constexpr int U = sizeof(T) == 4 ? 1 : 2;  // (two groups of fp32: 176 us at 1000 x 50001, one 153)
     for (int g0 = tid; g0 < s.groups; g0 += NT * U) {
         RawGroup<T> raw[U];
 #pragma unroll
@@ -806,7 +806,7 @@ int launch_rows(void (*kern)(KArgs...), const TeamPart& p, cudaStream_t st, cons
 // Parts of a row for the calls that need the whole row's statistics: more
 // while the CTAs do not fill the GPU (and a part keeps 4096 actions), and, for
 // the loss, so many that the rows in flight stay in L2 for its second pass (1000 x 50001
-// fp32: 220 us at four parts, 188 at two, 228 at one, whose rows are 118 MB).
+// fp32: 185 us at four parts, 153 at two, 175 at one, whose rows are 118 MB).
 int row_parts(int rows, int actions, int size, int nt, bool twice) {
     int parts = 1;
     const int fill = 4 * num_sms();
