@@ -407,6 +407,7 @@ __global__ void __launch_bounds__(NsTile<BN, BM>::THREADS, 1)
                 const bool wanted = row0 < p.M && col0 < p.N && (KIND == kNsApply || col0 >= row0);
                 NsFetched<KIND> f;
                 if (wanted) ns_fetch<KIND>(p, b, row0, col0, f);
+                __syncwarp();  // lanes at a matrix's edge took other branches; loads from tensor memory take whole warps
                 if (c == 0) {
                     if (!mbar_wait_warp(&tfull[a], (t / S::ACCS) & 1, p.status, kDevTimeoutDone)) gaveUp = true;
                     if (gaveUp) break;
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(NsTile<BN, BM>::THREADS, 1)
     tc_fence_before();
     __syncthreads();
     if (warp == 2) {
-        mbar_wait(done, 0, p.status, kDevTimeoutDone);
+        mbar_wait_warp(done, 0, p.status, kDevTimeoutDone);
         tc_fence_after();
         tmem_dealloc(tmem, S::TMEM_COLS);
     }
@@ -598,11 +599,12 @@ __global__ void __launch_bounds__(NsTile<128>::THREADS, 1)
             }
         }
     }
+    __syncwarp();    // (the cluster's barrier takes whole warps)
     cluster_sync();  // no CTA leaves while another reads its slabs
     tc_fence_before();
     __syncthreads();
     if (warp == 2) {
-        mbar_wait(done, 0, p.status, kDevTimeoutDone);
+        mbar_wait_warp(done, 0, p.status, kDevTimeoutDone);
         tc_fence_after();
         tmem_dealloc(tmem, 128);
     }

@@ -503,6 +503,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
         const int row0 = 32 * q + (WIDE ? 0 : 128 * i), c = 32 * (warp >> 2), col0 = c + (WIDE ? 128 * i : 0);
         if (row0 < rows && c < N && col0 < cols && (!WIDE || 32 * q < SP)) {
             float v[32];
+            __syncwarp();  // the first warp's lane 0 issued the next product
             tmem_ld32(acc + (uint32_t)(128 * k + c), v);
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] *= 32.0f;  // to the scale of ns_piece, 2^20
@@ -512,6 +513,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
     tc_fence_before();
     __syncthreads();
     if (warp == 2) {
+        __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem, 256);
     }

@@ -203,6 +203,23 @@ def test_small_side_is_as_exact_as_fp32(mg, batch, m, n, spectrum):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("batch,m,n", [(1, 130, 300), (1, 333, 1001), (40, 161, 200), (3, 200, 1100), (1, 1030, 1500), (2, 129, 133), (1, 100, 700)])
+def test_pieces_that_end_inside_a_warp(mg, batch, m, n):
+    """Matrices whose last 32 x 32 pieces and mirrored pieces hold fewer rows than a warp has lanes, by every kind of
+    product: the same bits every time, which are the result's (1.5 times the distance of the emulated roundings)."""
+    gen = torch.Generator(device="cuda").manual_seed(m + n)
+    x = torch.randn(batch, m, n, generator=gen, device="cuda")
+    space = workspace(mg, batch, m, n)
+    outs = [torch.empty(batch, m, n, dtype=torch.float16, device="cuda") for _ in range(20)]
+    for out in outs:
+        ok(mg, mg.mg_orthogonalize(x.data_ptr(), 0, n, m * n, out.data_ptr(), 2, n, m * n, batch, m, n, 3, space.data_ptr(), space.numel(), None))
+    assert status(mg) == 0
+    assert all(torch.equal(out, outs[0]) for out in outs)
+    want = newton_schulz(x[0], 3, False)
+    assert (outs[0][0].double() - want).norm() <= allowance(x[0], want, 3) + 2.0 ** -12 * want.norm()
+
+
+@pytest.mark.gpu
 def test_singular_values_come_near_one(mg):
     """Five steps take a well-spread spectrum into [0.6, 1.25] (the quintic's band [0.68, 1.21] and 0.3 % for the roundings)."""
     gen = torch.Generator(device="cuda").manual_seed(1)
