@@ -727,6 +727,13 @@ int type_size(int dtype) { return dtype == MG_DTYPE_F32 ? 4 : 2; }
 bool type_ok(int dtype) { return dtype == MG_DTYPE_F32 || dtype == MG_DTYPE_BF16 || dtype == MG_DTYPE_F16; }
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % (unsigned)bytes) == 0; }
 
+// Without its history a call has no tables either: their size goes by history_max.
+void leave_out_history(mg_logit_controls* c) {
+    c->history = nullptr;
+    c->history_len = nullptr;
+    c->history_max = 0;
+}
+
 // Checks what every call shares and copies the controls; a history that no
 // penalty reads is left out.
 int check_common(const char* name, const void* logits, int dtype, int64_t ld, const mg_logit_controls* controls, int rows,
@@ -753,11 +760,7 @@ int check_common(const char* name, const void* logits, int dtype, int64_t ld, co
                      aligned(c.presence, 4),
                  n + ": a control's buffer is not aligned to its type");
     *out = c;
-    if (!c.repetition && !c.frequency && !c.presence) out->history = nullptr;
-    if (!out->history) {
-        out->history_len = nullptr;
-        out->history_max = 0;
-    }
+    if (!c.history || (!c.repetition && !c.frequency && !c.presence)) leave_out_history(out);
     return MG_OK;
 }
 
@@ -851,7 +854,7 @@ int launch_control(const void* logits, int64_t ld, const mg_logit_controls& c, c
         const int64_t units = (int64_t)rows * p.parts;
         ctas = std::min(units, (int64_t)num_sms() * kControlCtas);
         p.span = (int)std::min((int64_t)actions, (units + ctas - 1) / ctas * kUnit);
-        p.tableBytes = c.history ? (int)HistoryTable::bytes(p.span, c.history_max) : 0;
+        p.tableBytes = c.history_max ? (int)HistoryTable::bytes(p.span, c.history_max) : 0;
     }
     MG_CUDA_TRY(MG_LAUNCH(kern, (unsigned)ctas, kCtaThreads<NT>, table_smem<NT>(p), st, static_cast<const T*>(logits), ld, c,
                           static_cast<const T*>(dOut), ldg, static_cast<T*>(out), ldo, p));
@@ -862,7 +865,7 @@ template <class T, bool BACKWARD>
 int control(const void* logits, int64_t ld, const mg_logit_controls& c, const void* dOut, int64_t ldg, void* out, int64_t ldo,
             int rows, int actions, cudaStream_t st) {
     auto f = launch_control<T, 32, BACKWARD, BACKWARD ? kWithMask : kWithBias | kWithMask>;
-    if (!warp_teams(rows, actions, c.history ? c.history_max : 0, false)) {
+    if (!warp_teams(rows, actions, c.history_max, false)) {
         switch (needed_controls(c, false)) {
             case 0: f = launch_control<T, 256, BACKWARD, 0>; break;
             case kWithMask: f = launch_control<T, 256, BACKWARD, kWithMask>; break;
@@ -970,7 +973,7 @@ int mg_logits_control_backward(const void* logits, int dtype, int64_t ld, const 
     MG_CHECK_ARG(d_logits != logits || ldd == ld, "logits_control_backward: in place needs ldd = ld");
     // only the repetition penalty and the mask reach the gradient
     c.bias = nullptr;
-    if (!c.repetition) c.history = nullptr;
+    if (!c.repetition) leave_out_history(&c);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (dtype == MG_DTYPE_F32)
         return control<float, true>(logits, ld, c, d_out, ldg, d_logits, ldd, rows, actions, st);

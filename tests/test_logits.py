@@ -255,6 +255,29 @@ def test_control_and_gradient(mg, rows, actions, pad, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,actions,history", [(2048, 4096, 4096), (1500, 3000, 4100), (4096, 4096, 2048), (700, 1000, 16000)])
+def test_gradient_of_a_history_without_repetition(mg, rows, actions, history, kind):
+    """Frequency and presence penalties have derivative 1: the gradient passes through, masked or not, whatever the history's
+    length; no table is made for it."""
+    code, dtype = TYPES[kind]
+    rng = np.random.default_rng(actions)
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x, dy = (torch.randn(rows, actions, generator=g, device="cuda").to(dtype) for _ in range(2))
+    c = make_controls(rng, rows, actions, ("mask",))
+    c["history"] = rng.integers(0, actions, (rows, history)).astype(np.int32)
+    c["frequency"] = c["presence"] = np.full(rows, 0.5, F)
+    dev = {}
+    cs = controls_struct(c, dev)
+    bits = np.unpackbits(c["mask"].view(np.uint8), axis=1, bitorder="little")[:, :actions].astype(bool)
+    want = torch.where(torch.from_numpy(bits).cuda(), dy, torch.zeros((), dtype=dtype, device="cuda"))
+    dx = torch.full((rows, actions), 7.0, dtype=dtype, device="cuda")
+    ok(mg, mg.mg_logits_control_backward(x.data_ptr(), code, actions, cs, dy.data_ptr(), actions, dx.data_ptr(), actions, rows, actions, None))
+    assert status(mg) == 0
+    assert torch.equal(dx, want)
+
+
+@pytest.mark.gpu
 def test_longest_history_and_largest_action_set(mg):
     """The limits: 2^18 actions and 2^14 entries, one action taking every entry."""
     actions, h = 1 << 18, 1 << 14
