@@ -40,6 +40,7 @@ int fail(int code, const std::string& msg) {
 }
 
 int cuda_fail(cudaError_t e, const char* what) {
+    cudaGetLastError();  // reported here: not once more by the next launch's check (errors that end the context stay)
     return fail(MG_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 

@@ -364,6 +364,28 @@ def test_captured_step_replays(mg, m, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n", [(64, 200), (200, 300)])
+def test_step_after_a_refused_call(mg, m, n):
+    """The error of a call that the runtime refused (host memory that no machine has) is that call's alone: the step behind
+    it does what it does without it, and not the momentum alone."""
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    start = [torch.randn(1, m, n, generator=gen, device="cuda") for _ in range(3)]
+    space, results = workspace(mg, 1, m, n), []
+    for refused in (False, True):
+        master, grad, momentum = (t.clone() for t in start)
+        weights = master.bfloat16()
+        if refused:
+            at = ctypes.c_void_p()
+            assert mg.mg_host_alloc(1 << 60, ctypes.byref(at)) == 2 and mg.mg_last_error()
+        ok(mg, mg.mg_muon_step(master.data_ptr(), grad.data_ptr(), momentum.data_ptr(), weights.data_ptr(), m * n, 1, m, n, None, 0, 0.0, 0.01,
+                               1.0, 0.9, 1, 0.1, 5, None, space.data_ptr(), space.numel(), None))
+        assert status(mg) == 0
+        results.append((master, momentum, weights))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
 def test_two_streams_two_workspaces_and_a_graph(mg):
     """Two calls at once with a workspace each, and a captured graph replayed beside one of them: the same bits as alone."""
     gen = torch.Generator(device="cuda").manual_seed(3)
