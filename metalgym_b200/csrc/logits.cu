@@ -510,7 +510,8 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
             h ^= h >> 15;
             h *= 0x846ca68bu;
             const float f = __uint_as_float(__byte_perm(h, 0x4B000000u, 0x7632));
-            if (f <= fmaf(limit, e, 8388608.0f)) pass |= 1u << i;
+            // (negated: the weight of a +infinity is NaN, and it passes)
+            if (!(f > fmaf(limit, e, 8388608.0f))) pass |= 1u << i;
         });
         // the lanes' candidates, one a lane at a time, each against the bound that the ones before it left
         auto still = [&](uint32_t bits) {  // those of them that pass under the bound as it is now
@@ -519,7 +520,7 @@ __global__ void __launch_bounds__(kCtaThreads<NT>, NT == 32 ? 1 : 4)
 #pragma unroll
             for (int i = 0; i < N; i++) {
                 const float f = (float)(race_bits(word, at(i)) >> 16), e = exp_fast(below(l[i], mine.v.m));
-                if (f <= now * e) out |= 1u << i;
+                if (!(f > now * e)) out |= 1u << i;
             }
             return out & bits;
         };

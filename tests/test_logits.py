@@ -441,6 +441,49 @@ def test_nan_and_minus_infinity_at_allowed_actions(mg):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("rows,actions,pad", [(24, 3, 0), (24, 40, 1), (24, 3000, 3), (8, 131072, 0), (3000, 1500, 5)])
+def test_plus_infinity_at_allowed_actions(mg, kind, rows, actions, pad):
+    """The largest l - log E is an allowed +infinity, the lowest of several: in the vector groups, at a row's edges, among
+    the actions that occurred, beside NaN and masked infinities, as head GEMMs that overflow leave them. The statistics
+    are NaN. Rows without one draw as ever."""
+    code, dtype = TYPES[kind]
+    rng = np.random.default_rng(actions)
+    ld = actions + pad
+    places = sorted({0, 1, 2, actions // 2, actions // 2 + 1, actions - 2, actions - 1, int(rng.integers(0, actions))} & set(range(actions)))
+    for kinds in ((), ("mask", "bias", "history")):
+        c = make_controls(rng, rows, actions, kinds)
+        x = logits_of(rng, rows, ld, kind)
+        for r in range(rows):
+            if r % 5 == 4:
+                continue
+            at = rng.choice(places, size=1 + r % 5 % 3, replace=False) if len(places) > 2 else [places[r % len(places)]]
+            if kinds and r % 2:
+                at = [int(c["history"][r, 0])]  # one that occurred, where the history has an entry
+            x[r, list(at)] = math.inf
+            if r % 7 == 3:
+                x[r, (int(at[0]) + 1) % actions] = math.nan
+        l, _, _ = control_reference(x[:, :actions].float().numpy(), c)
+        dev = {}
+        cs = controls_struct(c, dev)
+        xd = x.cuda()
+        words = rng.integers(1, 1 << 32, rows, dtype=np.uint64)
+        rd = torch.from_numpy(words.astype(np.uint32).view(np.int32).copy()).cuda()
+        act = torch.empty(rows, dtype=torch.int32, device="cuda")
+        lp, ent = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+        for greedy in (False, True):
+            ok(mg, mg.mg_logits_sample(xd.data_ptr(), code, ld, cs, None if greedy else rd.data_ptr(), act.data_ptr(), lp.data_ptr(),
+                                       ent.data_ptr(), None, rows, actions, None))
+            assert status(mg) == 0
+            key = l.astype(np.float64) if greedy else l - np.log(race(next_word(words), actions))
+            key = np.where(np.isnan(key), -np.inf, key)  # a NaN is never drawn
+            want = np.where((key > -np.inf).any(1), key.argmax(1), -1)
+            assert np.array_equal(act.cpu().numpy(), want), (kinds, greedy)
+            broken = (l == np.inf).any(1) | np.isnan(l).any(1)
+            assert np.array_equal(np.isnan(lp.cpu().numpy()), broken) and np.array_equal(np.isnan(ent.cpu().numpy()), broken)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", sorted(TYPES))
 @pytest.mark.parametrize("actions", [5, 40, 3000])
 def test_logits_at_the_ends_of_the_type(mg, kind, actions):
     """Rows of the type's lowest number (a mask some programs write), of large offsets and of wide spreads: the softmax of
