@@ -633,6 +633,29 @@ def test_many_rows(mg, monkeypatch, rows, actions, pad, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("history", [490, 492])
+@pytest.mark.parametrize("rows,actions", [(640, 1100), (2300, 1100)])
+def test_tables_of_many_rows(mg, monkeypatch, rows, actions, history):
+    """Histories on both sides of the 40 KB that the eight tables of a CTA of warp teams may take (491 entries at 1100
+    actions), under every combination of penalties, for the calls whose rows are then a warp's or a CTA's."""
+    made = make_controls
+
+    def longer(rng, rows, actions, kinds):
+        c = made(rng, rows, actions, kinds)
+        if "history" in c:
+            c["history"] = rng.integers(-3, actions + 3, (rows, history)).astype(np.int32)
+            c["history_len"] = rng.integers(history - 9, history + 9, rows).astype(np.int32)
+        return c
+
+    monkeypatch.setitem(globals(), "make_controls", longer)
+    monkeypatch.setitem(globals(), "KINDS", KINDS[3:])
+    test_control_and_gradient(mg, rows, actions, 3, "bf16")
+    test_sample(mg, rows, actions, 3, "bf16")
+    if rows > 2 * actions:
+        test_policy_loss(mg, rows, actions, 3, "bf16")
+
+
+@pytest.mark.gpu
 def test_loss_gradient_against_differences(mg):
     """d(sum of row losses) / d(raw logit) by central differences of the 64-bit loss, penalties included."""
     rng = np.random.default_rng(9)
