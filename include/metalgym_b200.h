@@ -455,8 +455,10 @@ int mg_muon_workspace(int batch, int rows, int cols, size_t* bytes);
  * 2.0315 G^2) X, which takes singular values into about [0.7, 1.2]; 5 steps
  * do for the Muon update. x [batch][rows][ld] of `dtype`, batch_stride
  * elements apart; out likewise with ldo, out_stride, of out_dtype
- * MG_DTYPE_BF16 or MG_DTYPE_F16: the products take fp16 operands, X stays
- * fp32 (measured 0.03 to 0.3 % of the result's norm off the exact iteration). A zero
+ * MG_DTYPE_BF16 or MG_DTYPE_F16: the products take operands of 22 bits (two
+ * fp16 numbers), X stays fp32. Measured off the exact iteration, of the result's
+ * norm: 2e-6 to 5e-5; where the smaller side is at most 128 and steps at most 6,
+ * 6e-6 at full rank, up to 3e-4 at rank 8 and 3e-3 at rank 1. A zero
  * matrix gives zeros. x and out must not overlap. workspace: device memory of
  * mg_muon_workspace bytes, 16-byte aligned. */
 int mg_orthogonalize(const void* x, int dtype, int64_t ld, int64_t batch_stride, void* out, int out_dtype, int64_t ldo,

@@ -4,14 +4,17 @@
 //   X0 = U / |U|_F;  G = X X^T (rows <= cols) or X^T X;  B = b G + c G^2;
 //   X <- a X + B X (or X B),  (a, b, c) = (3.4445, -4.7750, 2.0315).
 //
-// Number formats: the operands of the products are fp16 (11 significant
-// bits), scaled by 2^10 so that entries from 2^-24 of |U| up are normal
-// numbers and the largest (|X|, |G| <= 1.5, |B| <= 12) stay below 2^14. X
-// itself is carried in fp32 beside its fp16 copy: with a X taken from the
-// 16-bit copy, its rounding would be multiplied by a = 3.4 in every step in
-// the directions that U hardly has (4 % of the result's norm off after five
-// steps at rank 8 of 128, against 0.06 % this way); bf16 operands would be
-// 1.4 % off on full-rank matrices, against 0.2 %.
+// Number formats: the operands of the products are sums of two fp16 numbers
+// (22 significant bits), scaled by 2^10 so that entries from 2^-24 of |U| up
+// are normal numbers and the largest (|X|, |G| <= 1.5, |B| <= 12) stay below
+// 2^14. X itself is carried in fp32 beside its two parts, since a X multiplies
+// its rounding by a = 3.4 in every step in the directions that U hardly has.
+// Measured against the exact iteration, of the result's norm: 2e-6 to 5e-5 (129
+// x 1000 .. 4096 x 4096; full rank, rank 1/16 over a floor of 1e-3, rows from 1
+// to 1e-4), as fp32 products by a library are (1e-6 to 2e-5); products of one
+// fp16 number were 5e-4 to 2e-3 off, in less than half the time at 4096 x 4096
+// (1510 us; 3230 this way, 3780 once the power cap holds), 0.85 of it at 333 x
+// 1001 (117 / 138).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -115,7 +118,7 @@ __global__ void __launch_bounds__(kPrepThreads)
     }
 }
 
-// X = U / |U| (0 for a zero U), and its fp16 copy; four columns a thread (the
+// X = U / |U| (0 for a zero U), and its two fp16 parts; four columns a thread (the
 // workspace's rows are padded to eight).
 __global__ void __launch_bounds__(kPrepThreads)
     k_muon_normalise(MuonShape s, float* x32, __half* x16, const double* partial, int parts) {
@@ -134,24 +137,25 @@ __global__ void __launch_bounds__(kPrepThreads)
     const InverseNorm inv(sum);
     const int64_t total = (int64_t)s.rows * s.ldx / 4;
     float4* x = reinterpret_cast<float4*>(x32 + (int64_t)b * s.rows * s.ldx);
-    uint2* h = reinterpret_cast<uint2*>(x16 + (int64_t)b * s.rows * s.ldx);
+    __half* h = x16 + (int64_t)b * s.rows * s.ldx;
+    const int64_t lo = (int64_t)gridDim.y * s.rows * s.ldx;
     for (int64_t i = (int64_t)blockIdx.x * kPrepThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kPrepThreads) {
         float4 v = x[i];  // (the padding's values are never read as operands)
         v = make_float4(inv(v.x), inv(v.y), inv(v.z), inv(v.w));
         x[i] = v;
-        h[i] = pack_half4(v.x * kNsScale, v.y * kNsScale, v.z * kNsScale, v.w * kNsScale);
+        store_parts4(h + 4 * i, lo, v.x * kNsScale, v.y * kNsScale, v.z * kNsScale, v.w * kNsScale);
     }
 }
 
-template <int KIND, int BN, int BM, bool A_MN, bool B_MN>
+template <int KIND, int BN, bool A_MN, bool B_MN>
 int launch_tiled(const CUtensorMap& ta, const CUtensorMap& tb, NsProduct p, cudaStream_t st) {
-    using S = NsTile<BN, BM>;
-    auto kern = k_ns_product<KIND, BN, BM, A_MN, B_MN>;
+    using S = NsTile<BN>;
+    auto kern = k_ns_product<KIND, BN, A_MN, B_MN>;
     static std::atomic<uint64_t> done{0};
     MG_TRY(smem_limit_once(kern, S::SMEM_BYTES, done));
-    p.tilesM = (p.M + BM - 1) / BM;
+    p.tilesM = (p.M + 127) / 128;
     p.tilesN = (p.N + BN - 1) / BN;
-    const int64_t units = (int64_t)ns_tiles<KIND, BN, BM>(p.tilesM, p.tilesN) * p.batch;
+    const int64_t units = (int64_t)ns_tiles<KIND, BN>(p.tilesM, p.tilesN) * p.batch;
     if (units > INT32_MAX) return fail(MG_ERR_ARGUMENT, "newton_schulz: too many tiles");
     const int grid = (int)std::min<int64_t>(units, num_sms());
     MG_CUDA_TRY(MG_LAUNCH(kern, grid, S::THREADS, S::SMEM_BYTES, st, ta, tb, p));
@@ -185,11 +189,14 @@ int launch_split(const CUtensorMap& ta, const CUtensorMap& tb, NsProduct p, int 
 }
 
 // Few tiles split a K of four blocks or more over a cluster, while the clusters
-// fit the GPU at once (measured: clusters of four on 144 of 148 SMs run in two
-// waves). Otherwise the tile with the fewest cycles: whole rounds over the SMs,
-// of 590, 870 and 1164 cycles a K block for 128 x 128, 128 x 256 and 256 x 256
-// (their operand bytes at the 55 a cycle that L2 gives an SM), and an epilogue
-// behind the last tile, or behind every tile of 256 x 256.
+// fit the GPU at once (five steps of 512 x 2048: 295 us unsplit, 209 and 166 with
+// clusters of two and four; clusters of four on 144 of 148 SMs run in two waves).
+// Otherwise the tile with the fewest cycles: whole rounds over the SMs, of 1180
+// and 1745 cycles a K block for 128 x 128 and 128 x 256 (the operand bytes of
+// both parts at the 55 a cycle that L2 gives an SM), and an epilogue behind the
+// last tile (all products by 128 x 128 / by 128 x 256 / by this rule: 8 x 1024 x
+// 1024 676 / 800 / 639 us, 2 x 1500 x 4000 1363 / 1098 / 1101, 4096 x 4096 4286 /
+// 3425 / 3434, 1500 x 1500 389 / 538 / 390).
 template <int KIND, bool A_MN, bool B_MN>
 int launch_product(const CUtensorMap& ta, const CUtensorMap& tb, const NsProduct& p, cudaStream_t st) {
     const int64_t tiles = (int64_t)ns_tiles<KIND, 128>((p.M + 127) / 128, (p.N + 127) / 128) * p.batch;
@@ -198,19 +205,15 @@ int launch_product(const CUtensorMap& ta, const CUtensorMap& tb, const NsProduct
     while (splits < 4 && tiles * splits * 2 <= sms * 7 / 8 && blocks >= 4 && blocks >= 2 * splits) splits *= 2;
     if (splits > 1) return launch_split<KIND, A_MN, B_MN>(ta, tb, p, splits, st);
     const int64_t wide = (int64_t)ns_tiles<KIND, 256>((p.M + 127) / 128, (p.N + 255) / 256) * p.batch;
-    const int64_t square = (int64_t)ns_tiles<KIND, 256, 256>((p.M + 255) / 256, (p.N + 255) / 256) * p.batch;
     auto rounds = [&](int64_t n) { return (n + sms - 1) / sms; };
-    const int64_t cost128 = rounds(tiles) * 590 * blocks + 3000, costWide = rounds(wide) * 870 * blocks + 5000;
-    const int64_t costSquare = rounds(square) * (1164 * blocks + 9000);
-    if (costSquare < costWide && costSquare < cost128) return launch_tiled<KIND, 256, 256, A_MN, B_MN>(ta, tb, p, st);
-    return costWide < cost128 ? launch_tiled<KIND, 256, 128, A_MN, B_MN>(ta, tb, p, st)
-                              : launch_tiled<KIND, 128, 128, A_MN, B_MN>(ta, tb, p, st);
+    const int64_t cost128 = rounds(tiles) * 1180 * blocks + 3000, costWide = rounds(wide) * 1745 * blocks + 5000;
+    return costWide < cost128 ? launch_tiled<KIND, 256, A_MN, B_MN>(ta, tb, p, st) : launch_tiled<KIND, 128, A_MN, B_MN>(ta, tb, p, st);
 }
 
 struct Workspace {
     double* partial;
     float* x32;
-    __half* x16[2];
+    __half* x16[2];  // hi, then lo parts of the batch; G and B likewise
     __half *g16, *b16;
     size_t bytes;
 };
@@ -229,10 +232,10 @@ Workspace layout(int batch, int rows, int cols, void* base) {
     const size_t s = std::min(rows, cols), x = (size_t)batch * rows * round8(cols), g = (size_t)batch * s * round8((int)s);
     w.partial = static_cast<double*>(take((size_t)batch * kPrepMaxParts * 8));
     w.x32 = static_cast<float*>(take(x * 4));
-    w.x16[0] = static_cast<__half*>(take(x * 2));
-    w.x16[1] = static_cast<__half*>(take(x * 2));
-    w.g16 = static_cast<__half*>(take(g * 2));
-    w.b16 = static_cast<__half*>(take(g * 2));
+    w.x16[0] = static_cast<__half*>(take(x * 4));
+    w.x16[1] = static_cast<__half*>(take(x * 4));
+    w.g16 = static_cast<__half*>(take(g * 4));
+    w.b16 = static_cast<__half*>(take(g * 4));
     w.bytes = at;
     return w;
 }
@@ -268,11 +271,11 @@ int newton_schulz(const Workspace& w, int batch, int rows, int cols, int steps, 
     const bool wide = rows <= cols;  // G = X X^T, else X^T X
     const int s = std::min(rows, cols), l = std::max(rows, cols), lds = round8(s);
     CUtensorMap mx[2], mg16, mb16;
-    for (int i = 0; i < 2; i++) MG_TRY(make_tmap_f16_3d(&mx[i], w.x16[i], cols, rows, batch, shape.ldx, 128));
+    for (int i = 0; i < 2; i++) MG_TRY(make_tmap_f16_3d(&mx[i], w.x16[i], cols, rows, 2 * batch, shape.ldx, 128));
     CUtensorMap mxk[2];  // boxes of 64 rows, for X as an operand whose K index is the row
-    for (int i = 0; i < 2; i++) MG_TRY(make_tmap_f16_3d(&mxk[i], w.x16[i], cols, rows, batch, shape.ldx, 64));
-    MG_TRY(make_tmap_f16_3d(&mg16, w.g16, s, s, batch, lds, 128));
-    MG_TRY(make_tmap_f16_3d(&mb16, w.b16, s, s, batch, lds, 128));
+    for (int i = 0; i < 2; i++) MG_TRY(make_tmap_f16_3d(&mxk[i], w.x16[i], cols, rows, 2 * batch, shape.ldx, 64));
+    MG_TRY(make_tmap_f16_3d(&mg16, w.g16, s, s, 2 * batch, lds, 128));
+    MG_TRY(make_tmap_f16_3d(&mb16, w.b16, s, s, 2 * batch, lds, 128));
     NsProduct p{};
     p.batch = batch;
     p.status = status_ptr();

@@ -1,11 +1,15 @@
-// The tcgen05 products of a Newton-Schulz step (muon.cu): fp16 operands, fp32
-// accumulation in tensor memory, persistent CTAs that walk 128 x BN output
-// tiles with the accumulator double-buffered in tensor memory, so that the
-// epilogue of one tile runs beside the products of the next.
+// The tcgen05 products of a Newton-Schulz step (muon.cu): operands of two fp16
+// parts, fp32 accumulation in tensor memory, persistent CTAs that walk 128 x BN
+// output tiles with the accumulator double-buffered in tensor memory, so that
+// the epilogue of one tile runs beside the products of the next.
 //
-// (256 x 256 tiles of large matrices have one accumulator set: their operands
-// come at 64 bytes a product cycle and SM instead of 96, which L2 does not
-// sustain, and that is worth more than the overlap.)
+// An operand V is hi + lo, hi = fp16(V) and lo = fp16(V - hi): 22 bits. A
+// product is lo hi + hi lo + hi hi, three products of fp16 matrices that share
+// their loads: a K block of the lo parts of both operands and one of their hi
+// parts follow one another through the ring of stages. Two 16-bit matrices are
+// also what X, G and B are to memory: the lo parts of a batch lie behind its
+// hi parts, so that part and matrix together are a tensor map's third
+// coordinate.
 //
 //   kNsGram   G = X X^T or X^T X, symmetric: only tiles that reach the diagonal
 //             or lie above it are computed, and written to both places
@@ -51,8 +55,8 @@ struct NsProduct {
     int M, N, K, batch;
     int tilesM, tilesN;
     int ldo;            // row stride of out16, g16 and x32 (a multiple of 8)
-    __half* out16;      // [batch][M][ldo], scaled
-    const __half* g16;  // kNsPoly
+    __half* out16;      // [hi, lo][batch][M][ldo], scaled
+    const __half* g16;  // kNsPoly, likewise
     float* x32;         // kNsApply
     float a, b, c;
     int last;
@@ -60,17 +64,15 @@ struct NsProduct {
     int* status;
 };
 
-// A tile of BM x BN, BM = 128, or 256 in two halves that share B (one
-// accumulator set: 512 columns are all of tensor memory).
-template <int BN, int BM = 128>
+// A tile of 128 x BN. A stage is 64 columns of K of one part of both operands.
+template <int BN>
 struct NsTile {
-    static constexpr int BK = 64, HALVES = BM / 128, ACCS = HALVES == 1 ? 2 : 1;
-    static constexpr int STAGES = BM == 256 ? 3 : BN == 256 ? 4 : 5;
-    static constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int BK = 64, STAGES = BN == 256 ? 4 : 5;
+    static constexpr int A_BYTES = 128 * BK * 2, B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int EW = BN == 256 ? 8 : 16, THREADS = 64 + 32 * EW, SLAB = 4096;
-    static constexpr int PIECES = BN / (8 * EW);  // 32-column pieces of an epilogue warp and half
+    static constexpr int PIECES = BN / (8 * EW);  // 32-column pieces of an epilogue warp
     static constexpr int SLAB_OFF = STAGES * STAGE_BYTES, BAR_OFF = SLAB_OFF + EW * SLAB;
-    static constexpr int TMEM_COLS = ACCS * HALVES * BN;
+    static constexpr int TMEM_COLS = 2 * BN;
     static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024 /*align*/;
 };
 
@@ -88,14 +90,14 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, i
 
 // Tiles of one matrix, and the u-th of them; of a symmetric product only those
 // that do not lie wholly below the diagonal.
-template <int KIND, int BN, int BM = 128>
+template <int KIND, int BN>
 __host__ __device__ __forceinline__ int ns_tiles(int tilesM, int tilesN) {
     if (KIND == kNsApply) return tilesM * tilesN;
     int n = 0;
-    for (int i = 0; i < tilesM; i++) n += tilesN - i * BM / BN;
+    for (int i = 0; i < tilesM; i++) n += tilesN - i * 128 / BN;
     return n;
 }
-template <int KIND, int BN, int BM = 128>
+template <int KIND, int BN>
 __device__ __forceinline__ void ns_tile_at(int u, int tilesN, int& i, int& j) {
     if (KIND == kNsApply) {
         i = u / tilesN;
@@ -103,11 +105,11 @@ __device__ __forceinline__ void ns_tile_at(int u, int tilesN, int& i, int& j) {
         return;
     }
     i = 0;
-    while (u >= tilesN - i * BM / BN) {
-        u -= tilesN - i * BM / BN;
+    while (u >= tilesN - i * 128 / BN) {
+        u -= tilesN - i * 128 / BN;
         i++;
     }
-    j = i * BM / BN + u;
+    j = i * 128 / BN + u;
 }
 
 __device__ __forceinline__ uint32_t ns_slab_offset(int r, int k) { return (uint32_t)(r * 128 + ((k ^ (r & 7)) << 4)); }
@@ -116,6 +118,40 @@ __device__ __forceinline__ uint2 pack_half4(float a, float b, float c, float d) 
     const __half2 x = __floats2half2_rn(a, b), y = __floats2half2_rn(c, d);
     return make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
 }
+
+// Four values (already scaled) as two parts, `lo` elements apart.
+__device__ __forceinline__ void store_parts4(__half* hi, int64_t lo, float a, float b, float c, float d) {
+    const uint2 h = pack_half4(a, b, c, d);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h.x)), y = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
+    *reinterpret_cast<uint2*>(hi) = h;
+    *reinterpret_cast<uint2*>(hi + lo) = pack_half4(a - x.x, b - x.y, c - y.x, d - y.y);
+}
+// Likewise eight, from 16-byte boundaries on.
+__device__ __forceinline__ void store_parts8(__half* hi, int64_t lo, const float* v) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const __half2 a = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        const float2 f = __half22float2(a);
+        const __half2 b = __floats2half2_rn(v[2 * i] - f.x, v[2 * i + 1] - f.y);
+        h[i] = *reinterpret_cast<const uint32_t*>(&a);
+        l[i] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    *reinterpret_cast<uint4*>(hi) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(hi + lo) = make_uint4(l[0], l[1], l[2], l[3]);
+}
+// The sum of four values' parts.
+__device__ __forceinline__ float4 parts_sum4(const uint2& h, const uint2& l) {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
+    const float2 c = __half22float2(*reinterpret_cast<const __half2*>(&l.x)), d = __half22float2(*reinterpret_cast<const __half2*>(&l.y));
+    return make_float4(a.x + c.x, a.y + c.y, b.x + d.x, b.y + d.y);
+}
+// B = b G + c G G, scaled by 2^10 as G is; y: the product's accumulator, times 2^-10.
+__device__ __forceinline__ float4 ns_poly4(const NsProduct& p, const float4& y, const float4& g) {
+    return make_float4(fmaf(p.c, y.x, p.b * g.x), fmaf(p.c, y.y, p.b * g.y), fmaf(p.c, y.z, p.b * g.z), fmaf(p.c, y.w, p.b * g.w));
+}
+// Elements from the hi to the lo parts of the product's output (and of G).
+__device__ __forceinline__ int64_t ns_lo(const NsProduct& p) { return (int64_t)p.batch * p.M * p.ldo; }
 
 // Four columns (from col on) of a row of X; v: the accumulator, x and master:
 // what was read there (x 0 where X is not kept).
@@ -127,7 +163,7 @@ __device__ __forceinline__ void ns_apply4(const NsProduct& p, int64_t at, int64_
     for (int i = 0; i < 4; i++) y[i] = fmaf(p.a, xv[i], y[i] * (kNsUnscale * kNsUnscale));
     if (!p.last) {
         *reinterpret_cast<float4*>(p.x32 + at) = make_float4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<uint2*>(p.out16 + at) = pack_half4(y[0] * kNsScale, y[1] * kNsScale, y[2] * kNsScale, y[3] * kNsScale);
+        store_parts4(p.out16 + at, ns_lo(p), y[0] * kNsScale, y[1] * kNsScale, y[2] * kNsScale, y[3] * kNsScale);
         return;
     }
     const int n = min(4, p.N - col);
@@ -179,7 +215,7 @@ __device__ __forceinline__ void ns_apply4(const NsProduct& p, int64_t at, int64_
 template <int KIND>
 struct NsFetched {
     float4 x[KIND == kNsApply ? 8 : 1];
-    uint2 g[KIND == kNsPoly ? 8 : 1];
+    uint2 g[KIND == kNsPoly ? 8 : 1], gLo[KIND == kNsPoly ? 8 : 1];
 };
 template <int KIND>
 __device__ __forceinline__ void ns_fetch(const NsProduct& p, int b, int row0, int col0, NsFetched<KIND>& f) {
@@ -189,10 +225,13 @@ __device__ __forceinline__ void ns_fetch(const NsProduct& p, int b, int row0, in
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         if (KIND == kNsApply) f.x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (KIND == kNsPoly) f.g[i] = make_uint2(0u, 0u);
+        if (KIND == kNsPoly) f.g[i] = f.gLo[i] = make_uint2(0u, 0u);
         if (col < p.N && row0 + 4 * i + (lane >> 3) < p.M) {
             if (KIND == kNsApply) f.x[i] = ld_f4_now(p.x32 + at + (int64_t)(4 * i) * p.ldo);
-            if (KIND == kNsPoly) f.g[i] = *reinterpret_cast<const uint2*>(p.g16 + at + (int64_t)(4 * i) * p.ldo);
+            if (KIND == kNsPoly) {
+                f.g[i] = *reinterpret_cast<const uint2*>(p.g16 + at + (int64_t)(4 * i) * p.ldo);
+                f.gLo[i] = *reinterpret_cast<const uint2*>(p.g16 + ns_lo(p) + at + (int64_t)(4 * i) * p.ldo);
+            }
         }
     }
 }
@@ -240,17 +279,8 @@ __device__ __forceinline__ void ns_piece(const NsProduct& p, int b, int row0, in
                     y.y *= kNsUnscale;
                     y.z *= kNsUnscale;
                     y.w *= kNsUnscale;
-                    if constexpr (KIND == kNsPoly) {
-                        const uint2 gw = f.g[4 * h + i];
-                        const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&gw.x));
-                        const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&gw.y));
-                        y.x = fmaf(p.c, y.x, p.b * g0.x);
-                        y.y = fmaf(p.c, y.y, p.b * g0.y);
-                        y.z = fmaf(p.c, y.z, p.b * g1.x);
-                        y.w = fmaf(p.c, y.w, p.b * g1.y);
-                    }
-                    if (row < p.M)
-                        *reinterpret_cast<uint2*>(p.out16 + base + (int64_t)row * p.ldo + col) = pack_half4(y.x, y.y, y.z, y.w);
+                    if constexpr (KIND == kNsPoly) y = ns_poly4(p, y, parts_sum4(f.g[4 * h + i], f.gLo[4 * h + i]));
+                    if (row < p.M) store_parts4(p.out16 + base + (int64_t)row * p.ldo + col, ns_lo(p), y.x, y.y, y.z, y.w);
                     if (mirror) *cell = y;
                 }
             }
@@ -269,34 +299,74 @@ __device__ __forceinline__ void ns_piece(const NsProduct& p, int b, int row0, in
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 y[i] = *reinterpret_cast<const float*>(slab + ns_slab_offset(8 * q + i, lane >> 2) + (lane & 3) * 4);
-            const uint2 lo = pack_half4(y[0], y[1], y[2], y[3]), hi = pack_half4(y[4], y[5], y[6], y[7]);
-            *reinterpret_cast<uint4*>(p.out16 + at + 8 * q) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            store_parts8(p.out16 + at + 8 * q, ns_lo(p), y);
         }
     }
 }
 
-template <int KIND, int BN, int BM, bool A_MN, bool B_MN>
-__global__ void __launch_bounds__(NsTile<BN, BM>::THREADS, 1)
+// The three products of a K block by one thread: the mixed ones, whose lo stage
+// is then free, and that of the hi parts. (The accumulator is cut off, not
+// rounded, at every instruction.)
+template <int BN, bool A_MN, bool B_MN>
+__device__ __forceinline__ void ns_mma_block(uint32_t acc, uint32_t lo, uint32_t hi, uint64_t* emptyLo, uint64_t* emptyHi, bool accumulate) {
+    constexpr uint32_t idesc = idesc_f16_f32(BN, A_MN, B_MN);
+#pragma unroll
+    for (int part = 0; part < 3; part++) {
+        const uint32_t a = part == 0 ? lo : hi, b = (part == 1 ? lo : hi) + NsTile<BN>::A_BYTES;
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++) {
+            const uint64_t ad = A_MN ? smem_desc_sw128(a + kk * 2048, 8192, 1024) : smem_desc_sw128(a + kk * 32, 16, 1024);
+            const uint64_t bd = B_MN ? smem_desc_sw128(b + kk * 2048, 8192, 1024) : smem_desc_sw128(b + kk * 32, 16, 1024);
+            // kind::f16: the types are idesc's
+            tc_mma_bf16(acc, ad, bd, idesc, accumulate || part > 0 || kk > 0 ? 1u : 0u);
+        }
+        if (part == 1) tc_commit(emptyLo);
+    }
+    tc_commit(emptyHi);
+}
+// One part (matrix z of the tensor maps) of a K block of both operands into a stage.
+template <int BN, bool A_MN, bool B_MN>
+__device__ __forceinline__ void ns_load_stage(uint8_t* sA, const CUtensorMap* tmA, const CUtensorMap* tmB, int m0, int n0, int k0, int z,
+                                              uint64_t* full) {
+    uint8_t* sB = sA + NsTile<BN>::A_BYTES;
+    mbar_arrive_expect_tx(full, NsTile<BN>::STAGE_BYTES);
+    if (A_MN) {
+        tma_load_3d(sA, tmA, m0, k0, z, full);
+        tma_load_3d(sA + 8192, tmA, m0 + 64, k0, z, full);
+    } else {  // a box of 128 rows
+        tma_load_3d(sA, tmA, k0, m0, z, full);
+    }
+    if (B_MN) {
+#pragma unroll
+        for (int j = 0; j < BN / 64; j++) tma_load_3d(sB + j * 8192, tmB, n0 + 64 * j, k0, z, full);
+    } else {
+#pragma unroll
+        for (int j = 0; j < BN / 128; j++) tma_load_3d(sB + j * 16384, tmB, k0, n0 + 128 * j, z, full);
+    }
+}
+
+template <int KIND, int BN, bool A_MN, bool B_MN>
+__global__ void __launch_bounds__(NsTile<BN>::THREADS, 1)
     k_ns_product(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const NsProduct p) {
-    using S = NsTile<BN, BM>;
+    using S = NsTile<BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::BAR_OFF);
     uint64_t* empty = full + S::STAGES;
-    uint64_t* tfull = empty + S::STAGES;  // [ACCS]
-    uint64_t* tempty = tfull + S::ACCS;   // [ACCS]
-    uint64_t* done = tempty + S::ACCS;
+    uint64_t* tfull = empty + S::STAGES;  // [2]
+    uint64_t* tempty = tfull + 2;         // [2]
+    uint64_t* done = tempty + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
     mg_pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int perMatrix = ns_tiles<KIND, BN, BM>(p.tilesM, p.tilesN), units = perMatrix * p.batch;
+    const int perMatrix = ns_tiles<KIND, BN>(p.tilesM, p.tilesN), units = perMatrix * p.batch;
     const int nk = (p.K + S::BK - 1) / S::BK;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::STAGES; s++) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int a = 0; a < S::ACCS; a++) {
+        for (int a = 0; a < 2; a++) {
             mbar_init(&tfull[a], 1);
             mbar_init(&tempty[a], S::EW);
         }
@@ -322,32 +392,15 @@ __global__ void __launch_bounds__(NsTile<BN, BM>::THREADS, 1)
             for (int u = blockIdx.x; u < units && ok; u += gridDim.x) {
                 const int b = u / perMatrix;
                 int ti, tj;
-                ns_tile_at<KIND, BN, BM>(u - b * perMatrix, p.tilesN, ti, tj);
-                const int m0 = ti * BM, n0 = tj * BN;
-                for (int kb = 0; kb < nk; kb++, it++) {
+                ns_tile_at<KIND, BN>(u - b * perMatrix, p.tilesN, ti, tj);
+                for (int h = 0; h < 2 * nk; h++, it++) {  // the lo, then the hi part of each K block
                     const int s = it % S::STAGES;
                     if (!mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1, p.status, kDevTimeoutEmpty)) {
                         ok = false;
                         break;
                     }
-                    uint8_t* sA = smem + s * S::STAGE_BYTES;
-                    uint8_t* sB = sA + S::A_BYTES;
-                    const int k0 = kb * S::BK;
-                    mbar_arrive_expect_tx(&full[s], S::STAGE_BYTES);
-                    if (A_MN) {
-#pragma unroll
-                        for (int j = 0; j < BM / 64; j++) tma_load_3d(sA + j * 8192, &tmA, m0 + 64 * j, k0, b, &full[s]);
-                    } else {  // boxes of 128 rows
-#pragma unroll
-                        for (int j = 0; j < S::HALVES; j++) tma_load_3d(sA + j * 16384, &tmA, k0, m0 + 128 * j, b, &full[s]);
-                    }
-                    if (B_MN) {
-#pragma unroll
-                        for (int j = 0; j < BN / 64; j++) tma_load_3d(sB + j * 8192, &tmB, n0 + 64 * j, k0, b, &full[s]);
-                    } else {  // boxes of 128 rows
-#pragma unroll
-                        for (int j = 0; j < BN / 128; j++) tma_load_3d(sB + j * 16384, &tmB, k0, n0 + 128 * j, b, &full[s]);
-                    }
+                    ns_load_stage<BN, A_MN, B_MN>(smem + s * S::STAGE_BYTES, &tmA, &tmB, ti * 128, tj * BN, (h >> 1) * S::BK,
+                                                  (h & 1) ? b : b + p.batch, &full[s]);
                 }
             }
             // every issued copy has landed before this CTA can exit
@@ -356,35 +409,22 @@ __global__ void __launch_bounds__(NsTile<BN, BM>::THREADS, 1)
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            constexpr uint32_t idesc = idesc_f16_f32(BN, A_MN, B_MN);
             int it = 0, t = 0;
             bool ok = true;
             for (int u = blockIdx.x; u < units && ok; u += gridDim.x, t++) {
-                const int a = t % S::ACCS;
-                if (!mbar_wait(&tempty[a], ((t / S::ACCS) & 1) ^ 1, p.status, kDevTimeoutEmpty)) break;
+                const int a = t & 1;
+                if (!mbar_wait(&tempty[a], ((t >> 1) & 1) ^ 1, p.status, kDevTimeoutEmpty)) break;
                 tc_fence_after();
-                const uint32_t acc = tmem + (uint32_t)(a * S::HALVES * BN);
-                for (int kb = 0; kb < nk; kb++, it++) {
-                    const int s = it % S::STAGES;
-                    if (!mbar_wait(&full[s], (it / S::STAGES) & 1, p.status, kDevTimeoutFull)) {
+                for (int kb = 0; kb < nk; kb++, it += 2) {
+                    const int lo = it % S::STAGES, hi = (it + 1) % S::STAGES;
+                    if (!mbar_wait(&full[lo], (it / S::STAGES) & 1, p.status, kDevTimeoutFull) ||
+                        !mbar_wait(&full[hi], ((it + 1) / S::STAGES) & 1, p.status, kDevTimeoutFull)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t aBase = smem_u32(smem + s * S::STAGE_BYTES), bBase = aBase + S::A_BYTES;
-#pragma unroll
-                    for (int kk = 0; kk < 4; kk++) {
-                        const uint64_t bd = B_MN ? smem_desc_sw128(bBase + kk * 2048, 8192, 1024)
-                                                 : smem_desc_sw128(bBase + kk * 32, 16, 1024);
-#pragma unroll
-                        for (int h = 0; h < S::HALVES; h++) {
-                            const uint64_t ad = A_MN ? smem_desc_sw128(aBase + h * 16384 + kk * 2048, 8192, 1024)
-                                                     : smem_desc_sw128(aBase + h * 16384 + kk * 32, 16, 1024);
-                            // kind::f16: the types are idesc's
-                            tc_mma_bf16(acc + (uint32_t)(h * BN), ad, bd, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
-                        }
-                    }
-                    tc_commit(&empty[s]);
+                    ns_mma_block<BN, A_MN, B_MN>(tmem + (uint32_t)(a * BN), smem_u32(smem + lo * S::STAGE_BYTES),
+                                                 smem_u32(smem + hi * S::STAGE_BYTES), &empty[lo], &empty[hi], kb > 0);
                 }
                 if (ok) tc_commit(&tfull[a]);
             }
@@ -396,26 +436,25 @@ __global__ void __launch_bounds__(NsTile<BN, BM>::THREADS, 1)
         uint8_t* slab = smem + S::SLAB_OFF + e * S::SLAB;
         int t = 0;
         for (int u = blockIdx.x; u < units; u += gridDim.x, t++) {
-            const int b = u / perMatrix, a = t % S::ACCS;
+            const int b = u / perMatrix, a = t & 1;
             int ti, tj;
-            ns_tile_at<KIND, BN, BM>(u - b * perMatrix, p.tilesN, ti, tj);
-            const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * S::HALVES * BN + part);
+            ns_tile_at<KIND, BN>(u - b * perMatrix, p.tilesN, ti, tj);
+            const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN + part);
 #pragma unroll 1
-            for (int c = 0; c < S::HALVES * S::PIECES; c++) {
-                const int h = c / S::PIECES, at = 32 * (c % S::PIECES);
-                const int row0 = ti * BM + 128 * h + 32 * q, col0 = tj * BN + part + at;
+            for (int c = 0; c < S::PIECES; c++) {
+                const int at = 32 * c, row0 = ti * 128 + 32 * q, col0 = tj * BN + part + at;
                 const bool wanted = row0 < p.M && col0 < p.N && (KIND == kNsApply || col0 >= row0);
                 NsFetched<KIND> f;
                 if (wanted) ns_fetch<KIND>(p, b, row0, col0, f);
                 __syncwarp();  // lanes at a matrix's edge took other branches; loads from tensor memory take whole warps
                 if (c == 0) {
-                    if (!mbar_wait_warp(&tfull[a], (t / S::ACCS) & 1, p.status, kDevTimeoutDone)) gaveUp = true;
+                    if (!mbar_wait_warp(&tfull[a], (t >> 1) & 1, p.status, kDevTimeoutDone)) gaveUp = true;
                     if (gaveUp) break;
                     tc_fence_after();
                 }
                 float v[32];
-                tmem_ld32(acc + (uint32_t)(h * BN + at), v);
-                if (c == S::HALVES * S::PIECES - 1) {  // the accumulator is free for the next tile that uses it
+                tmem_ld32(acc + (uint32_t)at, v);
+                if (c == S::PIECES - 1) {  // the accumulator is free for the next tile that uses it
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&tempty[a]);
@@ -436,10 +475,10 @@ __global__ void __launch_bounds__(NsTile<BN, BM>::THREADS, 1)
 
 // Products of few tiles with K split over the CTAs of a cluster, one 128 x 128
 // tile per cluster: a tile's operands come at about 55 bytes a cycle and SM
-// from L2, 590 cycles for a K block whose products take 256, so that few tiles
+// from L2, 1180 cycles for a K block whose products take 768, so that few tiles
 // with a long K leave most of that rate unused. Every CTA leaves its part of
 // the sum in the slabs; CTA r then adds the parts of rows 32 r / splits .. of
-// each piece, in their order, and writes them. (512 x 2048: 178 -> 128 us.)
+// each piece, in their order, and writes them. (512 x 2048: 295 -> 166 us.)
 template <int KIND, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(NsTile<128>::THREADS, 1)
     k_ns_split(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const NsProduct p, int splits) {
@@ -482,25 +521,11 @@ __global__ void __launch_bounds__(NsTile<128>::THREADS, 1)
     if (warp == 0) {
         if (lane == 0) {
             int it = 0;
-            for (int kb = kFirst; kb < kEnd; kb++, it++) {
+            for (; it < 2 * (kEnd - kFirst); it++) {  // the lo, then the hi part of each K block
                 const int s = it % S::STAGES;
                 if (!mbar_wait(&empty[s], ((it / S::STAGES) & 1) ^ 1, p.status, kDevTimeoutEmpty)) break;
-                uint8_t* sA = smem + s * S::STAGE_BYTES;
-                uint8_t* sB = sA + S::A_BYTES;
-                const int k0 = kb * S::BK;
-                mbar_arrive_expect_tx(&full[s], S::STAGE_BYTES);
-                if (A_MN) {
-                    tma_load_3d(sA, &tmA, m0, k0, b, &full[s]);
-                    tma_load_3d(sA + 8192, &tmA, m0 + 64, k0, b, &full[s]);
-                } else {
-                    tma_load_3d(sA, &tmA, k0, m0, b, &full[s]);
-                }
-                if (B_MN) {
-                    tma_load_3d(sB, &tmB, n0, k0, b, &full[s]);
-                    tma_load_3d(sB + 8192, &tmB, n0 + 64, k0, b, &full[s]);
-                } else {
-                    tma_load_3d(sB, &tmB, k0, n0, b, &full[s]);
-                }
+                ns_load_stage<128, A_MN, B_MN>(smem + s * S::STAGE_BYTES, &tmA, &tmB, m0, n0, (kFirst + (it >> 1)) * S::BK,
+                                               (it & 1) ? b : b + p.batch, &full[s]);
             }
             // every issued copy has landed before this CTA can exit
             for (int k = it - S::STAGES < 0 ? 0 : it - S::STAGES; k < it; k++)
@@ -508,21 +533,14 @@ __global__ void __launch_bounds__(NsTile<128>::THREADS, 1)
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            constexpr uint32_t idesc = idesc_f16_f32(128, A_MN, B_MN);
-            for (int it = 0; it < kEnd - kFirst; it++) {
-                const int s = it % S::STAGES;
-                if (!mbar_wait(&full[s], (it / S::STAGES) & 1, p.status, kDevTimeoutFull)) break;
+            for (int it = 0; it < 2 * (kEnd - kFirst); it += 2) {
+                const int lo = it % S::STAGES, hi = (it + 1) % S::STAGES;
+                if (!mbar_wait(&full[lo], (it / S::STAGES) & 1, p.status, kDevTimeoutFull) ||
+                    !mbar_wait(&full[hi], ((it + 1) / S::STAGES) & 1, p.status, kDevTimeoutFull))
+                    break;
                 tc_fence_after();
-                const uint32_t aBase = smem_u32(smem + s * S::STAGE_BYTES), bBase = aBase + S::A_BYTES;
-#pragma unroll
-                for (int kk = 0; kk < 4; kk++) {
-                    const uint64_t ad = A_MN ? smem_desc_sw128(aBase + kk * 2048, 8192, 1024)
-                                             : smem_desc_sw128(aBase + kk * 32, 16, 1024);
-                    const uint64_t bd = B_MN ? smem_desc_sw128(bBase + kk * 2048, 8192, 1024)
-                                             : smem_desc_sw128(bBase + kk * 32, 16, 1024);
-                    tc_mma_bf16(tmem, ad, bd, idesc, (it > 0 || kk > 0) ? 1u : 0u);
-                }
-                tc_commit(&empty[s]);
+                ns_mma_block<128, A_MN, B_MN>(tmem, smem_u32(smem + lo * S::STAGE_BYTES), smem_u32(smem + hi * S::STAGE_BYTES), &empty[lo],
+                                              &empty[hi], it > 0);
             }
             tc_commit(done);  // covers every MMA issued, also after a timeout
         }
@@ -549,10 +567,13 @@ __global__ void __launch_bounds__(NsTile<128>::THREADS, 1)
         for (int r = first + (lane >> 3); r < first + share; r += 4) {
             const int row = row0 + r;
             const bool in = row < p.M && col < p.N;
-            uint2 gw = make_uint2(0u, 0u);
+            uint2 gw = make_uint2(0u, 0u), gLo = gw;
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f), m = x;
             const int64_t finAt = (int64_t)b * p.fin.stride + (int64_t)row * p.fin.ld + col;
-            if (KIND == kNsPoly && in) gw = *reinterpret_cast<const uint2*>(p.g16 + base + (int64_t)row * p.ldo + col);
+            if (KIND == kNsPoly && in) {
+                gw = *reinterpret_cast<const uint2*>(p.g16 + base + (int64_t)row * p.ldo + col);
+                gLo = *reinterpret_cast<const uint2*>(p.g16 + ns_lo(p) + base + (int64_t)row * p.ldo + col);
+            }
             if (KIND == kNsApply && in) {
                 x = ld_f4_now(p.x32 + base + (int64_t)row * p.ldo + col);
                 if (finVec && p.fin.master && col + 4 <= p.N) m = ld_f4_now(p.fin.master + finAt);
@@ -574,15 +595,8 @@ __global__ void __launch_bounds__(NsTile<128>::THREADS, 1)
             y.y *= kNsUnscale;
             y.z *= kNsUnscale;
             y.w *= kNsUnscale;
-            if (KIND == kNsPoly) {
-                const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&gw.x));
-                const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&gw.y));
-                y.x = fmaf(p.c, y.x, p.b * g0.x);
-                y.y = fmaf(p.c, y.y, p.b * g0.y);
-                y.z = fmaf(p.c, y.z, p.b * g1.x);
-                y.w = fmaf(p.c, y.w, p.b * g1.y);
-            }
-            if (in) *reinterpret_cast<uint2*>(p.out16 + base + (int64_t)row * p.ldo + col) = pack_half4(y.x, y.y, y.z, y.w);
+            if (KIND == kNsPoly) y = ns_poly4(p, y, parts_sum4(gw, gLo));
+            if (in) store_parts4(p.out16 + base + (int64_t)row * p.ldo + col, ns_lo(p), y.x, y.y, y.z, y.w);
             // (rows `first` .. of this CTA's slab are read by nobody else)
             if (mirror) *reinterpret_cast<float4*>(slab + off) = y;
         }
@@ -594,8 +608,7 @@ __global__ void __launch_bounds__(NsTile<128>::THREADS, 1)
 #pragma unroll
                 for (int i = 0; i < 8; i++)
                     y[i] = *reinterpret_cast<const float*>(slab + ns_slab_offset(r + i, lane >> 2) + (lane & 3) * 4);
-                const uint2 lo = pack_half4(y[0], y[1], y[2], y[3]), hi = pack_half4(y[4], y[5], y[6], y[7]);
-                *reinterpret_cast<uint4*>(p.out16 + base + (int64_t)mrow * p.ldo + row0 + r) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                store_parts8(p.out16 + base + (int64_t)mrow * p.ldo + row0 + r, ns_lo(p), y);
             }
         }
     }

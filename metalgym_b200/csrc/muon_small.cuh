@@ -12,9 +12,10 @@
 // Precision: P grows to a^steps in directions that U hardly has, so that the
 // rounding of P, G or X to 16 bits would show in the others. Every operand is
 // the sum of two fp16 numbers (22 bits), every product three tcgen05 products:
-// about 1e-5 of the result's norm off the exact iteration at full rank; at
-// rank 1 of 128 up to 2e-3, as the products with 16-bit operands are. P is scaled by 2^5, the
-// others by 2^10: within fp16's range for up to six steps (3.4445^6 2^5 < 2^16).
+// 6e-6 of the result's norm off the exact iteration at full rank, 3e-4 at rank
+// 8 of 128 and 3e-3 at rank 1, where the cuts of the accumulator are as large as
+// P's largest directions make them. P is scaled by 2^5, the others by 2^10:
+// within fp16's range for up to six steps (3.4445^6 2^5 < 2^16).
 #pragma once
 
 #include "logits.cuh"

@@ -202,6 +202,51 @@ def test_small_side_is_as_exact_as_fp32(mg, batch, m, n, spectrum):
         assert (master[i].double() - want).norm() <= 16 * (2.0 ** -22 + 8 * 2.0 ** -23) * growth * want.norm()
 
 
+def newton_schulz_parts(u, steps, gen):
+    """The iteration in 64 bits with operands of two fp16 parts, X through fp32, and products whose fp32 accumulator is cut
+    off after each of their 3 K / 16 instructions: 2^-24 of the sum a cut, and as noise 3 sqrt(3 K / 16) 2^-24 of an entry
+    (or of the entries' root mean square: partial sums are no smaller), seven times what independent cuts of up to a step give."""
+    def h(v):
+        hi = (v * 1024).half().double()
+        return (hi + (v * 1024 - hi).half().double()) / 1024
+
+    def product(a, b):
+        p, n = h(a) @ h(b), 3 * ((a.shape[1] + 15) // 16)
+        size = p.abs().clamp(min=float(p.norm()) / p.numel() ** 0.5)
+        return p * (1 - n * 2.0 ** -24) + 3 * n ** 0.5 * 2.0 ** -24 * size * torch.randn(p.shape, generator=gen, device=p.device, dtype=p.dtype)
+
+    x = u.double() / u.double().norm()
+    flip = x.shape[0] > x.shape[1]
+    x = x.t() if flip else x
+    for _ in range(steps):
+        x = x.float().double()
+        g = h(product(x, x.t()))
+        x = A * x + product(B * g + C * product(g, g), x)
+    return x.t() if flip else x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("spectrum", ["normal", "low rank", "decaying"])
+@pytest.mark.parametrize("batch,m,n", [(1, 129, 1000), (2, 333, 1001), (1, 1001, 333), (1, 640, 640), (4, 512, 1030), (3, 200, 140), (1, 1100, 1000),
+                                       (12, 1024, 1030)])
+def test_larger_sides_are_as_exact_as_smaller_ones(mg, batch, m, n, spectrum):
+    """Smaller sides above 128 take operands of 22 bits too: the master weights, which show the update without a 16-bit
+    rounding, are off by at most 1.5 times the distance of the emulated roundings and 2^-20 of the update."""
+    gen = torch.Generator(device="cuda").manual_seed(batch + m + n)
+    grad = torch.stack([matrix(gen, m, n, spectrum) for _ in range(batch)])
+    master, momentum = torch.zeros_like(grad), torch.zeros_like(grad)
+    weights = torch.zeros(batch, m, n, dtype=torch.bfloat16, device="cuda")
+    space = workspace(mg, batch, m, n)
+    ok(mg, mg.mg_muon_step(master.data_ptr(), grad.data_ptr(), momentum.data_ptr(), weights.data_ptr(), m * n, batch, m, n, None, 0, 0.0, -1.0,
+                           1.0, 0.0, 0, 0.0, 5, None, space.data_ptr(), space.numel(), None))
+    assert status(mg) == 0
+    for i in range(0, batch, max(1, batch - 1)):
+        want = newton_schulz(grad[i], 5, False)
+        near = newton_schulz_parts(grad[i], 5, gen)
+        off = (master[i].double() - want).norm()
+        assert off <= 1.5 * (near - want).norm() + 2.0 ** -20 * want.norm(), float(off / want.norm())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("batch,m,n", [(1, 130, 300), (1, 333, 1001), (40, 161, 200), (3, 200, 1100), (1, 1030, 1500), (2, 129, 133), (1, 100, 700)])
 def test_pieces_that_end_inside_a_warp(mg, batch, m, n):
