@@ -783,6 +783,7 @@ size_t table_smem(const TeamPart& p) {
 
 // the largest table (2^18 actions, 2^14 entries); a CTA's eight of warp teams take less
 constexpr int kTableSmemMax = 216 * 1024;
+static_assert(HistoryTable::bytes(MG_LOGITS_MAX_ACTIONS, MG_LOGITS_MAX_HISTORY) <= kTableSmemMax, "every table that the calls accept");
 
 // A launch of rows x parts CTAs (or warp teams), the parts of a row in one cluster.
 template <int NT, class... KArgs, class... Args>

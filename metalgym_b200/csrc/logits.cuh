@@ -18,9 +18,6 @@
 
 namespace mg {
 
-constexpr int kLogitsMaxActions = 1 << 18;   // the seen-bits of a row fit in 32 KB
-constexpr int kLogitsMaxHistory = 1 << 14;   // a count fits in 16 bits
-
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
@@ -43,9 +40,9 @@ struct HistoryTable {
     uint16_t* before;  // [words]
     int words;
 
-    __host__ __device__ static int words_of(int span) { return (span + 31) / 32; }
-    __host__ __device__ static int entries(int span, int history) { return span < history ? span : history; }
-    __host__ __device__ static size_t bytes(int span, int history) {
+    __host__ __device__ static constexpr int words_of(int span) { return (span + 31) / 32; }
+    __host__ __device__ static constexpr int entries(int span, int history) { return span < history ? span : history; }
+    __host__ __device__ static constexpr size_t bytes(int span, int history) {
         const int w = words_of(span), n = entries(span, history);
         return (size_t)w * 4 + (size_t)((n + 1) / 2) * 4 + (size_t)n * 8 + (size_t)((w + 1) / 2) * 4;
     }
@@ -68,6 +65,8 @@ struct HistoryTable {
         return (w & bit) ? count_at(before[i >> 5] + __popc(w & (bit - 1u))) : 0;
     }
 };
+
+static_assert(MG_LOGITS_MAX_HISTORY < 1 << 16, "counts and ranks are 16 bits");
 
 template <int NT>
 __device__ __forceinline__ void team_sync() {

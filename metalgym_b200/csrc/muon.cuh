@@ -221,7 +221,6 @@ template <int KIND>
 __device__ __forceinline__ void ns_fetch(const NsProduct& p, int b, int row0, int col0, NsFetched<KIND>& f) {
     const int lane = threadIdx.x & 31, col = col0 + 4 * (lane & 7);
     const int64_t at = ((int64_t)b * p.M + row0 + (lane >> 3)) * p.ldo + col;
-    if (KIND == kNsApply && !p.x32) return;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         if (KIND == kNsApply) f.x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
