@@ -447,13 +447,16 @@ int mg_logits_policy_loss(const void* logits, int dtype, int64_t ld, const mg_lo
 /* Bytes of the workspace that mg_orthogonalize and mg_muon_step need for
  * `batch` matrices of rows x cols. One workspace serves one call at a time:
  * calls that may overlap on the GPU (two streams, two captured graphs) need
- * one each. */
+ * one each. Matrices whose smaller side is at most 128 are done without it in up
+ * to 6 steps; the calls ask for it all the same, since the size goes by the
+ * shape alone. */
 int mg_muon_workspace(int batch, int rows, int cols, size_t* bytes);
 /* out = the matrix of x brought near the closest matrix with orthonormal rows
  * (rows <= cols) or columns, by `steps` (1..16) Newton-Schulz steps: X = x /
  * |x|_F, then G = X X^T (or X^T X, the smaller), X = 3.4445 X + (-4.7750 G +
  * 2.0315 G^2) X, which takes singular values into about [0.7, 1.2]; 5 steps
- * do for the Muon update. x [batch][rows][ld] of `dtype`, batch_stride
+ * do for the Muon update (iteration, coefficients and update as K. Jordan et
+ * al. published them: "Muon: an optimizer for hidden layers", 2024). x [batch][rows][ld] of `dtype`, batch_stride
  * elements apart; out likewise with ldo, out_stride, of out_dtype
  * MG_DTYPE_BF16 or MG_DTYPE_F16: the products take operands of 22 bits (two
  * fp16 numbers), X stays fp32. Measured off the exact iteration, of the result's
