@@ -456,7 +456,7 @@ int mg_muon_workspace(int batch, int rows, int cols, size_t* bytes);
  * |x|_F, then G = X X^T (or X^T X, the smaller), X = 3.4445 X + (-4.7750 G +
  * 2.0315 G^2) X, which takes singular values into about [0.7, 1.2]; 5 steps
  * do for the Muon update (iteration, coefficients and update as K. Jordan et
- * al. published them: "Muon: an optimizer for hidden layers", 2024). x [batch][rows][ld] of `dtype`, batch_stride
+ * al. published them: "Muon: An optimizer for hidden layers in neural networks", 2024). x [batch][rows][ld] of `dtype`, batch_stride
  * elements apart; out likewise with ldo, out_stride, of out_dtype
  * MG_DTYPE_BF16 or MG_DTYPE_F16: the products take operands of 22 bits (two
  * fp16 numbers), X stays fp32. Measured off the exact iteration, of the result's

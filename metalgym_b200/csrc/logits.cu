@@ -808,33 +808,59 @@ int launch_rows(void (*kern)(KArgs...), const TeamPart& p, cudaStream_t st, cons
     return check_launch(what);
 }
 
-// Parts of a row for the calls that need the whole row's statistics: more
-// while the CTAs do not fill the GPU (and a part keeps 4096 actions), and, for
-// the loss, so many that the rows in flight stay in L2 for its second pass (1000 x 50001
-// fp32: 185 us at four parts, 153 at two, 175 at one, whose rows are 118 MB).
-int row_parts(int rows, int actions, int size, int nt, bool twice) {
-    int parts = 1;
-    const int fill = 4 * num_sms();
-    while (parts < 8 && (int64_t)rows * parts < fill && actions / (2 * parts) >= 4096) parts *= 2;
-    if (twice)
-        while (parts < 8 && (int64_t)num_sms() * (1024 / nt) / parts * actions * size > (100 << 20)) parts *= 2;
-    return parts;
+// Parts of a row for the calls that need the whole row's statistics: the
+// fewest nanoseconds by what a CTA alone takes a logit, without and with
+// controls, and what a cluster of two, four or eight costs the call and each
+// row (its CTAs start together, which the GPU grants one cluster at a time).
+// Over 1 to 5000 rows of 6000 to 262144 actions of bf16 and fp32 the choice is
+// within 0.4 % (draw) and 1.5 % (loss) of the best of the four on average; us
+// with 1, 2, 4, 8 parts, all controls:
+//   draw   1 x 32768   20.6  14.5  12.4  13.2     loss   1 x 32768   26.4  17.1  12.2  10.8
+//         64 x 131072  63.0  45.6  35.7  44.7           64 x 50001   44.9  30.2  28.2  30.7
+//        200 x 20000   22.9  20.2  36.1  98.0          200 x 131072   154  92.9  87.0   103
+//        592 x 24000   31.8  43.4  82.4   265         1000 x 50001    145   130   169   331
+// A loss of more rows than the GPU holds CTAs takes two parts from 128 KB a row
+// on: what it reads and writes would not stay in L2 for the second pass (4096 x
+// 32768 fp32 without controls 252 us in one part, 224 in two).
+int row_parts(int rows, int actions, int size, bool controls, bool loss) {
+    const double fixed[2][4] = {{0, 900, 1500, 3800}, {0, 1000, 1100, 2800}};  // [draw, loss][parts 1, 2, 4, 8]
+    const double perRow[2][4] = {{0, 16, 110, 470}, {0, 10, 47, 160}}, perLogit[2][2] = {{0.23, 0.41}, {0.19, 0.55}};
+    int best = 0;
+    double least = 0.0;
+    for (int i = 0; i < 4 && (i == 0 || actions >= 2048 << i); i++) {  // (so long that no part is empty)
+        const double ns = fixed[loss][i] + perRow[loss][i] * rows + perLogit[loss][controls] * actions / (1 << i);
+        if (i == 0 || ns < least) best = i, least = ns;
+    }
+    if (loss && rows > 5 * num_sms() && (int64_t)actions * size >= 128 << 10) best = std::max(best, 1);
+    return 1 << best;
 }
 
-// Whether a warp takes a row. A CTA spends about 3000 instructions on a row
-// whatever its length (merging warps, barriers), a warp waits out its loads one
-// after the other: up to 256 actions a warp is never slower; longer rows take a
-// CTA while CTAs have SMs of their own (draw of 256 x 1000 with all controls:
-// 15.2 us, 20.5 by warps), and a warp where rows are many for their length
-// (8000 x 2048, draw 49 us, 90 by CTAs; control 45 / 72; loss 41 / 55; but
-// 1024 x 4096, loss 18.4 / 16.4, control 24.6 / 20.5), unless the eight history tables
-// would leave an SM few warps.
-bool warp_teams(int rows, int actions, int historyMax, bool loss) {
-    if (actions <= 256) return true;
-    if (rows <= 4 * num_sms()) return false;
-    if (actions <= 1024) return true;
-    const int64_t most = loss ? std::min<int64_t>(rows / 2, 2816) : std::min<int64_t>(2 * (int64_t)rows, 4096);
-    return actions <= most && (!historyMax || HistoryTable::bytes(actions, historyMax) * kWarpRows <= 40 * 1024);
+enum RowCall { kCallControl, kCallDraw, kCallLoss };
+
+// Whether a warp takes a row, instead of a CTA. A CTA spends about 3000
+// instructions on a row whatever its length (merging warps, barriers), a warp
+// waits out its loads one after the other, a row's history among them: warps are
+// faster where rows are many for their length and their history's, and where
+// rows are short. The choice is within 0.7 % (draw, loss) and 1.3 % (control) of
+// the better of the two on average over 4 to 8000 rows of 6 to 12000 actions with
+// histories of 0 to 2000; us by warps / by CTAs, mask, bias and a history of 64:
+//             180 x 300   600 x 1500   1000 x 2816   1000 x 3500   2048 x 4096   8000 x 6000
+//   control   4.5 / 6.4    6.7 / 7.3   10.6 / 12.4   13.3 / 13.0   14.4 / 22.8   64.5 / 88.8
+//   draw      9.5 / 8.7   14.9 / 15.9  20.1 / 21.1   24.1 / 21.7   24.6 / 41.3    131 / 194
+//   loss      8.2 / 9.1   12.6 / 10.2  18.6 / 16.3   23.4 / 18.3   25.3 / 29.8    157 / 152
+// and 1000 x 1024 with a history of 512 14.1 / 12.8, 21.1 / 19.3, 18.0 / 15.1.
+// Eight history tables beyond 100 KB leave an SM one CTA (4096 x 2048 with a
+// history of 1500, draw 137 / 106).
+bool warp_teams(RowCall call, int rows, int actions, int historyMax) {
+    if (actions <= 256 && historyMax <= 64) return true;
+    if (historyMax && HistoryTable::bytes(actions, historyMax) * kWarpRows > 100 * 1024) return false;
+    const int64_t r = rows, a = actions, h = historyMax;
+    const int sms = num_sms();
+    switch (call) {
+        case kCallControl: return r > sms && a <= 8192 && a + 9 * h <= 5 * r;
+        case kCallDraw: return r > 4 * sms && a <= 12000 && 4 * a + 9 * h <= 12 * r;
+        default: return r > sms && a <= 3600 && 2 * a + 8 * h <= 5 * r;
+    }
 }
 
 // The compiled controls that a call needs; `history`: the pass leaves out the
@@ -867,7 +893,7 @@ template <class T, bool BACKWARD>
 int control(const void* logits, int64_t ld, const mg_logit_controls& c, const void* dOut, int64_t ldg, void* out, int64_t ldo,
             int rows, int actions, cudaStream_t st) {
     auto f = launch_control<T, 32, BACKWARD, BACKWARD ? kWithMask : kWithBias | kWithMask>;
-    if (!warp_teams(rows, actions, c.history_max, false)) {
+    if (!warp_teams(kCallControl, rows, actions, c.history_max)) {
         switch (needed_controls(c, false)) {
             case 0: f = launch_control<T, 256, BACKWARD, 0>; break;
             case kWithMask: f = launch_control<T, 256, BACKWARD, kWithMask>; break;
@@ -885,7 +911,7 @@ int launch_sample(const void* logits, int64_t ld, const mg_logit_controls& c, ui
     auto kern = k_logits_sample<T, NT, GREEDY, WITH>;
     static std::atomic<uint64_t> done{0};
     MG_TRY(smem_limit_once(kern, kTableSmemMax, done));
-    const TeamPart p = plan(NT, rows, actions, NT == 32 ? 1 : row_parts(rows, actions, sizeof(T), NT, false), c.history_max);
+    const TeamPart p = plan(NT, rows, actions, NT == 32 ? 1 : row_parts(rows, actions, sizeof(T), WITH != 0, false), c.history_max);
     return launch_rows<NT>(kern, p, st, "k_logits_sample", static_cast<const T*>(logits), ld, c, rng, action, logProb, entropy,
                            value, p);
 }
@@ -894,7 +920,7 @@ template <class T, bool GREEDY>
 int sample_rows(const void* logits, int64_t ld, const mg_logit_controls& c, uint32_t* rng, int32_t* action, float* logProb,
                 float* entropy, float* value, int rows, int actions, cudaStream_t st) {
     auto f = launch_sample<T, 32, GREEDY, 3>;
-    if (!warp_teams(rows, actions, c.history_max, false)) {
+    if (!warp_teams(kCallDraw, rows, actions, c.history_max)) {
         switch (needed_controls(c, true)) {
             case 0: f = launch_sample<T, 256, GREEDY, 0>; break;
             case 1: f = launch_sample<T, 256, GREEDY, 1>; break;
@@ -918,7 +944,7 @@ int launch_loss(const void* logits, int64_t ld, const mg_logit_controls& c, void
     auto kern = k_logits_loss<T, NT, WITH>;
     static std::atomic<uint64_t> done{0};
     MG_TRY(smem_limit_once(kern, kTableSmemMax, done));
-    const TeamPart p = plan(NT, rows, actions, NT == 32 ? 1 : row_parts(rows, actions, sizeof(T), NT, true), c.history_max);
+    const TeamPart p = plan(NT, rows, actions, NT == 32 ? 1 : row_parts(rows, actions, sizeof(T), WITH != 0, true), c.history_max);
     return launch_rows<NT>(kern, p, st, "k_logits_loss", static_cast<const T*>(logits), ld, c, static_cast<T*>(d), ldd, p, L);
 }
 
@@ -926,7 +952,7 @@ template <class T>
 int loss(const void* logits, int64_t ld, const mg_logit_controls& c, void* d, int64_t ldd, int rows, int actions,
          const LossArgs& L, cudaStream_t st) {
     auto f = launch_loss<T, 32, 3>;
-    if (!warp_teams(rows, actions, c.history_max, true)) {
+    if (!warp_teams(kCallLoss, rows, actions, c.history_max)) {
         switch (needed_controls(c, true)) {
             case 0: f = launch_loss<T, 256, 0>; break;
             case 1: f = launch_loss<T, 256, 1>; break;

@@ -4,8 +4,8 @@
 //   X0 = U / |U|_F;  G = X X^T (rows <= cols) or X^T X;  B = b G + c G^2;
 //   X <- a X + B X (or X B),  (a, b, c) = (3.4445, -4.7750, 2.0315),
 //
-// the quintic iteration and optimiser that K. Jordan et al. published ("Muon:
-// an optimizer for hidden layers", 2024).
+// the quintic iteration and optimiser that K. Jordan et al. published ("Muon: An
+// optimizer for hidden layers in neural networks", 2024).
 //
 // Number formats: the operands of the products are sums of two fp16 numbers
 // (22 significant bits), scaled by 2^10 so that entries from 2^-24 of |U| up

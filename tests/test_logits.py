@@ -633,26 +633,36 @@ def test_many_rows(mg, monkeypatch, rows, actions, pad, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("history", [490, 492])
-@pytest.mark.parametrize("rows,actions", [(640, 1100), (2300, 1100)])
+@pytest.mark.parametrize("rows,actions,history", [(640, 1100, 90), (640, 1100, 700), (2800, 2000, 1240), (2800, 2000, 1244), (300, 200, 64), (300, 200, 65)])
 def test_tables_of_many_rows(mg, monkeypatch, rows, actions, history):
-    """Histories on both sides of the 40 KB that the eight tables of a CTA of warp teams may take (491 entries at 1100
-    actions), under every combination of penalties, for the calls whose rows are then a warp's or a CTA's."""
+    """History tables on both sides of what sends rows to warps or CTAs: their size (100 KB for the eight of a CTA of warp
+    teams: 1242 entries at 2000 actions) and their length for the rows, under every combination of penalties."""
     made = make_controls
 
     def longer(rng, rows, actions, kinds):
         c = made(rng, rows, actions, kinds)
         if "history" in c:
             c["history"] = rng.integers(-3, actions + 3, (rows, history)).astype(np.int32)
-            c["history_len"] = rng.integers(history - 9, history + 9, rows).astype(np.int32)
+            c["history_len"] = rng.integers(-2, 40, rows).astype(np.int32)
+            c["history_len"][:3] = history
         return c
 
     monkeypatch.setitem(globals(), "make_controls", longer)
     monkeypatch.setitem(globals(), "KINDS", KINDS[3:])
     test_control_and_gradient(mg, rows, actions, 3, "bf16")
     test_sample(mg, rows, actions, 3, "bf16")
-    if rows > 2 * actions:
-        test_policy_loss(mg, rows, actions, 3, "bf16")
+    test_policy_loss(mg, rows, actions, 3, "bf16")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,actions,pad", [(40, 20000, 3), (9, 8200, 1), (2, 262144, 0), (760, 33000, 1)])
+def test_rows_in_parts(mg, monkeypatch, rows, actions, pad):
+    """Rows of two, four and eight parts, and of two because they would not stay in L2."""
+    monkeypatch.setitem(globals(), "KINDS", [KINDS[0], KINDS[3]])
+    kind = "f32" if rows == 760 else "bf16"
+    if rows < 760:
+        test_sample(mg, rows, actions, pad, kind)
+    test_policy_loss(mg, rows, actions, pad, kind)
 
 
 @pytest.mark.gpu
