@@ -456,14 +456,15 @@ int mg_muon_workspace(int batch, int rows, int cols, size_t* bytes);
  * |x|_F, then G = X X^T (or X^T X, the smaller), X = 3.4445 X + (-4.7750 G +
  * 2.0315 G^2) X, which takes singular values into about [0.7, 1.2]; 5 steps
  * do for the Muon update (iteration, coefficients and update as K. Jordan et
- * al. published them: "Muon: An optimizer for hidden layers in neural networks", 2024). x [batch][rows][ld] of `dtype`, batch_stride
- * elements apart; out likewise with ldo, out_stride, of out_dtype
- * MG_DTYPE_BF16 or MG_DTYPE_F16: the products take operands of 22 bits (two
- * fp16 numbers), X stays fp32. Measured off the exact iteration, of the result's
- * norm: 2e-6 to 5e-5; where the smaller side is at most 128 and steps at most 6,
- * 6e-6 at full rank, up to 3e-4 at rank 8 and 3e-3 at rank 1. A zero
- * matrix gives zeros. x and out must not overlap. workspace: device memory of
- * mg_muon_workspace bytes, 16-byte aligned. */
+ * al. published them: "Muon: An optimizer for hidden layers in neural
+ * networks", 2024). x [batch][rows][ld] of `dtype`, batch_stride elements
+ * apart; out likewise with ldo, out_stride, of out_dtype MG_DTYPE_BF16 or
+ * MG_DTYPE_F16. The products take operands of 22 bits (two fp16 numbers), X
+ * stays fp32. Measured off the exact iteration, of the result's norm: 2e-6 to
+ * 5e-5; where the smaller side is at most 128 and steps at most 6, 6e-6 at full
+ * rank, up to 3e-4 at rank 8 and 3e-3 at rank 1. A zero matrix gives zeros. x
+ * and out must not overlap. workspace: device memory of mg_muon_workspace
+ * bytes, 16-byte aligned. */
 int mg_orthogonalize(const void* x, int dtype, int64_t ld, int64_t batch_stride, void* out, int out_dtype, int64_t ldo,
                      int64_t out_stride, int batch, int rows, int cols, int steps, void* workspace,
                      size_t workspace_bytes, mg_stream_t stream);
