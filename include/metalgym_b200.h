@@ -421,7 +421,8 @@ int mg_logits_control_backward(const void* logits, int dtype, int64_t ld, const 
  * threads. rng NULL: the largest controlled logit. Equal ones: the lowest
  * index. A row without an allowed action of a logit above -inf gets action
  * -1, log-probability 0 and entropy 0. A NaN or +infinity at an allowed action makes the row's
- * log-probability and entropy NaN; a NaN is never drawn. */
+ * log-probability and entropy NaN; a NaN is never drawn, and the first of the
+ * +infinities always is. */
 int mg_logits_sample(const void* logits, int dtype, int64_t ld, const mg_logit_controls* controls, uint32_t* rng,
                      int32_t* action, float* log_prob, float* entropy, float* value, int rows, int actions,
                      mg_stream_t stream);

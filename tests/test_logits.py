@@ -633,7 +633,8 @@ def test_many_rows(mg, monkeypatch, rows, actions, pad, kind):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,actions,history", [(640, 1100, 90), (640, 1100, 700), (2800, 2000, 1240), (2800, 2000, 1244), (300, 200, 64), (300, 200, 65)])
+@pytest.mark.parametrize("rows,actions,history", [(640, 1100, 90), (640, 1100, 700), (2800, 2000, 1240), (2800, 2000, 1244), (300, 200, 64), (300, 200, 65),
+                                                  (3, 1, 90), (5, 6, 300), (8, 33, 2000)])
 def test_tables_of_many_rows(mg, monkeypatch, rows, actions, history):
     """History tables on both sides of what sends rows to warps or CTAs: their size (100 KB for the eight of a CTA of warp
     teams: 1242 entries at 2000 actions) and their length for the rows, under every combination of penalties."""
