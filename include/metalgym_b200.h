@@ -448,9 +448,7 @@ int mg_logits_policy_loss(const void* logits, int dtype, int64_t ld, const mg_lo
 /* Bytes of the workspace that mg_orthogonalize and mg_muon_step need for
  * `batch` matrices of rows x cols. One workspace serves one call at a time:
  * calls that may overlap on the GPU (two streams, two captured graphs) need
- * one each. Matrices whose smaller side is at most 128 are done without it in up
- * to 6 steps; the calls ask for it all the same, since the size goes by the
- * shape alone. */
+ * one each. */
 int mg_muon_workspace(int batch, int rows, int cols, size_t* bytes);
 /* out = the matrix of x brought near the closest matrix with orthonormal rows
  * (rows <= cols) or columns, by `steps` (1..16) Newton-Schulz steps: X = x /
@@ -461,11 +459,11 @@ int mg_muon_workspace(int batch, int rows, int cols, size_t* bytes);
  * networks", 2024). x [batch][rows][ld] of `dtype`, batch_stride elements
  * apart; out likewise with ldo, out_stride, of out_dtype MG_DTYPE_BF16 or
  * MG_DTYPE_F16. The products take operands of 22 bits (two fp16 numbers), X
- * stays fp32. Measured off the exact iteration, of the result's norm: 2e-6 to
- * 5e-5; where the smaller side is at most 128 and steps at most 6, 6e-6 at full
- * rank, up to 3e-4 at rank 8 and 3e-3 at rank 1. A zero matrix gives zeros. x
- * and out must not overlap. workspace: device memory of mg_muon_workspace
- * bytes, 16-byte aligned. */
+ * stays fp32. Measured off the exact iteration in 5 steps, of the result's
+ * norm: 2e-6 to 5e-5, and up to 2e-4 at rank 1 or 2, as iterations of fp32
+ * products are (a step multiplies by 3.4 what they are off in the directions
+ * that x hardly has). A zero matrix gives zeros. x and out must not overlap.
+ * workspace: device memory of mg_muon_workspace bytes, 16-byte aligned. */
 int mg_orthogonalize(const void* x, int dtype, int64_t ld, int64_t batch_stride, void* out, int out_dtype, int64_t ldo,
                      int64_t out_stride, int batch, int rows, int cols, int steps, void* workspace,
                      size_t workspace_bytes, mg_stream_t stream);

@@ -331,7 +331,7 @@ bool small_enough(int rows, int cols, int steps) {
 }
 
 template <int SP, bool WIDE, class T, bool MUON>
-int launch_small(const MuonInput& in, const NsProduct& p, int steps, bool vec, cudaStream_t st) {
+int launch_small(const MuonInput& in, const NsProduct& p, float* x32, int steps, bool vec, cudaStream_t st) {
     auto kern = k_muon_small<SP, WIDE, T, MUON>;
     static std::atomic<uint64_t> done{0};
     MG_TRY(smem_limit_once(kern, MuonSmall::SMEM_BYTES, done));
@@ -353,12 +353,12 @@ int launch_small(const MuonInput& in, const NsProduct& p, int steps, bool vec, c
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = parts > 1 ? 2 : 1;
-    MG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, in, p, steps, vec ? 1 : 0, parts));
+    MG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, in, p, x32, steps, vec ? 1 : 0, parts));
     return check_launch("k_muon_small");
 }
 
 template <class T, bool MUON>
-int run_small(const MuonInput& in, const NsFinal& fin, int batch, int rows, int cols, int steps, bool vec, cudaStream_t st) {
+int run_small(const MuonInput& in, const Workspace& w, const NsFinal& fin, int batch, int rows, int cols, int steps, bool vec, cudaStream_t st) {
     NsProduct p{};
     p.M = rows;
     p.N = cols;
@@ -369,8 +369,8 @@ int run_small(const MuonInput& in, const NsFinal& fin, int batch, int rows, int 
     p.status = status_ptr();
     const bool narrow = std::min(rows, cols) <= 64;
     if (rows <= cols)
-        return narrow ? launch_small<64, true, T, MUON>(in, p, steps, vec, st) : launch_small<128, true, T, MUON>(in, p, steps, vec, st);
-    return narrow ? launch_small<64, false, T, MUON>(in, p, steps, vec, st) : launch_small<128, false, T, MUON>(in, p, steps, vec, st);
+        return narrow ? launch_small<64, true, T, MUON>(in, p, w.x32, steps, vec, st) : launch_small<128, true, T, MUON>(in, p, w.x32, steps, vec, st);
+    return narrow ? launch_small<64, false, T, MUON>(in, p, w.x32, steps, vec, st) : launch_small<128, false, T, MUON>(in, p, w.x32, steps, vec, st);
 }
 
 bool aligned_to(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % (unsigned)bytes) == 0; }
@@ -417,9 +417,9 @@ int mg_orthogonalize(const void* x, int dtype, int64_t ld, int64_t batch_stride,
     if (small_enough(rows, cols, steps)) {
         const int per = dtype == MG_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
         const bool vec = ld % per == 0 && batch_stride % per == 0 && aligned_to(x, 16);
-        if (dtype == MG_DTYPE_F32) return run_small<float, false>(in, fin, batch, rows, cols, steps, vec, st);
-        if (dtype == MG_DTYPE_BF16) return run_small<__nv_bfloat16, false>(in, fin, batch, rows, cols, steps, vec, st);
-        return run_small<__half, false>(in, fin, batch, rows, cols, steps, vec, st);
+        if (dtype == MG_DTYPE_F32) return run_small<float, false>(in, w, fin, batch, rows, cols, steps, vec, st);
+        if (dtype == MG_DTYPE_BF16) return run_small<__nv_bfloat16, false>(in, w, fin, batch, rows, cols, steps, vec, st);
+        return run_small<__half, false>(in, w, fin, batch, rows, cols, steps, vec, st);
     }
     int parts = 0;
     const bool vec = cols % 4 == 0 && ld % 4 == 0 && batch_stride % 4 == 0 && aligned_to(x, dtype == MG_DTYPE_F32 ? 16 : 8);
@@ -469,7 +469,7 @@ int mg_muon_step(float* master, const float* grad, float* momentum, void* weight
     fin.vec = cols % 4 == 0 && batch_stride % 4 == 0 && aligned_to(master, 16) && aligned_to(weights, 8);
     fin.keep = 1.0f - lr * weight_decay;
     fin.rate = lr * scale;
-    if (small_enough(rows, cols, steps)) return run_small<float, true>(in, fin, batch, rows, cols, steps, vec, st);
+    if (small_enough(rows, cols, steps)) return run_small<float, true>(in, w, fin, batch, rows, cols, steps, vec, st);
     int parts = 0;
     MG_TRY((prepare<float, true>(in, w, batch, rows, cols, vec, &parts, st)));
     return newton_schulz(w, batch, rows, cols, steps, parts, fin, st);

@@ -3,19 +3,22 @@
 //
 // The Newton-Schulz steps only multiply X by polynomials of G = X X^T, which
 // commute: with Q = a I + b G + c G^2 the next X is Q X and the next G is Q G Q.
-// So the long side is passed twice, for G and for the result P X with P the
-// product of the Qs, and the steps in between take s x s matrices alone, held
-// in shared memory by every CTA of the cluster (the same operations on the
-// same bits in each). 17 launches that each wait for the one before took 117 us
-// at 2 x 128 x 512.
+// So the long side is passed twice in a run of up to three steps, for G and for
+// P X with P the product of the Qs, and the steps in between take s x s matrices
+// alone, held in shared memory by every CTA of the cluster (the same operations
+// on the same bits in each). 17 launches that each wait for the one before took
+// 117 us at 2 x 128 x 512 with operands of one part.
 //
-// Precision: P grows to a^steps in directions that U hardly has, so that the
-// rounding of P, G or X to 16 bits would show in the others. Every operand is
-// the sum of two fp16 numbers (22 bits), every product three tcgen05 products:
-// 6e-6 of the result's norm off the exact iteration at full rank, 3e-4 at rank
-// 8 of 128 and 3e-3 at rank 1, where the cuts of the accumulator are as large as
-// P's largest directions make them. P is scaled by 2^5, the others by 2^10:
-// within fp16's range for up to six steps (3.4445^6 2^5 < 2^16).
+// Precision: every operand is the sum of two fp16 numbers (22 bits), every
+// product three tcgen05 products. P grows to a^k in directions that U hardly
+// has, and what G is off there by a^2 in every step, since no X checks it: after
+// three steps X is written out (or kept in tensor memory by a CTA of one piece)
+// and G taken from it anew. Off the exact iteration, of the result's norm, at 128
+// x 512 in five and six steps: 1.2e-4 and 1.9e-4 at rank 1, 3e-5 and 1e-4 at rank
+// 8 (fp32 products by a library 1.0e-4 and 2.2e-4, 2e-5 and 1e-4); all steps in
+// one run 2.6e-3 and 2.1e-2, 3.2e-4 and 3.5e-3 (a step of 2 x 128 x 512 in 47 us
+// of GPU time instead of 57, 128 x 4096 in 69 instead of 106). P is scaled by 2^5,
+// the others by 2^10.
 #pragma once
 
 #include "logits.cuh"
@@ -37,7 +40,7 @@ struct MuonInput {
     float* normSqOut;
 };
 
-constexpr int kMuonSmallSide = 128, kMuonSmallSteps = 6, kMuonSmallThreads = 512;
+constexpr int kMuonSmallSide = 128, kMuonSmallRun = 3, kMuonSmallSteps = 2 * kMuonSmallRun, kMuonSmallThreads = 512;
 constexpr int kMuonSmallCluster = 8;
 constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
 
@@ -212,10 +215,32 @@ __device__ __forceinline__ void tmem_load(uint32_t taddr, float* v) {
     }
 }
 
-// SP: the smaller side padded, 64 or 128. WIDE: rows <= cols.
+// A 32 x 32 piece of X at (row0, col0) of matrix b into x [batch][M][ldo], from
+// an accumulator scaled by 2^20 (lane r holds row r in v).
+__device__ __forceinline__ void ns_keep(const NsProduct& p, float* x, int b, int row0, int col0, uint8_t* slab, const float* v) {
+    const int lane = threadIdx.x & 31, k = lane & 7, col = col0 + 4 * k;
+    constexpr float kScale = kNsUnscale * kNsUnscale;
+    __syncwarp();  // the slab's last readers are done
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        *reinterpret_cast<float4*>(slab + ns_slab_offset(lane, i)) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    __syncwarp();
+    if (col >= p.N) return;  // (the four columns lie inside ldo)
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int r = 4 * i + (lane >> 3), row = row0 + r;
+        const float4 y = *reinterpret_cast<const float4*>(slab + ns_slab_offset(r, k));
+        if (row < p.M)
+            *reinterpret_cast<float4*>(x + ((int64_t)b * p.M + row) * p.ldo + col) =
+                make_float4(y.x * kScale, y.y * kScale, y.z * kScale, y.w * kScale);
+    }
+}
+
+// SP: the smaller side padded, 64 or 128. WIDE: rows <= cols. x32: X between two
+// runs of steps, [batch][rows][ldo].
 template <int SP, bool WIDE, class T, bool MUON>
 __global__ void __launch_bounds__(kMuonSmallThreads, 1)
-    k_muon_small(const MuonInput in, const NsProduct p, int steps, int vec, int parts) {
+    k_muon_small(const MuonInput in, const NsProduct p, float* x32, int steps, int vec, int parts) {
     using S = MuonSmall;
     constexpr int KS = SP / 16, COLS = SP / 4;  // COLS: columns of an s x s matrix that a thread holds
     constexpr int WARPS = kMuonSmallThreads / 32;
@@ -237,7 +262,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
         fence_barrier_init();
     }
     if (warp == 2) {
-        tmem_alloc(tmem_slot, 256);
+        tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
     tc_fence_before();
@@ -274,10 +299,18 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
     // this CTA's pieces of 128 along the long side
     const int pieces = (l + 127) / 128, first = (int)((int64_t)pieces * rank / parts), end = (int)((int64_t)pieces * (rank + 1) / parts);
     // eight columns of U: cell g (16 to a tile row) of piece i, zeros outside the matrix
+    MuonInput kept{};  // X after a run
+    kept.x = x32;
+    kept.ld = p.ldo;
+    kept.stride = (int64_t)rows * p.ldo;
+    bool again = false;
     auto cell = [&](int i, int g, bool update, float* u) {
         const int r = (g >> 4) + (WIDE ? 0 : 128 * i), c = 8 * (g & 15) + (WIDE ? 128 * i : 0);
         if (r < rows && c < cols) {
-            muon_load8<T, MUON>(in, b, r, c, cols, vec != 0, update, scale, u);
+            if (again)
+                muon_load8<float, false>(kept, b, r, c, cols, true, false, 1.0f, u);
+            else
+                muon_load8<T, MUON>(in, b, r, c, cols, vec != 0, update, scale, u);
         } else {
 #pragma unroll
             for (int k = 0; k < 8; k++) u[k] = 0.0f;
@@ -316,7 +349,7 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
         __syncthreads();
         sum = *sNorm;
     }
-    const InverseNorm inv(sum);
+    InverseNorm inv(sum);
     // the piece of X in `held` into a tile; piece `next` is loaded behind it
     auto load = [&](int i) {
 #pragma unroll
@@ -335,188 +368,226 @@ __global__ void __launch_bounds__(kMuonSmallThreads, 1)
         handOver();
     };
 
-    // G's part from this CTA's pieces, the tiles alternating between two places
-    for (int i = first; i < end; i++) {
-        const int k = (i - first) & 1;
-        uint8_t* mat = k ? mP : mQ;
-        if (i - first >= 2) wait(k);
-        tile(mat, i + 1);
-        if (tid == 0) {
-            split_mma<!WIDE, !WIDE, SP, 8>(tmem, smem_u32(mat), smem_u32(mat), i > first);
-            tc_commit(&bar[k]);
-        }
-    }
-    if (end - first >= 2) wait((end - first) & 1);
-    if (end > first) wait((end - first - 1) & 1);
     const int q = warp & 3, row = 32 * q + lane, c0 = (warp >> 2) * COLS;
     const uint32_t acc = tmem + ((uint32_t)(32 * q) << 16);
     const bool holds = 32 * q < SP;  // warps 2 and 3 of four have no rows of a 64-row matrix
-    if (holds) {
-        float v[COLS];
-        if (end > first) {
-            tmem_load<COLS>(acc + (uint32_t)c0, v);
-        } else {
-#pragma unroll
-            for (int k = 0; k < COLS; k++) v[k] = 0.0f;
-        }
-#pragma unroll
-        for (int k = 0; k < COLS / 4; k++)
-            *reinterpret_cast<float4*>(mG + tile_offset(row, c0 / 4 + k)) =
-                make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-    }
-    if (parts > 1) {
-        // CTA k sums rows k SP / parts .. of all parts, in their order, and hands
-        // them back to all: nobody else reads or writes those rows meanwhile
-        __syncwarp();
-        cluster_sync();
-        const int mine = SP / parts;
-        for (int j = tid; j < mine * SP / 4; j += kMuonSmallThreads) {
-            const uint32_t off = tile_offset(rank * mine + j / (SP / 4), j % (SP / 4));
-            float4 v[kMuonSmallCluster], t;
-#pragma unroll
-            for (int k = 0; k < kMuonSmallCluster; k++)
-                if (k < parts) v[k] = *reinterpret_cast<const float4*>(cluster_peer(mG, k) + off);
-            t = v[0];
-#pragma unroll
-            for (int k = 1; k < kMuonSmallCluster; k++)
-                if (k < parts) {
-                    t.x += v[k].x;
-                    t.y += v[k].y;
-                    t.z += v[k].z;
-                    t.w += v[k].w;
-                }
-#pragma unroll
-            for (int k = 0; k < kMuonSmallCluster; k++)
-                if (k < parts) *reinterpret_cast<float4*>(const_cast<uint8_t*>(cluster_peer(mG, k)) + off) = t;
-        }
-        __syncwarp();
-        cluster_sync();
-    } else {
-        __syncthreads();
-    }
-    // G in two parts, over the fp32 tile (each thread takes its values out first)
+    const uint32_t aG = smem_u32(mG), aQ = smem_u32(mQ), aP = smem_u32(mP);
     constexpr float kAcc = kNsUnscale * kNsUnscale;  // of a product of two matrices scaled by 2^10
-    {
-        float g[COLS];
+    constexpr int N = WIDE ? 128 : SP;                // columns of a piece of P X
+    const int cX = 32 * (warp >> 2);
+    const bool holdsX = cX < N && (!WIDE || holds);
+    // X of the run before into a tile, out of columns 256 .. of tensor memory, where a CTA of one piece keeps it
+    auto retile = [&](uint8_t* mat) {
+        if (holdsX) {
+            float v[32];
+            tmem_ld32(acc + (uint32_t)(256 + cX), v);
+#pragma unroll
+            for (int k = 0; k < 32; k++) v[k] *= 0.03125f;  // (scaled by 2^15 there)
+#pragma unroll
+            for (int k = 0; k < 4; k++) split_store8(mat, sw128_offset(row, cX / 8 + k), v + 8 * k);
+        }
+        handOver();
+    };
+#pragma unroll 1
+    for (;;) {
+        const int run = min(steps, kMuonSmallRun);
+        // G's part from this CTA's pieces, the tiles alternating between two places
+        const bool resident = again && end - first == 1;
+        for (int i = first; i < end; i++) {
+            const int k = (i - first) & 1;
+            uint8_t* mat = k ? mP : mQ;
+            if (i - first >= 2) wait(k);
+            if (resident)
+                retile(mat);
+            else
+                tile(mat, i + 1);
+            if (tid == 0) {
+                split_mma<!WIDE, !WIDE, SP, 8>(tmem, smem_u32(mat), smem_u32(mat), i > first);
+                tc_commit(&bar[k]);
+            }
+        }
+        if (end - first >= 2) wait((end - first) & 1);
+        if (end > first) wait((end - first - 1) & 1);
         if (holds) {
+            float v[COLS];
+            if (end > first) {
+                tmem_load<COLS>(acc + (uint32_t)c0, v);
+            } else {
+#pragma unroll
+                for (int k = 0; k < COLS; k++) v[k] = 0.0f;
+            }
 #pragma unroll
             for (int k = 0; k < COLS / 4; k++)
-                *reinterpret_cast<float4*>(g + 4 * k) = *reinterpret_cast<const float4*>(mG + tile_offset(row, c0 / 4 + k));
+                *reinterpret_cast<float4*>(mG + tile_offset(row, c0 / 4 + k)) =
+                    make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
         }
-        __syncthreads();
-        if (holds) {
+        if (parts > 1) {
+            // CTA k sums rows k SP / parts .. of all parts, in their order, and hands
+            // them back to all: nobody else reads or writes those rows meanwhile
+            __syncwarp();
+            cluster_sync();
+            const int mine = SP / parts;
+            for (int j = tid; j < mine * SP / 4; j += kMuonSmallThreads) {
+                const uint32_t off = tile_offset(rank * mine + j / (SP / 4), j % (SP / 4));
+                float4 v[kMuonSmallCluster], t;
 #pragma unroll
-            for (int k = 0; k < COLS; k++) g[k] *= kAcc * kNsScale;
+                for (int k = 0; k < kMuonSmallCluster; k++)
+                    if (k < parts) v[k] = *reinterpret_cast<const float4*>(cluster_peer(mG, k) + off);
+                t = v[0];
 #pragma unroll
-            for (int k = 0; k < COLS / 8; k++) split_store8(mG, sw128_offset(row, c0 / 8 + k), g + 8 * k);
+                for (int k = 1; k < kMuonSmallCluster; k++)
+                    if (k < parts) {
+                        t.x += v[k].x;
+                        t.y += v[k].y;
+                        t.z += v[k].z;
+                        t.w += v[k].w;
+                    }
+#pragma unroll
+                for (int k = 0; k < kMuonSmallCluster; k++)
+                    if (k < parts) *reinterpret_cast<float4*>(const_cast<uint8_t*>(cluster_peer(mG, k)) + off) = t;
+            }
+            __syncwarp();
+            cluster_sync();
+        } else {
+            __syncthreads();
         }
-    }
-    handOver();
-
-    // the steps
-    const uint32_t aG = smem_u32(mG), aQ = smem_u32(mQ), aP = smem_u32(mP);
-    // an accumulator, scaled by 2^10 more than the matrix, into the matrix
-    auto take = [&](uint32_t column, uint8_t* mat) {
-        if (!holds) return;
-        float v[COLS];
-        tmem_load<COLS>(acc + column + (uint32_t)c0, v);
+        // G in two parts, over the fp32 tile (each thread takes its values out first)
+        {
+            float g[COLS];
+            if (holds) {
 #pragma unroll
-        for (int k = 0; k < COLS; k++) v[k] *= kNsUnscale;
+                for (int k = 0; k < COLS / 4; k++)
+                    *reinterpret_cast<float4*>(g + 4 * k) = *reinterpret_cast<const float4*>(mG + tile_offset(row, c0 / 4 + k));
+            }
+            __syncthreads();
+            if (holds) {
 #pragma unroll
-        for (int k = 0; k < COLS / 8; k++) split_store8(mat, sw128_offset(row, c0 / 8 + k), v + 8 * k);
-    };
-    auto multiply = [&](uint32_t column, uint32_t x, uint32_t y, int bit) {
-        if (tid == 0) {
-            split_mma<false, false, SP, KS>(tmem + column, x, y, false);
-            tc_commit(&bar[bit]);
-        }
-    };
-    // P's products run behind those that the next G waits for, and are taken up
-    // while the next product runs.
-    for (int step = 0; step < steps; step++) {
-        const bool more = step + 1 < steps;
-        multiply(0, aG, aG, 0);
-        wait(0);
-        if (holds) {  // Q = a I + b G + c G^2
-            float v[COLS];
-            tmem_load<COLS>(acc + (uint32_t)c0, v);
+                for (int k = 0; k < COLS; k++) g[k] *= kAcc * kNsScale;
 #pragma unroll
-            for (int k = 0; k < COLS / 8; k++) {
-                float g[8];
-                split_load8(mG, sw128_offset(row, c0 / 8 + k), g);
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    float y = fmaf(kNsC * kNsUnscale, v[8 * k + i], kNsB * g[i]);  // times 2^10
-                    if (c0 + 8 * k + i == row && row < s) y += kNsA * kNsScale;
-                    g[i] = y;
-                }
-                split_store8(mQ, sw128_offset(row, c0 / 8 + k), g);
-                if (step == 0) {  // P = Q, scaled by 2^5 throughout
-#pragma unroll
-                    for (int i = 0; i < 8; i++) g[i] *= 0.03125f;
-                    split_store8(mP, sw128_offset(row, c0 / 8 + k), g);
-                }
+                for (int k = 0; k < COLS / 8; k++) split_store8(mG, sw128_offset(row, c0 / 8 + k), g + 8 * k);
             }
         }
         handOver();
-        if (more) multiply(0, aQ, aG, 0);
-        if (step > 0) multiply(128, aQ, aP, 1);
-        if (more) {
-            wait(0);
-            take(0, mG);  // Q G, in G's place
-            handOver();
-            multiply(0, aQ, aG, 0);
-        }
-        if (step > 0) {
-            wait(1);
-            take(128, mP);
-        }
-        if (more) {
-            wait(0);
-            take(0, mG);  // Q G Q
-        }
-        handOver();
-    }
 
-    // P X, piece by piece: the next piece's product beside this one's epilogue. The
-    // tiles take G's place, the epilogue's slabs Q's.
-    constexpr int N = WIDE ? 128 : SP;
-    uint8_t* slab = mQ + warp * 4096;
-    auto issue = [&](int i) {
-        const int k = (i - first) & 1;
-        tile(mG, i + 1);
-        if (tid == 0) {
-            if (WIDE)
-                split_mma<false, true, N, KS>(tmem + 128 * k, aP, aG, false);
-            else
-                split_mma<false, false, N, KS>(tmem + 128 * k, aG, aP, false);
-            tc_commit(&bar[k]);
-        }
-    };
-    if (first < end) {
-        load(first);
-        issue(first);
-    }
-    for (int i = first; i < end; i++) {
-        const int k = (i - first) & 1;
-        wait(k);
-        if (i + 1 < end) issue(i + 1);
-        const int row0 = 32 * q + (WIDE ? 0 : 128 * i), c = 32 * (warp >> 2), col0 = c + (WIDE ? 128 * i : 0);
-        if (row0 < rows && c < N && col0 < cols && (!WIDE || 32 * q < SP)) {
-            float v[32];
-            __syncwarp();  // the first warp's lane 0 issued the next product
-            tmem_ld32(acc + (uint32_t)(128 * k + c), v);
+        // the steps
+        // an accumulator, scaled by 2^10 more than the matrix, into the matrix
+        auto take = [&](uint32_t column, uint8_t* mat) {
+            if (!holds) return;
+            float v[COLS];
+            tmem_load<COLS>(acc + column + (uint32_t)c0, v);
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] *= 32.0f;  // to the scale of ns_piece, 2^20
-            ns_piece<kNsApply>(p, b, row0, col0, slab, v, NsFetched<kNsApply>{});
+            for (int k = 0; k < COLS; k++) v[k] *= kNsUnscale;
+#pragma unroll
+            for (int k = 0; k < COLS / 8; k++) split_store8(mat, sw128_offset(row, c0 / 8 + k), v + 8 * k);
+        };
+        auto multiply = [&](uint32_t column, uint32_t x, uint32_t y, int bit) {
+            if (tid == 0) {
+                split_mma<false, false, SP, KS>(tmem + column, x, y, false);
+                tc_commit(&bar[bit]);
+            }
+        };
+        // P's products run behind those that the next G waits for, and are taken up
+        // while the next product runs.
+        for (int step = 0; step < run; step++) {
+            const bool more = step + 1 < run;
+            multiply(0, aG, aG, 0);
+            wait(0);
+            if (holds) {  // Q = a I + b G + c G^2
+                float v[COLS];
+                tmem_load<COLS>(acc + (uint32_t)c0, v);
+#pragma unroll
+                for (int k = 0; k < COLS / 8; k++) {
+                    float g[8];
+                    split_load8(mG, sw128_offset(row, c0 / 8 + k), g);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        float y = fmaf(kNsC * kNsUnscale, v[8 * k + i], kNsB * g[i]);  // times 2^10
+                        if (c0 + 8 * k + i == row && row < s) y += kNsA * kNsScale;
+                        g[i] = y;
+                    }
+                    split_store8(mQ, sw128_offset(row, c0 / 8 + k), g);
+                    if (step == 0) {  // P = Q, scaled by 2^5 throughout
+#pragma unroll
+                        for (int i = 0; i < 8; i++) g[i] *= 0.03125f;
+                        split_store8(mP, sw128_offset(row, c0 / 8 + k), g);
+                    }
+                }
+            }
+            handOver();
+            if (more) multiply(0, aQ, aG, 0);
+            if (step > 0) multiply(128, aQ, aP, 1);
+            if (more) {
+                wait(0);
+                take(0, mG);  // Q G, in G's place
+                handOver();
+                multiply(0, aQ, aG, 0);
+            }
+            if (step > 0) {
+                wait(1);
+                take(128, mP);
+            }
+            if (more) {
+                wait(0);
+                take(0, mG);  // Q G Q
+            }
+            handOver();
         }
+
+        // P X, piece by piece: the next piece's product beside this one's epilogue. The
+        // tiles take G's place, the epilogue's slabs Q's.
+        uint8_t* slab = mQ + warp * 4096;
+        const bool keep = steps > run && end - first == 1;
+        auto issue = [&](int i) {
+            const int k = (i - first) & 1;
+            if (resident)
+                retile(mG);
+            else
+                tile(mG, i + 1);
+            if (tid == 0) {
+                const uint32_t d = tmem + (keep ? 256 : 128 * k);
+                if (WIDE)
+                    split_mma<false, true, N, KS>(d, aP, aG, false);
+                else
+                    split_mma<false, false, N, KS>(d, aG, aP, false);
+                tc_commit(&bar[k]);
+            }
+        };
+        if (first < end) {
+            if (!resident) load(first);
+            issue(first);
+        }
+        for (int i = first; i < end; i++) {
+            const int k = (i - first) & 1;
+            wait(k);
+            if (keep) break;
+            if (i + 1 < end) issue(i + 1);
+            const int row0 = 32 * q + (WIDE ? 0 : 128 * i), col0 = cX + (WIDE ? 128 * i : 0);
+            if (holdsX && row0 < rows && col0 < cols) {
+                float v[32];
+                __syncwarp();  // the first warp's lane 0 issued the next product
+                tmem_ld32(acc + (uint32_t)(128 * k + cX), v);
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] *= 32.0f;  // to the scale of ns_piece, 2^20
+                if (steps > run)
+                    ns_keep(p, x32, b, row0, col0, slab, v);
+                else
+                    ns_piece<kNsApply>(p, b, row0, col0, slab, v, NsFetched<kNsApply>{});
+            }
+        }
+        steps -= run;
+        if (steps == 0) break;
+        // the next run: X from what this CTA wrote or kept, its slabs' place free
+        again = true;
+        inv.p = inv.q = inv.m = 1.0f;
+        __syncthreads();
+        if (end - first > 1) load(first);
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 2) {
         __syncwarp();
         tc_fence_after();
-        tmem_dealloc(tmem, 256);
+        tmem_dealloc(tmem, 512);
     }
 }
 

@@ -247,6 +247,59 @@ def test_larger_sides_are_as_exact_as_smaller_ones(mg, batch, m, n, spectrum):
         assert off <= 1.5 * (near - want).norm() + 2.0 ** -20 * want.norm(), float(off / want.norm())
 
 
+def newton_schulz_runs(u, steps, gen):
+    """The form that smaller sides up to 128 take, with the roundings and cuts of newton_schulz_parts: three steps at a time on
+    G = X X^T and P, the product of their polynomials of G; X between the runs in fp32."""
+    def h(v, scale=1024):
+        hi = (v * scale).half().double()
+        return (hi + (v * scale - hi).half().double()) / scale
+
+    def product(a, b):
+        p, n = a @ b, 3 * ((a.shape[1] + 15) // 16)
+        size = p.abs().clamp(min=float(p.norm()) / p.numel() ** 0.5)
+        return p * (1 - n * 2.0 ** -24) + 3 * n ** 0.5 * 2.0 ** -24 * size * torch.randn(p.shape, generator=gen, device=p.device, dtype=p.dtype)
+
+    x = u.double() / u.double().norm()
+    flip = x.shape[0] > x.shape[1]
+    x = (x.t() if flip else x).float().double()
+    eye = torch.eye(x.shape[0], device=x.device, dtype=x.dtype)
+    while steps:
+        run = min(steps, 3)
+        g, total = h(product(h(x), h(x).t())), None
+        for step in range(run):
+            q = h(A * eye + B * g + C * product(g, g))
+            total = h(q if total is None else product(q, total.t()), 32)
+            if step + 1 < run:
+                g = h(product(q, h(product(q, g)).t()))
+        x = product(total, h(x)).float().double()
+        steps -= run
+    return x.t() if flip else x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps", [2, 3, 4, 5, 6])
+@pytest.mark.parametrize("rank", [1, 2, 8, 0])
+@pytest.mark.parametrize("batch,m,n", [(1, 16, 200), (2, 64, 512), (1, 128, 512), (3, 512, 128), (1, 100, 3000), (1, 1500, 60), (1, 128, 128)])
+def test_small_sides_of_any_rank_and_steps(mg, batch, m, n, rank, steps):
+    """Matrices of few directions (0: as many as the smaller side, badly conditioned): the update is off by at most twice the
+    distance of the emulated roundings and cuts and 2^-20 of it. (An emulation of one run of all the steps would allow 20
+    times that at five steps and 100 times at six: G and P grow apart by a^2 a step in the directions that are hardly there.)"""
+    gen = torch.Generator(device="cuda").manual_seed(batch + m + n + rank)
+    r = rank or min(m, n)
+    grad = torch.stack([torch.randn(m, r, generator=gen, device="cuda") @ torch.randn(r, n, generator=gen, device="cuda") for _ in range(batch)])
+    master, momentum = torch.zeros_like(grad), torch.zeros_like(grad)
+    weights = torch.zeros(batch, m, n, dtype=torch.bfloat16, device="cuda")
+    space = workspace(mg, batch, m, n)
+    ok(mg, mg.mg_muon_step(master.data_ptr(), grad.data_ptr(), momentum.data_ptr(), weights.data_ptr(), m * n, batch, m, n, None, 0, 0.0, -1.0,
+                           1.0, 0.0, 0, 0.0, steps, None, space.data_ptr(), space.numel(), None))
+    assert status(mg) == 0
+    for i in range(0, batch, max(1, batch - 1)):
+        want = newton_schulz(grad[i], steps, False)
+        near = newton_schulz_runs(grad[i], steps, gen)
+        off = (master[i].double() - want).norm()
+        assert off <= 2 * (near - want).norm() + 2.0 ** -20 * want.norm(), float(off / want.norm())
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("batch,m,n", [(1, 130, 300), (1, 333, 1001), (40, 161, 200), (3, 200, 1100), (1, 1030, 1500), (2, 129, 133), (1, 100, 700)])
 def test_pieces_that_end_inside_a_warp(mg, batch, m, n):
