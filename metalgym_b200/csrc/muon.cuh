@@ -74,6 +74,7 @@ struct NsTile {
     static constexpr int SLAB_OFF = STAGES * STAGE_BYTES, BAR_OFF = SLAB_OFF + EW * SLAB;
     static constexpr int TMEM_COLS = 2 * BN;
     static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024 /*align*/;
+    static_assert(SMEM_BYTES > 225 * 1024, "no other CTA that holds tensor memory beside it (as in MuonSmall)");
 };
 
 // Instruction descriptor, kind::f16: fp16 A and B, fp32 accumulator, M = 128.

@@ -47,7 +47,11 @@ constexpr float kNsA = 3.4445f, kNsB = -4.7750f, kNsC = 2.0315f;
 struct MuonSmall {
     static constexpr int MAT = 65536;  // a matrix's or a tile's two fp16 parts
     static constexpr int BAR_OFF = 3 * MAT;
-    static constexpr int SMEM_BYTES = BAR_OFF + 256 + 1024 /*align*/;
+    // All that a CTA can have, more than the 198 KB in use: a CTA waits for its
+    // tensor memory without a limit, and its cluster for it. Beside another kernel's
+    // clusters that hold tensor memory the two could wait for each other.
+    static constexpr int SMEM_BYTES = 227 * 1024;
+    static_assert(BAR_OFF + 256 + 1024 /*align*/ <= SMEM_BYTES, "the matrices, barriers and sums");
 };
 
 // The sum of N squares. 64-bit conversions run at 16 a cycle and SM, so that
